@@ -15,7 +15,7 @@ for f in $ALL; do
   if [ -n "$ONLY" ] && [ "$f" != mtl_elementwise ] && ! echo ",$ONLY," | grep -q ",$f,"; then
     cp $R/build/obj/$f.o $OBJ/$f.o
   else
-    hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wall -Wno-unused-function "$@" -c $R/med-ts-llm_amd/csrc/$f.hip -o $OBJ/$f.o &
+    hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wall -Wno-unused-function -Xclang -target-feature -Xclang -packed-fp32-ops "$@" -c $R/med-ts-llm_amd/csrc/$f.hip -o $OBJ/$f.o &
   fi
 done
 wait
