@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define MTL_ABI_VERSION 15
+#define MTL_ABI_VERSION 16
 
 enum { MTL_OK = 0, MTL_ERR_ARG = -1, MTL_ERR_ALIGN = -2, MTL_ERR_UNSUPPORTED = -3, MTL_ERR_LAUNCH = -4,
        MTL_ERR_WORKSPACE = -5 };
@@ -231,6 +231,38 @@ typedef struct mtl_adam_tensor {
 int mtl_adam_step(const mtl_adam_tensor* tensors, int count, float lr, float beta1, float beta2, float eps,
                   float weight_decay, int decoupled, int64_t step, void* stream);
 
+/* The same step with both moments in 8 bits (csrc/mtl_optim8.hip states the formats): blocks of 64 consecutive elements of the flat tensor, e4m3 first moment,
+ * the root of the second as unsigned 4.4 numbers, one power-of-two exponent each per block. fp32: 16 B of traffic per element instead of 28, 2.03 B of state instead of 8.
+ * All arithmetic in fp32, one rounding per operation in a fixed order: the result is a function of the inputs and `step`, bit for bit, on any machine. The root is rounded
+ * against a threshold taken from (step, element index); a tensor updated in two pieces is therefore not the tensor updated in one.
+ * Hyper-parameters are doubles (1 - beta is formed before the rounding to fp32). All-zero codes and exponents are zero moments. */
+#define MTL_ADAM8_MAX_TENSORS 40   /* per launch: 40 x 80 B of kernel arguments */
+#define MTL_ADAM8_BLOCK 64
+typedef struct mtl_adam8_tensor {
+    void* p;
+    const void* g;
+    uint8_t* m8;         /* [n] */
+    uint8_t* r8;         /* [n] */
+    int8_t* ex;          /* [ceil(n / 64), 2]: exponents of m and r; 2-byte aligned */
+    int64_t n;
+    void* shadow;        /* bf16 or NULL, as in mtl_adam_tensor */
+    int64_t cols, ld_shadow;
+    int64_t param_dtype; /* MTL_F32 | MTL_BF16 (p and g) */
+} mtl_adam8_tensor;
+int mtl_adam8_step(const mtl_adam8_tensor* tensors, int count, double lr, double beta1, double beta2, double eps, double weight_decay, int decoupled, int64_t step,
+                   void* stream);
+typedef struct mtl_adam8_state {
+    uint8_t* m8;
+    uint8_t* r8;
+    int8_t* ex;
+    int64_t n;
+    void* m;             /* first / second moment: outputs of mtl_adam8_moments (either may be NULL), fp32 inputs of mtl_adam8_quantize */
+    void* v;
+    int64_t dtype;       /* of m and v */
+} mtl_adam8_state;
+int mtl_adam8_moments(const mtl_adam8_state* states, int count, void* stream);
+int mtl_adam8_quantize(const mtl_adam8_state* states, int count, int64_t step, void* stream);
+
 /* ------------------------------------------------------------------ attention (flash-style, never materialises scores)
  * O = softmax(scale * Q K^T [+ causal mask]) V per (batch, head); fp32 softmax statistics, bf16 I/O.
  * Replaces (a) the reprogramming cross-attention einsum/softmax/einsum (R:models/medtsllm.py:586-589;
@@ -420,6 +452,46 @@ int mtl_backbone_prefix_build(const mtl_backbone_weights* w, const void* h0_pref
 int mtl_backbone_bwd(const mtl_backbone_weights* w, const void* h0, const void* dout, void* dh0 /* both of w->stream_dtype */, void* saved,
                      void* work, int64_t B, int64_t T, int64_t n_last, int64_t n_grad,
                      const mtl_backbone_dropout* drop /* the forward's */, void* stream);
+
+/* ------------------------------------------------------------------ token table: lookup with scaling, gradient by sorted tokens
+ * out[i, :] = scale * table[ids[i], :] (torch.nn.functional.embedding; the frozen gather of R:models/medtsllm.py:331-337 is mtl_assemble_llm_input). An id outside
+ * [0, V) gives a row of zeros and no gradient (rows behind the last token of a padded batch). ids int32 or int64 (ids_i64). Rows contiguous, any row stride. */
+int mtl_embedding_fwd(const void* ids, int ids_i64, int64_t N, const void* table, int table_dtype, int64_t V, int64_t d, int64_t ld_table, float scale,
+                      void* out, int out_dtype, int64_t ld_out, void* stream);
+/* grad[v, :] (+)= scale * sum over {i : ids[i] = v, v != padding_idx} of dout[i, :]. The tokens are sorted by id (stable, so a row's terms are added in one fixed order: the
+ * result does not depend on how the launch is scheduled); sums in fp32, one rounding to grad_dtype. accumulate = 0 writes all V rows (zeros where no token points),
+ * accumulate = 1 touches the rows that occur only. padding_idx < 0: none. N < 2^31, V < 2^31 - 1. */
+size_t mtl_embedding_bwd_workspace_bytes(int64_t N, int64_t V, int64_t d);
+int mtl_embedding_bwd(const void* ids, int ids_i64, int64_t N, const void* dout, int dout_dtype, int64_t ld_dout, int64_t V, int64_t d, int64_t padding_idx, float scale,
+                      void* grad, int grad_dtype, int64_t ld_grad, int accumulate, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------ query / key norm per head + rotary embedding, one pass
+ * per row (b, t) and head: n = x * rsqrt(mean(x^2) + eps); y = rotate(n * w) with the half-split rotation of mtl_rope_inplace on the first R of D elements (pairs j, j + R/2;
+ * cos / sin f32 [n_pos, R], the first R/2 columns are read), the other D - R are normalised only. Position of a row: positions[b * pos_bs + t] (int32 / int64) or, with
+ * positions NULL, pos0 + t. A row whose position is outside [0, n_pos) comes out as NaN (nothing is read out of range).
+ * q [B, T, Hq * D], k [B, T, Hkv * D]: dtype f32 or bf16, unit inner stride, batch / row strides in elements; outputs likewise and may BE the inputs (in place).
+ * wq, wk [D] of w_dtype. D even, 2 <= D <= 512; R even, 2 <= R <= D. */
+typedef struct mtl_qk_norm_rope_args {
+    const void* q; int64_t q_bs, q_ts;
+    const void* k; int64_t k_bs, k_ts;
+    void* q_out; int64_t qo_bs, qo_ts;      /* forward: the outputs; backward: dq */
+    void* k_out; int64_t ko_bs, ko_ts;      /*                                 dk */
+    const void* wq; const void* wk; int w_dtype;
+    const float* cos_t; const float* sin_t; int64_t n_pos;
+    const void* positions; int pos_i64; int64_t pos_bs; int64_t pos0;
+    int64_t B, T, Hq, Hkv, D, R;
+    float eps;
+    int dtype;
+    /* backward only: gradients of the outputs; dwq / dwk f32 [D] (both NULL: not wanted) */
+    const void* dq_out; int64_t dqo_bs, dqo_ts;
+    const void* dk_out; int64_t dko_bs, dko_ts;
+    float* dwq; float* dwk;
+    void* workspace; size_t workspace_bytes;
+} mtl_qk_norm_rope_args;
+int mtl_qk_norm_rope_fwd(const mtl_qk_norm_rope_args* args, void* stream);
+size_t mtl_qk_norm_rope_bwd_workspace_bytes(int64_t B, int64_t T, int64_t D);
+/* dx = r (a - n mean(a n)), a = rotate^T(dy) * w, dw = sum over rows and heads of rotate^T(dy) * n (fixed order); the normalisation is recomputed from x */
+int mtl_qk_norm_rope_bwd(const mtl_qk_norm_rope_args* args, void* stream);
 
 #ifdef __cplusplus
 }

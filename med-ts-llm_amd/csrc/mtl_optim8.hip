@@ -1,0 +1,392 @@
+// Adam / AdamW step with the two moments held in 8 bits (mtl_adam8_step), their read-back (mtl_adam8_moments) and their packing (mtl_adam8_quantize).
+//
+// Blocks of 64 consecutive elements (flat index) share two power-of-two scales, one signed byte each:
+//   m = e4m3(cm) 2^em       round to nearest even, em = floor(log2 max |m|) - 7: the block's largest value lands in [128, 256] of e4m3's 448
+//   r = u44(cr) 2^er        the ROOT of the second moment (v = r^2: half of v's exponent range), unsigned, 4 exponent and 4 mantissa bits:
+//                           u44(c) = c for c < 16, else (16 + c % 16) 2^(c / 16 - 1); er = floor(log2 max r) - 17, so codes end at 240; 255 is NaN
+// Both formats are floating, so a power-of-two scale costs no precision, multiplies exactly, and a block whose scale changes keeps every value on its grid.
+// r is rounded up or down by a threshold u(i, t) = frac(i a1 + t a2), (a1, a2) = the 2-D additive recurrence of the plastic number (1 / 1.3247.., 1 / 1.3247..^2):
+// equidistributed over the elements of a step and over the steps of an element. Rounding to nearest would freeze r: with beta2 = 0.999 a step moves it by
+// about 1 / 2000 of its value, half a grid step is 1 / 64 .. 1 / 32. No generator state: the step number and the element's index are all of it.
+// r > 0 never gets code 0 (m / (0 + eps) would explode); what is not finite becomes the NaN code of that element alone.
+//
+// Every operation is ONE fp32 operation, rounded to nearest, in the order written (no contraction into fma, exact division and square root): a change in the last bit moves
+// a value that sits at a rounding border to the next code, and this way the codes are a function of the inputs that any IEEE machine reproduces bit for bit.
+#include "mtl_common.h"
+
+#pragma clang fp contract(off)
+
+namespace {
+
+constexpr int MAX_T = MTL_ADAM8_MAX_TENSORS;
+constexpr int THREADS = 256;
+constexpr int ITERS = 4;                                       // 4 elements per lane and iteration: all loads of a chunk are in flight before the first use
+constexpr int CHUNK = THREADS * 4 * ITERS;                     // elements per workgroup: a whole number of 64-element blocks
+
+struct Adam8Table {
+    mtl_adam8_tensor t[MAX_T];
+    int first_block[MAX_T + 1];
+    int count;
+};
+struct Adam8Hyper { float om_b1, b2, om_b2, eps, wd, decay, inv_bc2, step_size; uint32_t t_thr; int mode; };   // mode: 0 no decay, 1 L2, 2 decoupled
+
+struct State8Table {
+    mtl_adam8_state t[MAX_T];
+    int first_block[MAX_T + 1];
+    int count;
+};
+
+__device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// largest of 16 lanes (one DPP row = one 64-element block at 4 elements per lane), in every one of them
+template <int CTRL>
+__device__ __forceinline__ uint32_t row_max_step(uint32_t v) {
+    const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xf, 0xf, false);
+    return o > v ? o : v;
+}
+__device__ __forceinline__ uint32_t row_max(uint32_t v) {
+    v = row_max_step<0x121>(v);       // row_ror 1, 2, 4, 8
+    v = row_max_step<0x122>(v);
+    v = row_max_step<0x124>(v);
+    return row_max_step<0x128>(v);
+}
+// bits of |x|, 0 where it is not finite: ordered like the values
+__device__ __forceinline__ uint32_t finite_bits(float x) {
+    const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
+    return b < 0x7f800000u ? b : 0u;
+}
+__device__ __forceinline__ int scale_exp(uint32_t top_bits, int below) {
+    const int e = (int)(top_bits >> 23) - 127 - below;
+    return e < -126 ? -126 : e;                                // (the largest is 127 - 7)
+}
+
+__device__ __forceinline__ void decode4(uint32_t cm, uint32_t cr, float sm, float sr, float (&m)[4], float (&r)[4]) {
+    m[0] = __builtin_amdgcn_cvt_f32_fp8((int)cm, 0) * sm; m[1] = __builtin_amdgcn_cvt_f32_fp8((int)cm, 1) * sm;
+    m[2] = __builtin_amdgcn_cvt_f32_fp8((int)cm, 2) * sm; m[3] = __builtin_amdgcn_cvt_f32_fp8((int)cm, 3) * sm;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const uint32_t c = (cr >> (8 * e)) & 0xffu;
+        float v = c < 16u ? (float)c : __uint_as_float((c + 130u * 16u) << 19);
+        v = c == 255u ? __uint_as_float(0x7fc00000u) : v;
+        r[e] = v * sr;
+    }
+}
+
+__device__ __forceinline__ uint32_t encode_root(float r, float inv, uint32_t u) {
+    const float y = r * inv;
+    const uint32_t large = ((__float_as_uint(y) + (u >> 13)) >> 19) - 130u * 16u;
+    const uint32_t small = (uint32_t)__builtin_floorf(y + (float)(u >> 8) * 0x1p-24f);
+    uint32_t c = y >= 16.0f ? large : small;
+    c = (r > 0.f && c < 1u) ? 1u : c;
+    return (__float_as_uint(r) & 0x7f800000u) == 0x7f800000u ? 255u : c;
+}
+
+// codes of 4 elements and the block's exponents (the same in the 16 lanes of a block); every lane of the wave is active
+__device__ __forceinline__ void encode4(const float (&m)[4], const float (&r)[4], uint32_t idx, uint32_t t_thr, uint32_t& cm, uint32_t& cr, uint32_t& ex) {
+    uint32_t tm = 0, tr = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const uint32_t a = finite_bits(m[e]), b = finite_bits(r[e]);
+        tm = a > tm ? a : tm;
+        tr = b > tr ? b : tr;
+    }
+    const int em = scale_exp(row_max(tm), 7), er = scale_exp(row_max(tr), 17);
+    const float im = pow2i(-em), ir = pow2i(-er);
+    int pk = __builtin_amdgcn_cvt_pk_fp8_f32(m[0] * im, m[1] * im, 0, false);
+    pk = __builtin_amdgcn_cvt_pk_fp8_f32(m[2] * im, m[3] * im, pk, true);
+    cm = (uint32_t)pk;
+    cr = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if ((__float_as_uint(m[e]) & 0x7f800000u) == 0x7f800000u) cm = (cm & ~(0xffu << (8 * e))) | (0x7fu << (8 * e));
+        cr |= encode_root(r[e], ir, (idx + (uint32_t)e) * 0xC13FA9A9u + t_thr) << (8 * e);
+    }
+    ex = ((uint32_t)em & 0xffu) | (((uint32_t)er & 0xffu) << 8);
+}
+
+// 4 code bytes at p, nv of them in range
+__device__ __forceinline__ uint32_t load_codes(const uint8_t* p, int nv, bool vec) {
+    if (vec && nv == 4) return *reinterpret_cast<const uint32_t*>(p);
+    uint32_t c = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (e < nv) c |= (uint32_t)p[e] << (8 * e);
+    return c;
+}
+__device__ __forceinline__ void store_codes(uint8_t* p, uint32_t c, int nv, bool vec) {
+    if (vec && nv == 4) { *reinterpret_cast<uint32_t*>(p) = c; return; }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (e < nv) p[e] = (uint8_t)(c >> (8 * e));
+}
+
+__device__ __forceinline__ void adam8_one(float& p, float g, float& m, float& r, const Adam8Hyper& h) {
+    float v = r * r;
+    if (h.mode == 2) p = p * h.decay;
+    else if (h.mode == 1) g = g + p * h.wd;
+    m = m + (g - m) * h.om_b1;
+    v = v * h.b2 + (g * g) * h.om_b2;
+    r = __builtin_sqrtf(v);
+    const float denom = r * h.inv_bc2 + h.eps;
+    p = p - (m / denom) * h.step_size;
+}
+
+// HBM-bound: fp32 16 + 2/32 B per element (p read and written, g read, two code bytes read and written, two exponent bytes per 64 elements each way), bf16 10 + 2/32.
+template <bool P16>
+__device__ __forceinline__ void adam8_chunk(const mtl_adam8_tensor& t, int64_t base, const Adam8Hyper& h) {
+    float* p32 = reinterpret_cast<float*>(t.p);
+    const float* g32 = reinterpret_cast<const float*>(t.g);
+    bf16_t* p16 = reinterpret_cast<bf16_t*>(t.p);
+    const bf16_t* g16 = reinterpret_cast<const bf16_t*>(t.g);
+    const bool vec = (((uintptr_t)t.p | (uintptr_t)t.g) & (P16 ? 7 : 15)) == 0;
+    const bool vec8 = (((uintptr_t)t.m8 | (uintptr_t)t.r8) & 3) == 0;
+    float pp[ITERS][4], gg[ITERS][4];
+    uint32_t cm[ITERS], cr[ITERS], ex[ITERS];
+#pragma unroll
+    for (int i = 0; i < ITERS; ++i) {
+        const int64_t e0 = base + ((int64_t)i * THREADS + threadIdx.x) * 4;
+        const int64_t left = t.n - e0;
+        const int nv = left >= 4 ? 4 : (left > 0 ? (int)left : 0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) pp[i][e] = gg[i][e] = 0.f;
+        cm[i] = cr[i] = ex[i] = 0;
+        if (nv > 0) {
+            ex[i] = *reinterpret_cast<const uint16_t*>(t.ex + (e0 >> 6) * 2);
+            cm[i] = load_codes(t.m8 + e0, nv, vec8);
+            cr[i] = load_codes(t.r8 + e0, nv, vec8);
+            if (P16) {
+                if (vec && nv == 4) {
+                    const u32x2 a = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p16 + e0)), b = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(g16 + e0));
+                    pp[i][0] = __uint_as_float(a[0] << 16); pp[i][1] = __uint_as_float(a[0] & 0xffff0000u); pp[i][2] = __uint_as_float(a[1] << 16); pp[i][3] = __uint_as_float(a[1] & 0xffff0000u);
+                    gg[i][0] = __uint_as_float(b[0] << 16); gg[i][1] = __uint_as_float(b[0] & 0xffff0000u); gg[i][2] = __uint_as_float(b[1] << 16); gg[i][3] = __uint_as_float(b[1] & 0xffff0000u);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (e < nv) { pp[i][e] = bf16_to_f32(p16[e0 + e]); gg[i][e] = bf16_to_f32(g16[e0 + e]); }
+                }
+            } else if (vec && nv == 4) {
+                const f32x4 a = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(p32 + e0)), b = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(g32 + e0));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) { pp[i][e] = a[e]; gg[i][e] = b[e]; }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (e < nv) { pp[i][e] = p32[e0 + e]; gg[i][e] = g32[e0 + e]; }
+            }
+        }
+    }
+    bf16_t* sh = reinterpret_cast<bf16_t*>(t.shadow);
+#pragma unroll
+    for (int i = 0; i < ITERS; ++i) {
+        const int64_t e0 = base + ((int64_t)i * THREADS + threadIdx.x) * 4;
+        const int64_t left = t.n - e0;
+        const int nv = left >= 4 ? 4 : (left > 0 ? (int)left : 0);
+        float m[4], r[4];
+        decode4(cm[i], cr[i], pow2i((int8_t)(ex[i] & 0xffu)), pow2i((int8_t)(ex[i] >> 8)), m, r);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            adam8_one(pp[i][e], gg[i][e], m[e], r[e], h);
+            if (e >= nv) m[e] = r[e] = 0.f;                     // (elements behind the tensor's end have no part in their block's scales)
+        }
+        uint32_t nm, nr, nx;
+        encode4(m, r, (uint32_t)e0, h.t_thr, nm, nr, nx);
+        if (nv == 0) continue;                                  // (no cross-lane operation below)
+        store_codes(t.m8 + e0, nm, nv, vec8);
+        store_codes(t.r8 + e0, nr, nv, vec8);
+        if ((threadIdx.x & 15) == 0) *reinterpret_cast<uint16_t*>(t.ex + (e0 >> 6) * 2) = (uint16_t)nx;
+        if (P16) {
+            const u32x2 pk = {pack_bf16x2(pp[i][0], pp[i][1]), pack_bf16x2(pp[i][2], pp[i][3])};      // one rounding of the updated parameter
+            if (vec && nv == 4) __builtin_nontemporal_store(pk, reinterpret_cast<u32x2*>(p16 + e0));
+            else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (e < nv) p16[e0 + e] = f32_to_bf16(pp[i][e]);
+            }
+        } else if (vec && nv == 4) {
+            __builtin_nontemporal_store((f32x4){pp[i][0], pp[i][1], pp[i][2], pp[i][3]}, reinterpret_cast<f32x4*>(p32 + e0));
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (e < nv) p32[e0 + e] = pp[i][e];
+        }
+        if (sh) {                                               // bf16 copy [n / cols, ld_shadow] of the updated weight
+            const uint32_t cols = (uint32_t)t.cols;
+            uint32_t row = (uint32_t)e0 / cols, col = (uint32_t)e0 - row * cols;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (e < nv) sh[(int64_t)row * t.ld_shadow + col] = f32_to_bf16(pp[i][e]);
+                if (++col == cols) { col = 0; ++row; }
+            }
+        }
+    }
+}
+
+__global__ __launch_bounds__(THREADS) void adam8_step_kernel(const Adam8Table tab, const Adam8Hyper h) {
+    int ti = 0;
+    const int b = blockIdx.x;
+    while (ti + 1 < tab.count && b >= tab.first_block[ti + 1]) ++ti;
+    const mtl_adam8_tensor t = tab.t[ti];
+    const int64_t base = (int64_t)(b - tab.first_block[ti]) * CHUNK;
+    if (t.param_dtype == MTL_BF16) adam8_chunk<true>(t, base, h);
+    else adam8_chunk<false>(t, base, h);
+}
+
+__device__ __forceinline__ void store_moment(void* dst, int64_t e0, int nv, const float (&x)[4], bool b16) {
+    if (!dst) return;
+    if (b16) {
+        bf16_t* d = reinterpret_cast<bf16_t*>(dst) + e0;
+        if (nv == 4 && ((uintptr_t)d & 7) == 0) {
+            *reinterpret_cast<u32x2*>(d) = (u32x2){pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
+            return;
+        }
+        for (int e = 0; e < nv; ++e) d[e] = f32_to_bf16(x[e]);
+    } else {
+        float* d = reinterpret_cast<float*>(dst) + e0;
+        if (nv == 4 && ((uintptr_t)d & 15) == 0) { *reinterpret_cast<f32x4*>(d) = (f32x4){x[0], x[1], x[2], x[3]}; return; }
+        for (int e = 0; e < nv; ++e) d[e] = x[e];
+    }
+}
+
+// read-back of the codes: 2 B read, 4 (bf16) or 8 B written per element
+__global__ __launch_bounds__(THREADS) void adam8_moments_kernel(const State8Table tab) {
+    int ti = 0;
+    const int b = blockIdx.x;
+    while (ti + 1 < tab.count && b >= tab.first_block[ti + 1]) ++ti;
+    const mtl_adam8_state t = tab.t[ti];
+    const int64_t base = (int64_t)(b - tab.first_block[ti]) * CHUNK;
+    const bool vec8 = (((uintptr_t)t.m8 | (uintptr_t)t.r8) & 3) == 0;
+#pragma unroll
+    for (int i = 0; i < ITERS; ++i) {
+        const int64_t e0 = base + ((int64_t)i * THREADS + threadIdx.x) * 4;
+        if (e0 >= t.n) break;
+        const int nv = t.n - e0 >= 4 ? 4 : (int)(t.n - e0);
+        const uint32_t ex = *reinterpret_cast<const uint16_t*>(t.ex + (e0 >> 6) * 2);
+        float m[4], r[4], v[4];
+        decode4(load_codes(t.m8 + e0, nv, vec8), load_codes(t.r8 + e0, nv, vec8), pow2i((int8_t)(ex & 0xffu)), pow2i((int8_t)(ex >> 8)), m, r);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = r[e] * r[e];
+        store_moment(t.m, e0, nv, m, t.dtype == MTL_BF16);
+        store_moment(t.v, e0, nv, v, t.dtype == MTL_BF16);
+    }
+}
+
+// packing of fp32 moments (taking over a run whose moments are held in 32 bits)
+__global__ __launch_bounds__(THREADS) void adam8_quantize_kernel(const State8Table tab, uint32_t t_thr) {
+    int ti = 0;
+    const int b = blockIdx.x;
+    while (ti + 1 < tab.count && b >= tab.first_block[ti + 1]) ++ti;
+    const mtl_adam8_state t = tab.t[ti];
+    const int64_t base = (int64_t)(b - tab.first_block[ti]) * CHUNK;
+    const bool vec8 = (((uintptr_t)t.m8 | (uintptr_t)t.r8) & 3) == 0;
+    const float* ms = reinterpret_cast<const float*>(t.m);
+    const float* vs = reinterpret_cast<const float*>(t.v);
+#pragma unroll
+    for (int i = 0; i < ITERS; ++i) {
+        const int64_t e0 = base + ((int64_t)i * THREADS + threadIdx.x) * 4;
+        const int64_t left = t.n - e0;
+        const int nv = left >= 4 ? 4 : (left > 0 ? (int)left : 0);
+        float m[4], r[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            m[e] = e < nv ? ms[e0 + e] : 0.f;
+            r[e] = e < nv ? __builtin_sqrtf(vs[e0 + e]) : 0.f;
+        }
+        uint32_t nm, nr, nx;
+        encode4(m, r, (uint32_t)e0, t_thr, nm, nr, nx);
+        if (nv == 0) continue;
+        store_codes(t.m8 + e0, nm, nv, vec8);
+        store_codes(t.r8 + e0, nr, nv, vec8);
+        if ((threadIdx.x & 15) == 0) *reinterpret_cast<uint16_t*>(t.ex + (e0 >> 6) * 2) = (uint16_t)nx;
+    }
+}
+
+int check_state(const mtl_adam8_state& t, bool read_back) {
+    if (t.n < 0 || (t.n > 0 && (!t.m8 || !t.r8 || !t.ex))) return MTL_ERR_ARG;
+    if (t.n > 0 && !read_back && (!t.m || !t.v)) return MTL_ERR_ARG;
+    if ((uintptr_t)t.ex & 1) return MTL_ERR_ALIGN;
+    if (t.dtype != MTL_F32 && !(read_back && t.dtype == MTL_BF16)) return MTL_ERR_ARG;
+    return ((uintptr_t)t.m | (uintptr_t)t.v) & (t.dtype == MTL_F32 ? 3 : 1) ? MTL_ERR_ALIGN : MTL_OK;
+}
+
+template <typename Launch>
+int for_tables(const mtl_adam8_state* states, int count, bool read_back, Launch launch) {
+    for (int i = 0; i < count; ++i)
+        if (const int rc = check_state(states[i], read_back)) return rc;
+    for (int i = 0; i < count;) {
+        State8Table tab;
+        tab.count = 0;
+        int64_t blocks = 0;
+        for (; i < count && tab.count < MAX_T; ++i) {
+            if (states[i].n == 0) continue;
+            const int64_t nb = (states[i].n + CHUNK - 1) / CHUNK;
+            if (nb > 0x7fffffff) return MTL_ERR_UNSUPPORTED;
+            if (blocks + nb > 0x7fffffff) break;                // (this one goes into the next launch)
+            tab.t[tab.count] = states[i];
+            tab.first_block[tab.count++] = (int)blocks;
+            blocks += nb;
+        }
+        tab.first_block[tab.count] = (int)blocks;
+        if (blocks == 0) continue;
+        launch(tab, (unsigned)blocks);
+        MTL_CHECK_LAUNCH();
+    }
+    return MTL_OK;
+}
+
+}  // namespace
+
+extern "C" int mtl_adam8_step(const mtl_adam8_tensor* tensors, int count, double lr, double beta1, double beta2, double eps, double weight_decay, int decoupled, int64_t step, void* stream) {
+    if (count < 0 || (count > 0 && !tensors) || step < 1 || !(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) || !(eps >= 0.0) || !(weight_decay >= 0.0)) return MTL_ERR_ARG;
+    for (int i = 0; i < count; ++i) {
+        const mtl_adam8_tensor& t = tensors[i];
+        if (t.n < 0 || (t.param_dtype != MTL_F32 && t.param_dtype != MTL_BF16)) return MTL_ERR_ARG;
+        if (t.n == 0) continue;
+        if (!t.p || !t.g || !t.m8 || !t.r8 || !t.ex) return MTL_ERR_ARG;
+        if ((((uintptr_t)t.p | (uintptr_t)t.g) & (t.param_dtype == MTL_BF16 ? 1 : 3)) || ((uintptr_t)t.ex & 1) || ((uintptr_t)t.shadow & 1)) return MTL_ERR_ALIGN;
+        if (t.shadow && (t.cols <= 0 || t.ld_shadow < t.cols || t.n % t.cols != 0 || t.n >= ((int64_t)1 << 32))) return MTL_ERR_ARG;
+    }
+    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    Adam8Hyper h;
+    h.om_b1 = (float)(1.0 - beta1); h.b2 = (float)beta2; h.om_b2 = (float)(1.0 - beta2); h.eps = (float)eps; h.wd = (float)weight_decay;
+    h.decay = (float)(1.0 - lr * weight_decay);
+    h.inv_bc2 = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)step)));
+    h.step_size = (float)(lr / (1.0 - pow(beta1, (double)step)));
+    h.t_thr = (uint32_t)step * 0x91E10DA5u;
+    h.mode = weight_decay == 0.0 ? 0 : (decoupled ? 2 : 1);
+    for (int i = 0; i < count;) {
+        Adam8Table tab;
+        tab.count = 0;
+        int64_t blocks = 0;
+        double bytes = 0;
+        for (; i < count && tab.count < MAX_T; ++i) {
+            const mtl_adam8_tensor& t = tensors[i];
+            if (t.n == 0) continue;
+            const int64_t nb = (t.n + CHUNK - 1) / CHUNK;
+            if (nb > 0x7fffffff) return MTL_ERR_UNSUPPORTED;
+            if (blocks + nb > 0x7fffffff) break;
+            tab.t[tab.count] = t;
+            tab.first_block[tab.count++] = (int)blocks;
+            blocks += nb;
+            bytes += (double)t.n * ((t.param_dtype == MTL_BF16 ? 10.0 : 16.0) + 4.0 / 64 + (t.shadow ? 2.0 : 0.0));
+        }
+        tab.first_block[tab.count] = (int)blocks;
+        if (blocks == 0) continue;
+        MTL_LAUNCH("adam8_step_kernel", bytes, 1, adam8_step_kernel, dim3((unsigned)blocks), dim3(THREADS), 0, st, tab, h);
+        MTL_CHECK_LAUNCH();
+    }
+    return MTL_OK;
+}
+
+extern "C" int mtl_adam8_moments(const mtl_adam8_state* states, int count, void* stream) {
+    if (count < 0 || (count > 0 && !states)) return MTL_ERR_ARG;
+    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    return for_tables(states, count, true, [&](const State8Table& tab, unsigned blocks) { hipLaunchKernelGGL(adam8_moments_kernel, dim3(blocks), dim3(THREADS), 0, st, tab); });
+}
+
+extern "C" int mtl_adam8_quantize(const mtl_adam8_state* states, int count, int64_t step, void* stream) {
+    if (count < 0 || (count > 0 && !states) || step < 0) return MTL_ERR_ARG;
+    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    return for_tables(states, count, false, [&](const State8Table& tab, unsigned blocks) {
+        hipLaunchKernelGGL(adam8_quantize_kernel, dim3(blocks), dim3(THREADS), 0, st, tab, (uint32_t)step * 0x91E10DA5u);
+    });
+}

@@ -1,0 +1,409 @@
+// RMS norm of every query and key head and the rotary embedding behind it in one pass (mtl_qk_norm_rope_fwd), and its backward pass.
+//
+//   r = 1 / sqrt(mean_j x_j^2 + eps),  n = r x,  y = Rot(n w)            Rot: half-split rotation of the first R of D elements by the row's position (pairs j, j + R/2)
+//   u = Rot^T dy,  dw = sum u n,  a = u w,  dx = r (a - n mean_j(a_j n_j))
+//
+// HBM-bound: the forward reads and writes (Hq + Hkv) D elements per row, the backward reads two and writes one (r is recomputed from x, which it reads anyway: nothing is saved).
+// Layout: a wave owns a row (one token) and walks its heads; a group of LPH lanes owns a head, each lane W consecutive PAIRS, i.e. W elements of each half: the rotation needs no
+// exchange between lanes, the two sums take log2(LPH) DPP steps, and what the heads of a row share (cos, sin, both weights) is loaded once per row or wave and stays in registers.
+// Pairs beyond R/2 (elements R .. D-1, split in halves the same way) are rotated by angle 0. All arithmetic fp32, one rounding at the store.
+#include "mtl_common.h"
+
+namespace {
+
+constexpr int WAVES = 4;
+
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float v) {
+    return v + __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, 0xf, 0xf, true));
+}
+// sum over groups of L lanes, in every lane of the group (all 64 lanes active)
+template <int L>
+__device__ __forceinline__ float group_sum(float v) {
+    v = dpp_add<0xB1>(v);                       // quad_perm: neighbours
+    v = dpp_add<0x4E>(v);                       // quad_perm: pairs
+    if (L >= 8) v = dpp_add<0x141>(v);          // row_half_mirror: the other quad of 8
+    if (L >= 16) v = dpp_add<0x140>(v);         // row_mirror: the other half of 16
+    if (L >= 32) v += __shfl_xor(v, 16, 64);
+    if (L >= 64) v += __shfl_xor(v, 32, 64);
+    return v;
+}
+
+template <typename T, int W>
+__device__ __forceinline__ void load_w(const T* p, float (&x)[W]);
+template <>
+__device__ __forceinline__ void load_w<float, 8>(const float* p, float (&x)[8]) {
+    const f32x4 a = reinterpret_cast<const f32x4*>(p)[0], b = reinterpret_cast<const f32x4*>(p)[1];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { x[j] = a[j]; x[4 + j] = b[j]; }
+}
+template <>
+__device__ __forceinline__ void load_w<bf16_t, 8>(const bf16_t* p, float (&x)[8]) {
+    const u32x4 a = *reinterpret_cast<const u32x4*>(p);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { x[2 * j] = __uint_as_float(a[j] << 16); x[2 * j + 1] = __uint_as_float(a[j] & 0xffff0000u); }
+}
+template <>
+__device__ __forceinline__ void load_w<float, 1>(const float* p, float (&x)[1]) { x[0] = *p; }
+template <>
+__device__ __forceinline__ void load_w<bf16_t, 1>(const bf16_t* p, float (&x)[1]) { x[0] = bf16_to_f32(*p); }
+__device__ __forceinline__ void store_w(float* p, const float (&x)[8]) {
+    reinterpret_cast<f32x4*>(p)[0] = (f32x4){x[0], x[1], x[2], x[3]};
+    reinterpret_cast<f32x4*>(p)[1] = (f32x4){x[4], x[5], x[6], x[7]};
+}
+__device__ __forceinline__ void store_w(bf16_t* p, const float (&x)[8]) {
+    *reinterpret_cast<u32x4*>(p) = (u32x4){pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7])};
+}
+__device__ __forceinline__ void store_w(float* p, const float (&x)[1]) { *p = x[0]; }
+__device__ __forceinline__ void store_w(bf16_t* p, const float (&x)[1]) { *p = f32_to_bf16(x[0]); }
+
+// where a lane's C chunks of W pairs sit: lo[c] / hi[c] = the elements of the two halves, turn[c] = index of the first pair in the cos / sin row or -1 (not rotated), on[c] = in the head
+template <int W, int LPH, int C>
+struct Lane {
+    int lo[C], hi[C], turn[C];
+    bool on[C];
+    __device__ __forceinline__ Lane(int D, int R) {
+        const int l = threadIdx.x & (LPH - 1), rp = R >> 1, pairs = D >> 1;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int j = (c * LPH + l) * W;
+            on[c] = j < pairs;
+            const int jj = on[c] ? j : 0;
+            const bool rot = jj < rp;
+            lo[c] = rot ? jj : R + (jj - rp);
+            hi[c] = rot ? jj + rp : R + (jj - rp) + ((D - R) >> 1);
+            turn[c] = rot ? jj : -1;
+        }
+    }
+};
+
+__device__ __forceinline__ float weight_at(const void* w, int dtype, int i) {
+    return dtype == MTL_BF16 ? bf16_to_f32(reinterpret_cast<const bf16_t*>(w)[i]) : reinterpret_cast<const float*>(w)[i];
+}
+template <int W, int LPH, int C>
+__device__ __forceinline__ void load_weights(const void* w, int dtype, const Lane<W, LPH, C>& L, float (&lo)[C][W], float (&hi)[C][W]) {
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+            lo[c][j] = L.on[c] ? weight_at(w, dtype, L.lo[c] + j) : 0.f;
+            hi[c][j] = L.on[c] ? weight_at(w, dtype, L.hi[c] + j) : 0.f;
+        }
+}
+
+// cos / sin of a row's pairs; a position outside the table turns every element of the row into NaN
+template <int W, int LPH, int C>
+__device__ __forceinline__ void load_turn(const mtl_qk_norm_rope_args& a, int64_t b, int64_t t, const Lane<W, LPH, C>& L, float (&cs)[C][W], float (&sn)[C][W]) {
+    int64_t pos = a.pos0 + t;
+    if (a.positions) pos = a.pos_i64 ? reinterpret_cast<const int64_t*>(a.positions)[b * a.pos_bs + t] : (int64_t)reinterpret_cast<const int32_t*>(a.positions)[b * a.pos_bs + t];
+    const bool in = pos >= 0 && pos < a.n_pos;
+    const float nan = __uint_as_float(0x7fc00000u);
+    const float* cr = a.cos_t + (in ? pos : 0) * a.R;
+    const float* sr = a.sin_t + (in ? pos : 0) * a.R;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        if (L.turn[c] >= 0) {
+            load_w<float, W>(cr + L.turn[c], cs[c]);
+            load_w<float, W>(sr + L.turn[c], sn[c]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < W; ++j) { cs[c][j] = 1.f; sn[c][j] = 0.f; }
+        }
+        if (!in)
+#pragma unroll
+            for (int j = 0; j < W; ++j) cs[c][j] = sn[c][j] = nan;
+    }
+}
+
+// heads [h0, h1) of one row: forward
+template <typename T, int W, int LPH, int C>
+__device__ __forceinline__ void heads_fwd(const T* __restrict__ x, T* y, int h0, int h1, int D, float eps, float inv_d, const Lane<W, LPH, C>& L, const float (&wl)[C][W], const float (&wh)[C][W],
+                                          const float (&cs)[C][W], const float (&sn)[C][W]) {
+    constexpr int G = 64 / LPH, U = (W == 8 && C == 1) ? 2 : 1;      // heads per step of the wave, steps whose loads are in flight together
+    const int g = (threadIdx.x & 63) / LPH;
+    for (int h = h0; h < h1; h += G * U) {
+        float lo[U][C][W], hi[U][C][W];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const int hh = h + u * G + g;
+                if (hh < h1 && L.on[c]) {
+                    load_w<T, W>(x + (int64_t)hh * D + L.lo[c], lo[u][c]);
+                    load_w<T, W>(x + (int64_t)hh * D + L.hi[c], hi[u][c]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < W; ++j) lo[u][c][j] = hi[u][c][j] = 0.f;
+                }
+            }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int hh = h + u * G + g;
+            float ss = 0.f;
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int j = 0; j < W; ++j) ss += lo[u][c][j] * lo[u][c][j] + hi[u][c][j] * hi[u][c][j];
+            ss = group_sum<LPH>(ss);
+            const float r = 1.0f / __builtin_sqrtf(ss * inv_d + eps);
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                float yl[W], yh[W];
+#pragma unroll
+                for (int j = 0; j < W; ++j) rope_pair(lo[u][c][j] * r * wl[c][j], hi[u][c][j] * r * wh[c][j], cs[c][j], sn[c][j], yl[j], yh[j]);
+                if (hh < h1 && L.on[c]) {
+                    store_w(y + (int64_t)hh * D + L.lo[c], yl);
+                    store_w(y + (int64_t)hh * D + L.hi[c], yh);
+                }
+            }
+        }
+    }
+}
+
+template <typename T, int W, int LPH, int C>
+__global__ __launch_bounds__(WAVES * 64) void qk_norm_rope_fwd_kernel(const mtl_qk_norm_rope_args a, int hq_per, int hk_per) {
+    const Lane<W, LPH, C> L((int)a.D, (int)a.R);
+    const int64_t rows = a.B * a.T;
+    const float inv_d = 1.0f / (float)a.D;
+    float ql[C][W], qh[C][W], kl[C][W], kh[C][W];
+    load_weights(a.wq, a.w_dtype, L, ql, qh);
+    load_weights(a.wk, a.w_dtype, L, kl, kh);
+    const int part = blockIdx.y;                       // few rows: a row's heads are spread over gridDim.y waves
+    const int q0 = part * hq_per, q1 = q0 + hq_per < a.Hq ? q0 + hq_per : (int)a.Hq;
+    const int k0 = part * hk_per, k1 = k0 + hk_per < a.Hkv ? k0 + hk_per : (int)a.Hkv;
+    for (int64_t row = (int64_t)blockIdx.x * WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); row < rows; row += (int64_t)gridDim.x * WAVES) {
+        const int64_t b = row / a.T, t = row - b * a.T;
+        float cs[C][W], sn[C][W];
+        load_turn(a, b, t, L, cs, sn);
+        heads_fwd<T, W, LPH, C>((const T*)a.q + b * a.q_bs + t * a.q_ts, (T*)a.q_out + b * a.qo_bs + t * a.qo_ts, q0, q1, (int)a.D, a.eps, inv_d, L, ql, qh, cs, sn);
+        heads_fwd<T, W, LPH, C>((const T*)a.k + b * a.k_bs + t * a.k_ts, (T*)a.k_out + b * a.ko_bs + t * a.ko_ts, k0, k1, (int)a.D, a.eps, inv_d, L, kl, kh, cs, sn);
+    }
+}
+
+// all heads of one row: backward; gl / gh accumulate dw
+template <typename T, int W, int LPH, int C, bool DW>
+__device__ __forceinline__ void heads_bwd(const T* __restrict__ x, const T* dy, T* dx, int h1, int D, float eps, float inv_d, const Lane<W, LPH, C>& L, const float (&wl)[C][W],
+                                          const float (&wh)[C][W], const float (&cs)[C][W], const float (&sn)[C][W], float (&gl)[C][W], float (&gh)[C][W]) {
+    constexpr int G = 64 / LPH;
+    const int g = (threadIdx.x & 63) / LPH;
+    for (int h = 0; h < h1; h += G) {
+        const int hh = h + g;
+        float lo[C][W], hi[C][W], al[C][W], ah[C][W];
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            if (hh < h1 && L.on[c]) {
+                load_w<T, W>(x + (int64_t)hh * D + L.lo[c], lo[c]);
+                load_w<T, W>(x + (int64_t)hh * D + L.hi[c], hi[c]);
+                load_w<T, W>(dy + (int64_t)hh * D + L.lo[c], al[c]);
+                load_w<T, W>(dy + (int64_t)hh * D + L.hi[c], ah[c]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < W; ++j) lo[c][j] = hi[c][j] = al[c][j] = ah[c][j] = 0.f;
+            }
+        }
+        float ss = 0.f, sa = 0.f;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                float ul, uh;
+                rope_pair(al[c][j], ah[c][j], cs[c][j], -sn[c][j], ul, uh);          // the inverse rotation
+                al[c][j] = ul; ah[c][j] = uh;
+                ss += lo[c][j] * lo[c][j] + hi[c][j] * hi[c][j];
+                sa += ul * wl[c][j] * lo[c][j] + uh * wh[c][j] * hi[c][j];
+            }
+        ss = group_sum<LPH>(ss);
+        sa = group_sum<LPH>(sa);
+        const float r = 1.0f / __builtin_sqrtf(ss * inv_d + eps);
+        const float m = sa * r * r * inv_d;                     // n mean(a n) = x r mean(a x r)
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            float yl[W], yh[W];
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                if (DW && hh < h1) { gl[c][j] += al[c][j] * (lo[c][j] * r); gh[c][j] += ah[c][j] * (hi[c][j] * r); }
+                yl[j] = r * (al[c][j] * wl[c][j] - lo[c][j] * m);
+                yh[j] = r * (ah[c][j] * wh[c][j] - hi[c][j] * m);
+            }
+            if (hh < h1 && L.on[c]) {
+                store_w(dx + (int64_t)hh * D + L.lo[c], yl);
+                store_w(dx + (int64_t)hh * D + L.hi[c], yh);
+            }
+        }
+    }
+}
+
+// part [gridDim.x][2][D] (DW): every workgroup's weight gradients, summed over its waves and lane groups in a fixed order
+template <typename T, int W, int LPH, int C, bool DW>
+__global__ __launch_bounds__(WAVES * 64) void qk_norm_rope_bwd_kernel(const mtl_qk_norm_rope_args a, float* __restrict__ part) {
+    const Lane<W, LPH, C> L((int)a.D, (int)a.R);
+    const int64_t rows = a.B * a.T;
+    const float inv_d = 1.0f / (float)a.D;
+    float ql[C][W], qh[C][W], kl[C][W], kh[C][W], gql[C][W], gqh[C][W], gkl[C][W], gkh[C][W];
+    load_weights(a.wq, a.w_dtype, L, ql, qh);
+    load_weights(a.wk, a.w_dtype, L, kl, kh);
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int j = 0; j < W; ++j) gql[c][j] = gqh[c][j] = gkl[c][j] = gkh[c][j] = 0.f;
+    for (int64_t row = (int64_t)blockIdx.x * WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); row < rows; row += (int64_t)gridDim.x * WAVES) {
+        const int64_t b = row / a.T, t = row - b * a.T;
+        float cs[C][W], sn[C][W];
+        load_turn(a, b, t, L, cs, sn);
+        heads_bwd<T, W, LPH, C, DW>((const T*)a.q + b * a.q_bs + t * a.q_ts, (const T*)a.dq_out + b * a.dqo_bs + t * a.dqo_ts, (T*)a.q_out + b * a.qo_bs + t * a.qo_ts, (int)a.Hq, (int)a.D, a.eps, inv_d,
+                                    L, ql, qh, cs, sn, gql, gqh);
+        heads_bwd<T, W, LPH, C, DW>((const T*)a.k + b * a.k_bs + t * a.k_ts, (const T*)a.dk_out + b * a.dko_bs + t * a.dko_ts, (T*)a.k_out + b * a.ko_bs + t * a.ko_ts, (int)a.Hkv, (int)a.D, a.eps, inv_d,
+                                    L, kl, kh, cs, sn, gkl, gkh);
+    }
+    if (!DW) return;
+    // lane groups of a wave, then the waves: [WAVES * 64 / LPH][D] in LDS, one weight at a time
+    constexpr int G = 64 / LPH;
+    __shared__ float sums[WAVES * G * 2 * LPH * C * W];
+    const int slot = (threadIdx.x >> 6) * G + (threadIdx.x & 63) / LPH, D = (int)a.D;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+            if (L.on[c])
+#pragma unroll
+                for (int j = 0; j < W; ++j) {
+                    sums[slot * D + L.lo[c] + j] = which ? gkl[c][j] : gql[c][j];
+                    sums[slot * D + L.hi[c] + j] = which ? gkh[c][j] : gqh[c][j];
+                }
+        __syncthreads();
+        for (int i = threadIdx.x; i < D; i += WAVES * 64) {
+            float s = 0.f;
+#pragma unroll 8
+            for (int k = 0; k < WAVES * G; ++k) s += sums[k * D + i];
+            part[((int64_t)blockIdx.x * 2 + which) * D + i] = s;
+        }
+    }
+}
+
+// dw[which][i] = sum over the workgroups of the backward: 16 waves take a sixteenth each, in order
+__global__ __launch_bounds__(1024) void qk_norm_rope_dw_kernel(const float* __restrict__ part, int n, int D, float* __restrict__ dwq, float* __restrict__ dwk) {
+    __shared__ float sums[16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int i = blockIdx.x * 64 + lane, which = blockIdx.y;
+    float s = 0.f;
+    if (i < D) {
+        const int k0 = n * wave / 16, k1 = n * (wave + 1) / 16;
+#pragma unroll 8
+        for (int k = k0; k < k1; ++k) s += part[((int64_t)k * 2 + which) * D + i];
+    }
+    sums[wave][lane] = s;
+    __syncthreads();
+    if (wave == 0 && i < D) {
+        s = sums[0][lane];
+#pragma unroll
+        for (int w = 1; w < 16; ++w) s += sums[w][lane];
+        (which ? dwk : dwq)[i] = s;
+    }
+}
+
+inline unsigned fwd_blocks(int64_t rows) { const int64_t b = (rows + WAVES - 1) / WAVES; return (unsigned)(b < 2048 ? b : 2048); }
+inline unsigned bwd_blocks(int64_t rows) { const int64_t b = (rows + WAVES - 1) / WAVES; return (unsigned)(b < 1024 ? b : 1024); }
+
+template <typename T, int W, int LPH, int C>
+int launch(const mtl_qk_norm_rope_args& a, bool bwd, hipStream_t st) {
+    const int64_t rows = a.B * a.T;
+    if (!bwd) {
+        // one wave per row; where that leaves the chip empty, a row's heads go to several waves (each a whole number of the wave's head groups)
+        constexpr int G = 64 / LPH;
+        int parts = 1;
+        const int64_t steps = ((a.Hq > a.Hkv ? a.Hq : a.Hkv) + G - 1) / G;
+        while (parts < steps && rows * parts < 4096) parts *= 2;
+        if (parts > steps) parts = (int)steps;
+        const int hq = (int)(((a.Hq + parts - 1) / parts + G - 1) / G * G), hk = (int)(((a.Hkv + parts - 1) / parts + G - 1) / G * G);
+        hipLaunchKernelGGL((qk_norm_rope_fwd_kernel<T, W, LPH, C>), dim3(fwd_blocks(rows), parts), dim3(WAVES * 64), 0, st, a, hq, hk);
+        MTL_CHECK_LAUNCH();
+        return MTL_OK;
+    }
+    const unsigned blocks = bwd_blocks(rows);
+    float* part = reinterpret_cast<float*>(a.workspace);
+    if (!a.dwq) {
+        hipLaunchKernelGGL((qk_norm_rope_bwd_kernel<T, W, LPH, C, false>), dim3(blocks), dim3(WAVES * 64), 0, st, a, part);
+        MTL_CHECK_LAUNCH();
+        return MTL_OK;
+    }
+    hipLaunchKernelGGL((qk_norm_rope_bwd_kernel<T, W, LPH, C, true>), dim3(blocks), dim3(WAVES * 64), 0, st, a, part);
+    MTL_CHECK_LAUNCH();
+    hipLaunchKernelGGL(qk_norm_rope_dw_kernel, dim3((unsigned)((a.D + 63) / 64), 2), dim3(1024), 0, st, part, (int)blocks, (int)a.D, a.dwq, a.dwk);
+    MTL_CHECK_LAUNCH();
+    return MTL_OK;
+}
+
+// 8 pairs per lane with 16-byte accesses where every row, head and half starts on a 16-byte border; else one pair per lane and chunk
+inline bool rows_fit(const void* p, int64_t bs, int64_t ts, int size) {
+    return ((uintptr_t)p & 15) == 0 && (bs * size) % 16 == 0 && (ts * size) % 16 == 0;
+}
+
+template <typename T>
+int dispatch(const mtl_qk_norm_rope_args& a, bool bwd, hipStream_t st) {
+    const int s = (int)sizeof(T);
+    bool wide = (a.R / 2) % 8 == 0 && ((a.D - a.R) / 2) % 8 == 0 && rows_fit(a.q, a.q_bs, a.q_ts, s) && rows_fit(a.k, a.k_bs, a.k_ts, s) && rows_fit(a.q_out, a.qo_bs, a.qo_ts, s) &&
+                rows_fit(a.k_out, a.ko_bs, a.ko_ts, s) && (((uintptr_t)a.cos_t | (uintptr_t)a.sin_t) & 15) == 0;
+    if (bwd) wide = wide && rows_fit(a.dq_out, a.dqo_bs, a.dqo_ts, s) && rows_fit(a.dk_out, a.dko_bs, a.dko_ts, s);
+    const int pairs = (int)(a.D / 2);
+    if (wide) {
+        if (pairs <= 32) return launch<T, 8, 4, 1>(a, bwd, st);
+        if (pairs <= 64) return launch<T, 8, 8, 1>(a, bwd, st);
+        if (pairs <= 128) return launch<T, 8, 16, 1>(a, bwd, st);
+        return launch<T, 8, 32, 1>(a, bwd, st);
+    }
+    if (pairs <= 64) return launch<T, 1, 64, 1>(a, bwd, st);
+    if (pairs <= 128) return launch<T, 1, 64, 2>(a, bwd, st);
+    return launch<T, 1, 64, 4>(a, bwd, st);
+}
+
+int check_args(const mtl_qk_norm_rope_args* a, bool bwd) {
+    if (!a || a->B < 0 || a->T < 0 || a->Hq <= 0 || a->Hkv <= 0 || a->D < 2 || a->R < 2 || a->D % 2 || a->R % 2 || a->R > a->D || a->n_pos < 0 || !(a->eps >= 0.f)) return MTL_ERR_ARG;
+    if (a->D > 512 || a->Hq > 65536 || a->Hkv > 65536) return MTL_ERR_UNSUPPORTED;
+    if ((a->dtype != MTL_F32 && a->dtype != MTL_BF16) || (a->w_dtype != MTL_F32 && a->w_dtype != MTL_BF16)) return MTL_ERR_ARG;
+    if (bwd && !a->dwq != !a->dwk) return MTL_ERR_ARG;
+    if (a->B == 0 || a->T == 0) return MTL_OK;
+    if (!a->q || !a->k || !a->q_out || !a->k_out || !a->wq || !a->wk || !a->cos_t || !a->sin_t || a->n_pos == 0) return MTL_ERR_ARG;
+    if (bwd && (!a->dq_out || !a->dk_out)) return MTL_ERR_ARG;
+    const uintptr_t e = a->dtype == MTL_BF16 ? 1 : 3, w = a->w_dtype == MTL_BF16 ? 1 : 3;
+    if ((((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->q_out | (uintptr_t)a->k_out) & e) || (((uintptr_t)a->wq | (uintptr_t)a->wk) & w) || (((uintptr_t)a->cos_t | (uintptr_t)a->sin_t) & 3) ||
+        ((uintptr_t)a->positions & (a->pos_i64 ? 7 : 3)))
+        return MTL_ERR_ALIGN;
+    if (bwd && ((((uintptr_t)a->dq_out | (uintptr_t)a->dk_out) & e) || (((uintptr_t)a->dwq | (uintptr_t)a->dwk | (uintptr_t)a->workspace) & 3))) return MTL_ERR_ALIGN;
+    return MTL_OK;
+}
+
+__global__ void zero_pair_kernel(float* a, float* b, int n) {
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i < n) a[i] = b[i] = 0.f;
+}
+
+}  // namespace
+
+extern "C" int mtl_qk_norm_rope_fwd(const mtl_qk_norm_rope_args* a, void* stream) {
+    const int rc = check_args(a, false);
+    if (rc) return rc;
+    if (a->B == 0 || a->T == 0) return MTL_OK;
+    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    return a->dtype == MTL_BF16 ? dispatch<bf16_t>(*a, false, st) : dispatch<float>(*a, false, st);
+}
+
+extern "C" size_t mtl_qk_norm_rope_bwd_workspace_bytes(int64_t B, int64_t T, int64_t D) {
+    if (B <= 0 || T <= 0 || D <= 0) return 16;
+    return (size_t)bwd_blocks(B * T) * 2 * (size_t)D * 4;
+}
+
+extern "C" int mtl_qk_norm_rope_bwd(const mtl_qk_norm_rope_args* a, void* stream) {
+    const int rc = check_args(a, true);
+    if (rc) return rc;
+    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    if (a->B == 0 || a->T == 0) {
+        if (a->dwq) {
+            hipLaunchKernelGGL(zero_pair_kernel, dim3((unsigned)((a->D + 255) / 256)), dim3(256), 0, st, a->dwq, a->dwk, (int)a->D);
+            MTL_CHECK_LAUNCH();
+        }
+        return MTL_OK;
+    }
+    if (a->dwq && (!a->workspace || a->workspace_bytes < mtl_qk_norm_rope_bwd_workspace_bytes(a->B, a->T, a->D))) return MTL_ERR_WORKSPACE;
+    return a->dtype == MTL_BF16 ? dispatch<bf16_t>(*a, true, st) : dispatch<float>(*a, true, st);
+}

@@ -2,6 +2,7 @@
 
 The product path has NO CPU / PyTorch fallback: if the library is missing or a call fails we raise.
 """
+import contextlib
 import ctypes as C
 import os
 
@@ -13,7 +14,7 @@ LIB_PATH = os.environ.get("MTL_LIB_PATH") or os.path.join(_HERE, "libmedtsllm_hi
 MTL_F32, MTL_BF16 = 0, 1
 EPI_STORE, EPI_GELU, EPI_RESID, EPI_DGELU, EPI_ACCUM, EPI_SWIGLU, EPI_DSWIGLU = 0, 1, 2, 3, 4, 5, 6
 ARCH_GPT2, ARCH_LLAMA = 0, 1
-ABI_VERSION = 15
+ABI_VERSION = 16
 
 i64, vp, f32, i32 = C.c_int64, C.c_void_p, C.c_float, C.c_int
 
@@ -53,6 +54,28 @@ class AdamTensor(C.Structure):
 
 
 ADAM_MAX_TENSORS = 24
+
+
+class Adam8Tensor(C.Structure):
+    _fields_ = [("p", vp), ("g", vp), ("m8", vp), ("r8", vp), ("ex", vp), ("n", i64), ("shadow", vp), ("cols", i64), ("ld_shadow", i64), ("param_dtype", i64)]
+
+
+class Adam8State(C.Structure):
+    _fields_ = [("m8", vp), ("r8", vp), ("ex", vp), ("n", i64), ("m", vp), ("v", vp), ("dtype", i64)]
+
+
+ADAM8_BLOCK = 64
+f64 = C.c_double
+
+
+class QkNormRopeArgs(C.Structure):
+    _fields_ = [("q", vp), ("q_bs", i64), ("q_ts", i64), ("k", vp), ("k_bs", i64), ("k_ts", i64),
+                ("q_out", vp), ("qo_bs", i64), ("qo_ts", i64), ("k_out", vp), ("ko_bs", i64), ("ko_ts", i64),
+                ("wq", vp), ("wk", vp), ("w_dtype", i32), ("cos_t", vp), ("sin_t", vp), ("n_pos", i64),
+                ("positions", vp), ("pos_i64", i32), ("pos_bs", i64), ("pos0", i64),
+                ("B", i64), ("T", i64), ("Hq", i64), ("Hkv", i64), ("D", i64), ("R", i64), ("eps", f32), ("dtype", i32),
+                ("dq_out", vp), ("dqo_bs", i64), ("dqo_ts", i64), ("dk_out", vp), ("dko_bs", i64), ("dko_ts", i64),
+                ("dwq", vp), ("dwk", vp), ("workspace", vp), ("workspace_bytes", C.c_size_t)]
 
 
 class AttnFwdArgs(C.Structure):
@@ -117,6 +140,15 @@ SIGNATURES = {
     "mtl_channel_mix_workspace_bytes": (C.c_size_t, [i64, i64, i64]),
     "mtl_channel_mix_bwd": (i32, [vp, vp, vp, i32, vp, vp, vp, vp, i64, i64, i64, i64, i64, vp]),
     "mtl_adam_step": (i32, [C.POINTER(AdamTensor), i32, f32, f32, f32, f32, f32, i32, i64, vp]),
+    "mtl_adam8_step": (i32, [vp, i32, f64, f64, f64, f64, f64, i32, i64, vp]),
+    "mtl_adam8_moments": (i32, [vp, i32, vp]),
+    "mtl_adam8_quantize": (i32, [vp, i32, i64, vp]),
+    "mtl_embedding_fwd": (i32, [vp, i32, i64, vp, i32, i64, i64, i64, f32, vp, i32, i64, vp]),
+    "mtl_embedding_bwd_workspace_bytes": (C.c_size_t, [i64, i64, i64]),
+    "mtl_embedding_bwd": (i32, [vp, i32, i64, vp, i32, i64, i64, i64, i64, f32, vp, i32, i64, i32, vp, C.c_size_t, vp]),
+    "mtl_qk_norm_rope_fwd": (i32, [C.POINTER(QkNormRopeArgs), vp]),
+    "mtl_qk_norm_rope_bwd_workspace_bytes": (C.c_size_t, [i64, i64, i64]),
+    "mtl_qk_norm_rope_bwd": (i32, [C.POINTER(QkNormRopeArgs), vp]),
     "mtl_attention_fwd": (i32, [C.POINTER(AttnFwdArgs), vp]),
     "mtl_attention_bwd": (i32, [C.POINTER(AttnBwdArgs), vp]),
     "mtl_norm_fwd": (i32, [vp, vp, vp, vp, i64, vp, i64, i64, f32, i32, i64, i64, i64, i32, vp]),
@@ -192,6 +224,14 @@ def check(code, what=""):
 def ptr(t):
     """device pointer of a tensor (None -> NULL)"""
     return None if t is None else C.c_void_p(t.data_ptr())
+
+
+_HERE_AND_NOW = contextlib.nullcontext()
+
+
+def on_device(t):
+    """context in which the current device is the tensor's own (launches and `stream()` follow the current device)"""
+    return _HERE_AND_NOW if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def stream():

@@ -1,7 +1,11 @@
 """Adam / AdamW on the HIP path: torch.optim.Adam semantics (R:tasks/base.py:97,99), one streaming launch for all
 trainable tensors (`mtl_adam_step`), optionally emitting the bf16 autocast copy of a weight while it is being updated.
 
-state_dict layout matches torch.optim.Adam ("step", "exp_avg", "exp_avg_sq"), so checkpoints interchange."""
+state_dict layout matches torch.optim.Adam ("step", "exp_avg", "exp_avg_sq"), so checkpoints interchange.
+
+HipAdam(state_bits=8) holds both moments in 8 bits (`mtl_adam8_step`: 2.03 bytes of state per parameter instead of 8): state "step", "exp_avg_q", "exp_avg_sq_q" (codes of the
+parameter's shape), "q_exp" (exponents [blocks of 64, 2]). A state saved at the other width is converted at the first step after it is loaded."""
+import collections
 import ctypes as C
 
 import torch
@@ -22,8 +26,113 @@ class Bf16Shadow:
         return self.version == self.param._version
 
 
+_STATE8 = ("exp_avg_q", "exp_avg_sq_q", "q_exp")
+Adam8State = collections.namedtuple("Adam8State", ["exp_avg", "exp_avg_sq", "exponents"])
+Adam8State.__doc__ = """moments in 8 bits: uint8 codes of the first moment and of the root of the second, in the parameter's shape, and one signed exponent byte of each per block of 64
+consecutive elements, uint8 [ceil(n / 64), 2]"""
+
+
+def _check_state8(st, what):
+    n = st.exp_avg.numel()
+    ok = all(t.dtype == torch.uint8 and t.is_contiguous() for t in st) and st.exp_avg.shape == st.exp_avg_sq.shape and tuple(st.exponents.shape) == ((n + N.ADAM8_BLOCK - 1) // N.ADAM8_BLOCK, 2)
+    if not ok:
+        raise ValueError(f"{what}: an 8-bit state is contiguous uint8: two code tensors of one shape and exponents [ceil(n / 64), 2]")
+
+
+def _one_gpu(tensors, what):
+    if not all(t.is_cuda for t in tensors):
+        raise N.MtlError(f"{what} needs tensors on the GPU (no CPU fallback)")
+    if any(t.device != tensors[0].device for t in tensors):
+        raise ValueError(f"{what}: tensors on different devices")
+
+
+def adam8_state(p):
+    """the state of a parameter that has not been stepped: zero moments"""
+    return Adam8State(torch.zeros(p.shape, dtype=torch.uint8, device=p.device), torch.zeros(p.shape, dtype=torch.uint8, device=p.device),
+                      torch.zeros(((p.numel() + N.ADAM8_BLOCK - 1) // N.ADAM8_BLOCK, 2), dtype=torch.uint8, device=p.device))
+
+
+@torch.no_grad()
+def adam8_step(params, grads, states, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, decoupled_weight_decay=False, shadows=None):
+    """one Adam / AdamW step, in place, of several tensors (contiguous, f32 or bf16, gradients likewise) whose moments are Adam8States; `step` counts from 1 and is the same for all.
+    shadows: Bf16Shadow or None for each. One launch per 40 tensors. Same result for the same inputs and step, bit for bit. (In a captured graph the step number is a constant.)"""
+    params, grads, states = list(params), list(grads), list(states)
+    shadows = [None] * len(params) if shadows is None else list(shadows)
+    if not len(params) == len(grads) == len(states) == len(shadows):
+        raise ValueError("adam8_step: as many gradients, states and shadows as parameters")
+    step, (b1, b2) = int(step), betas
+    if step < 1 or not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and eps >= 0.0 and weight_decay >= 0.0):
+        raise ValueError("adam8_step: step >= 1, betas in [0, 1), eps and weight_decay not negative")
+    if not params:
+        return
+    arr = (N.Adam8Tensor * len(params))()
+    for i, (p, g, st, sh) in enumerate(zip(params, grads, states, shadows)):
+        if p.dtype not in (torch.float32, torch.bfloat16) or not p.is_contiguous() or g.dtype != p.dtype or g.shape != p.shape or not g.is_contiguous():
+            raise ValueError("adam8_step: contiguous f32 or bf16 parameters with gradients of the same type and shape")
+        _check_state8(st, "adam8_step")
+        if st.exp_avg.numel() != p.numel():
+            raise ValueError("adam8_step: a state of another size than its parameter")
+        a = arr[i]
+        a.p, a.g, a.m8, a.r8, a.ex, a.n = p.data_ptr(), g.data_ptr(), st.exp_avg.data_ptr(), st.exp_avg_sq.data_ptr(), st.exponents.data_ptr(), p.numel()
+        a.param_dtype = N.MTL_BF16 if p.dtype == torch.bfloat16 else N.MTL_F32
+        if sh is not None:
+            a.shadow, a.cols, a.ld_shadow = sh.tensor.data_ptr(), p.shape[1], sh.tensor.stride(0)
+    for name, ptrs in (("parameter", [p.data_ptr() for p in params if p.numel()]), ("state", [st.exp_avg.data_ptr() for st in states if st.exp_avg.numel()])):
+        if len(set(ptrs)) < len(ptrs):
+            raise ValueError(f"adam8_step: the same {name} twice in one step")
+    _one_gpu([t for p, g, st, sh in zip(params, grads, states, shadows) for t in (p, g, *st, *(() if sh is None else (sh.tensor,)))], "adam8_step")
+    with N.on_device(params[0]):
+        N.check(N.lib().mtl_adam8_step(arr, len(params), float(lr), float(b1), float(b2), float(eps), float(weight_decay), 1 if decoupled_weight_decay else 0, step, N.stream()), "mtl_adam8_step")
+    for p, st, sh in zip(params, states, shadows):   # the kernel wrote through raw pointers: bump the autograd versions like an in-place op
+        torch.autograd.graph.increment_version((p, *st))
+        if sh is not None:
+            sh.version = p._version
+
+
+def _state8_array(states, ms, vs):
+    arr = (N.Adam8State * len(states))()
+    for a, st, m, v in zip(arr, states, ms, vs):
+        a.m8, a.r8, a.ex, a.n = st.exp_avg.data_ptr(), st.exp_avg_sq.data_ptr(), st.exponents.data_ptr(), st.exp_avg.numel()
+        a.m, a.v, a.dtype = m.data_ptr(), v.data_ptr(), N.MTL_BF16 if m.dtype == torch.bfloat16 else N.MTL_F32
+    return arr
+
+
+@torch.no_grad()
+def adam8_moments(states, dtype=torch.float32):
+    """[(exp_avg, exp_avg_sq)] that the states' codes stand for: exact in f32; in bf16 the first moment is exact, the second rounded once"""
+    states = list(states)
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError("adam8_moments: f32 or bf16")
+    for st in states:
+        _check_state8(st, "adam8_moments")
+    if not states:
+        return []
+    _one_gpu([t for st in states for t in st], "adam8_moments")
+    with N.on_device(states[0].exp_avg):
+        out = [(torch.empty(st.exp_avg.shape, dtype=dtype, device=st.exp_avg.device), torch.empty(st.exp_avg.shape, dtype=dtype, device=st.exp_avg.device)) for st in states]
+        N.check(N.lib().mtl_adam8_moments(_state8_array(states, *zip(*out)), len(states), N.stream()), "mtl_adam8_moments")
+    return out
+
+
+@torch.no_grad()
+def adam8_quantize(exp_avg, exp_avg_sq, step=0):
+    """Adam8State of fp32 moments (`step`: how many steps they have seen; it selects the rounding thresholds)"""
+    if exp_avg.dtype != torch.float32 or exp_avg_sq.dtype != torch.float32 or exp_avg.shape != exp_avg_sq.shape or int(step) < 0:
+        raise ValueError("adam8_quantize: two fp32 moments of one shape, step not negative")
+    m, v = exp_avg.contiguous(), exp_avg_sq.contiguous()
+    _one_gpu([m, v], "adam8_quantize")
+    with N.on_device(m):
+        st = adam8_state(m)
+        N.check(N.lib().mtl_adam8_quantize(_state8_array([st], [m], [v]), 1, int(step), N.stream()), "mtl_adam8_quantize")
+    return st
+
+
 class HipAdam(torch.optim.Optimizer):
-    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, decoupled_weight_decay=False):
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, decoupled_weight_decay=False, state_bits=32):
+        """state_bits = 8: both moments of every parameter in 8 bits (see the module's docstring)"""
+        if state_bits not in (8, 32):
+            raise ValueError(f"HipAdam: state_bits is 8 or 32, got {state_bits!r}")
+        self.state_bits = state_bits
         defaults = dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, decoupled_weight_decay=decoupled_weight_decay)
         super().__init__(params, defaults)
         self._shadows = {}
@@ -61,10 +170,32 @@ class HipAdam(torch.optim.Optimizer):
             for k in ("exp_avg", "exp_avg_sq"):
                 if torch.is_tensor(rec.get(k)):
                     self.state[p][k] = rec[k].detach().to(device=p.device, dtype=torch.float32).contiguous().clone()
+            for k in _STATE8:
+                if torch.is_tensor(rec.get(k)):
+                    self.state[p][k] = rec[k].detach().to(device=p.device).contiguous().clone()
+
+    def moments(self, dtype=torch.float32):
+        """{parameter: (exp_avg, exp_avg_sq)} of every parameter that has been stepped, whatever width they are held in"""
+        held = {p: st for p, st in self.state.items() if st}
+        coded = [p for p, st in held.items() if _STATE8[0] in st]
+        out = dict(zip(coded, adam8_moments([Adam8State(*(held[p][k] for k in _STATE8)) for p in coded], dtype)))
+        return {p: out[p] if p in out else (st["exp_avg"].to(dtype), st["exp_avg_sq"].to(dtype)) for p, st in held.items()}
+
+    def _to_width(self, st, p):
+        """a state at the optimiser's own width: new, or converted from what a checkpoint of the other width held"""
+        if self.state_bits == 8 and _STATE8[0] not in st:
+            new = adam8_quantize(st.pop("exp_avg"), st.pop("exp_avg_sq"), st["step"]) if "exp_avg" in st else adam8_state(p)
+            st.update(zip(_STATE8, new))
+        elif self.state_bits == 32 and "exp_avg" not in st:
+            # moments are fp32 also for bf16 parameters (setup.dtype = "bf16"): the update is formed in fp32 and the parameter rounded once
+            st["exp_avg"], st["exp_avg_sq"] = (adam8_moments([Adam8State(*(st.pop(k) for k in _STATE8))])[0] if _STATE8[0] in st else
+                                               [torch.zeros_like(p, dtype=torch.float32, memory_format=torch.contiguous_format) for _ in range(2)])
 
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
+        if self.state_bits == 8 and torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            raise N.MtlError("HipAdam(state_bits=8).step() inside a graph capture: a replay would repeat one step number (its bias corrections and rounding thresholds)")
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
@@ -78,9 +209,7 @@ class HipAdam(torch.optim.Optimizer):
                 st = self.state[p]
                 if not st:
                     st["step"] = 0
-                    # moments are fp32 also for bf16 parameters (setup.dtype = "bf16"): the update is formed in fp32 and the parameter rounded once
-                    st["exp_avg"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.contiguous_format)
-                    st["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.contiguous_format)
+                self._to_width(st, p)
                 st["step"] = int(st["step"]) + 1
                 by_step.setdefault(st["step"], []).append(p)
             batches = []
@@ -106,7 +235,12 @@ class HipAdam(torch.optim.Optimizer):
         return loss
 
     def _launch(self, group, step, ps):
-        """one mtl_adam_step launch (all tensors of `ps`, which share `step`) on the current stream"""
+        """one mtl_adam_step / mtl_adam8_step launch (all tensors of `ps`, which share `step`) on the current stream"""
+        if self.state_bits == 8:
+            grads = [p.grad if p.grad.dtype == p.dtype and p.grad.is_contiguous() else p.grad.to(p.dtype).contiguous() for p in ps]
+            adam8_step(ps, grads, [Adam8State(*(self.state[p][k] for k in _STATE8)) for p in ps], step, group["lr"], group["betas"], group["eps"], group["weight_decay"],
+                       group["decoupled_weight_decay"], [self._shadows.get(id(p)) for p in ps])
+            return
         arr = (N.AdamTensor * len(ps))()
         keep = []
         for i, p in enumerate(ps):

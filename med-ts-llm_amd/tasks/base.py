@@ -169,7 +169,12 @@ class BaseTask(ABC):
             # same update rule as torch.optim.Adam/AdamW, one streaming launch for all tensors, and the bf16 autocast
             # copy of the big mapping weight is written by the same kernel (hip/optim.py)
             from ..hip.optim import HipAdam
-            o = HipAdam(params, lr=lr, weight_decay=0.01 if opt == "adamw" else 0.0, decoupled_weight_decay=opt == "adamw")
+            # setup.optimizer_state_bits = 8: both moments in 8 bits (2.03 bytes of state per parameter instead of 8, 16 bytes of HBM traffic per step instead of 28). A step on a
+            # part of a tensor's rows would cut its 64-element blocks elsewhere than the whole tensor's step does: not combined with the row-sharded forms.
+            bits = int(self.config.setup.get("optimizer_state_bits", 32))
+            if bits != 32 and (su is not None or getattr(self.model, "_map_shard", None) is not None):
+                raise ValueError("setup.optimizer_state_bits = 8 cannot be combined with setup.shard_optimizer / setup.shard_mapping")
+            o = HipAdam(params, lr=lr, weight_decay=0.01 if opt == "adamw" else 0.0, decoupled_weight_decay=opt == "adamw", state_bits=bits)
             if self.config.setup.get("overlap_optimizer", False) and hasattr(self.model, "late_parameters") and su is None:
                 # opt-in: the tail's parameters are read only after the backbone, their update can run on a side stream under the next step's
                 # front end + backbone. Bit-identical runs (tests/test_gpu_model.py), but measured FLAT on 1 GPU (metric step 5.57 vs 5.57-5.66 ms,
@@ -253,6 +258,8 @@ class BaseTask(ABC):
             p = by_name.get(n)
             if p is None:
                 continue
+            if "q_exp" in rec and (id(p) in owned_rows or (shard is not None and getattr(p, "_dp_sharded", False))):
+                raise ValueError(f"{n}: a checkpoint with 8-bit optimiser state cannot be resumed with row-sharded parameters (its 64-element blocks cross the rows)")
             st = {}
             for k, v in rec.items():
                 if torch.is_tensor(v) and v.dim() > 0:

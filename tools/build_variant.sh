@@ -9,7 +9,7 @@ case "$1" in only=*) ONLY=${1#only=}; shift;; esac
 R=$(cd "$(dirname "$0")/.." && pwd)
 OBJ=$R/build/obj_$TAG
 mkdir -p $OBJ $R/tools/diag
-ALL="mtl_gemm mtl_attention mtl_norm mtl_elementwise mtl_tokenizer mtl_backbone mtl_optim mtl_stats"
+ALL="mtl_gemm mtl_attention mtl_norm mtl_elementwise mtl_tokenizer mtl_backbone mtl_optim mtl_optim8 mtl_embedding mtl_qknorm mtl_stats"
 for f in $ALL; do
   # mtl_elementwise holds mtl_build_flags(): it is always rebuilt with the variant's flags, so that the variant reports what it is
   if [ -n "$ONLY" ] && [ "$f" != mtl_elementwise ] && ! echo ",$ONLY," | grep -q ",$f,"; then
