@@ -5,8 +5,8 @@
 //
 // Both are HBM-bound (one multiply or add per element moved). The gradient is a scatter-add; atomics would make it depend on the order in which workgroups run, so
 // the tokens are first SORTED by id (stable least-significant-digit radix sort of (id, position)) and every table row is then summed in position order:
-//   1. sort: up to 16384 tokens in ONE workgroup's LDS, more in tiles of 4096 (count, scan, scatter per digit). The dense gradient's zero rows are written by the other workgroups
-//      of the first launch that has a single busy workgroup: the fill (V d elements, most of the traffic for a large vocabulary) hides the sort.
+//   1. sort: up to 8192 tokens in ONE workgroup's LDS, more in tiles of 4096 (two launches per digit: count, scatter). The dense gradient's zero rows are written by the other
+//      workgroups of the first launch: the fill (V d elements, most of the traffic for a large vocabulary) hides the sort.
 //   2. sum: a wave owns a WINDOW of consecutive sorted tokens and a chunk of columns, walks the window with the running sum of the current id in registers and writes a row
 //      whenever the id changes: balanced whatever the distribution of the ids is, and no list of runs is needed. A run that crosses a window border leaves an fp32 partial per window
 //      (one slot for a run that came in, one for a run that goes out).
@@ -15,8 +15,11 @@
 
 namespace {
 
-constexpr int SORT_MAX = 16384;          // tokens that one workgroup sorts in its LDS
+// Tokens that one workgroup sorts in its LDS: 4096 14 us, 8192 24 us (16 keys per thread spill: 16384 tokens 117 us, against 29 us and three more launches in tiles).
+constexpr int SORT_MAX = 8192;
 constexpr int TILE = 4096;               // tokens per workgroup of the tiled sort
+constexpr int64_t CACHE_BYTES = (int64_t)256 << 20;      // the Infinity Cache
+constexpr int JOIN_SHORT = 16;           // windows behind its first one up to which a crossing run is joined by one wave
 constexpr int MAX_BINS = 512;            // digits of up to 9 bits: two passes for every vocabulary up to 262143
 
 // ---------------------------------------------------------------- element access: W consecutive elements <-> fp32
@@ -63,43 +66,117 @@ struct Io<bf16_t, W> {
     }
 };
 
+// W consecutive elements as loaded: held like this until they are used, so that many rows are in flight in few registers
+template <typename T, int W>
+struct Raw {
+    static constexpr int WORDS = (W * (int)sizeof(T) + 3) / 4;
+    uint32_t w[WORDS];
+    // STREAM: read once, past the caches
+    template <bool STREAM, typename V>
+    static __device__ __forceinline__ V get(const void* p) {
+        const V* v = reinterpret_cast<const V*>(p);
+        return STREAM ? __builtin_nontemporal_load(v) : *v;
+    }
+    template <bool STREAM>
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (sizeof(T) * W == 16) {
+            const u32x4 v = get<STREAM, u32x4>(p);
+            w[0] = v[0]; w[1] = v[1]; w[2] = v[2]; w[3] = v[3];
+        } else if constexpr (sizeof(T) * W == 8) {
+            const u32x2 v = get<STREAM, u32x2>(p);
+            w[0] = v[0]; w[1] = v[1];
+        } else if constexpr (sizeof(T) == 4) w[0] = get<STREAM, uint32_t>(p);
+        else w[0] = get<STREAM, uint16_t>(p);
+    }
+    __device__ __forceinline__ float at(int j) const {
+        if (sizeof(T) == 4) return __uint_as_float(w[j]);
+        return __uint_as_float((j & 1) ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16);
+    }
+};
+
 __device__ __forceinline__ int64_t load_id(const void* ids, int ids_i64, int64_t i) {
     return ids_i64 ? reinterpret_cast<const int64_t*>(ids)[i] : (int64_t)reinterpret_cast<const int32_t*>(ids)[i];
 }
 
 // ---------------------------------------------------------------- lookup
-// a wave holds 64 / LPR rows (LPR lanes per row, W columns per lane and step): narrow tables fill the wave too
+// rows narrower than a wave: 64 / LPR rows per wave (LPR lanes per row, W columns per lane and step)
 template <typename TT, typename OT, int W>
-__global__ __launch_bounds__(256) void embedding_fwd_kernel(const void* __restrict__ ids, int ids_i64, int64_t N, const TT* __restrict__ table, int64_t V, int64_t d, int64_t ld_table,
-                                                            float scale, OT* __restrict__ out, int64_t ld_out, int lpr_log2) {
+__global__ __launch_bounds__(256) void embedding_fwd_narrow_kernel(const void* __restrict__ ids, int ids_i64, int64_t N, const TT* __restrict__ table, int64_t V, int64_t d, int64_t ld_table,
+                                                                   float scale, OT* __restrict__ out, int64_t ld_out, int lpr_log2) {
     const int lpr = 1 << lpr_log2;
     const int rows_per_block = 256 >> lpr_log2;
-    const int l = threadIdx.x & (lpr - 1);
+    const int64_t c = (int64_t)(threadIdx.x & (lpr - 1)) * W;
+    if (c >= d) return;
     for (int64_t i = (int64_t)blockIdx.x * rows_per_block + (threadIdx.x >> lpr_log2); i < N; i += (int64_t)gridDim.x * rows_per_block) {
         const int64_t id = load_id(ids, ids_i64, i);
         const bool in = id >= 0 && id < V;
-        const TT* src = table + (in ? id : 0) * ld_table;
-        OT* dst = out + i * ld_out;
-#pragma unroll 4
-        for (int64_t c = (int64_t)l * W; c < d; c += (int64_t)lpr * W) {
-            float x[W];
-            Io<TT, W>::load(src, c, x);
+        float x[W];
+        Io<TT, W>::load(table + (in ? id : 0) * ld_table, c, x);
 #pragma unroll
-            for (int j = 0; j < W; ++j) x[j] = in ? x[j] * scale : 0.f;
-            Io<OT, W>::store(dst, c, x);
+        for (int j = 0; j < W; ++j) x[j] = in ? x[j] * scale : 0.f;
+        Io<OT, W>::store(out + i * ld_out, c, x);
+    }
+}
+
+// a wave owns ROWS consecutive tokens and walks their columns: ROWS loads are in flight per step (one row per wave is bound by the latency id -> row -> store). `split` > 1: few tokens,
+// a row's columns are spread over that many waves.
+template <typename TT, typename OT, int W, int ROWS>
+__global__ __launch_bounds__(256) void embedding_fwd_kernel(const void* __restrict__ ids, int ids_i64, int64_t N, const TT* __restrict__ table, int64_t V, int64_t d, int64_t ld_table, float scale,
+                                                            OT* __restrict__ out, int64_t ld_out, int split) {
+    const int lane = threadIdx.x & 63;
+    const int64_t item = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t group = item / split;
+    const int64_t i0 = group * ROWS;
+    if (i0 >= N) return;
+    const int n = N - i0 < ROWS ? (int)(N - i0) : ROWS;
+    int64_t mine = -1;
+    if (lane < n) mine = load_id(ids, ids_i64, i0 + lane);
+    const int lo = (int)mine, hi = (int)(mine >> 32);
+    const TT* src[ROWS];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+        const int64_t id = (int64_t)(uint32_t)__builtin_amdgcn_readlane(lo, r) | ((int64_t)__builtin_amdgcn_readlane(hi, r) << 32);
+        const bool in = id >= 0 && id < V;
+        src[r] = in ? table + id * ld_table : nullptr;
+    }
+    for (int64_t c = ((item - group * split) * 64 + lane) * W; c < d; c += (int64_t)64 * W * split) {
+        Raw<TT, W> x[ROWS];
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r)
+            if (src[r]) x[r].template load<false>(src[r] + c);
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            if (r >= n) break;
+            float y[W];
+#pragma unroll
+            for (int j = 0; j < W; ++j) y[j] = src[r] ? x[r].at(j) * scale : 0.f;
+            Io<OT, W>::store(out + (i0 + r) * ld_out, c, y);
         }
     }
 }
 
 // ---------------------------------------------------------------- zero rows of the dense gradient
-struct Fill { char* p; int64_t rows, row_bytes, ld_bytes; int width; };      // width: 16, 4 or 2 bytes per store
+// width: 16, 4 or 2 bytes per store. stream: the gradient is larger than the Infinity Cache (256 MB): non-temporal stores from few workgroups. 2.1 GB: ordinary stores 345 us and the sum
+// behind them 65 us (it evicts their dirty lines), non-temporal from 128 workgroups 353 and 42; 154 MB, which the cache holds: 24 us against 29 and more.
+struct Fill { char* p; int64_t rows, row_bytes, ld_bytes; int width, stream; };
 
 __device__ __forceinline__ void fill_zero(const Fill& f, int64_t block, int64_t blocks) {
     const int64_t per_row = f.row_bytes / f.width, total = f.rows * per_row;
-    const bool flat = f.row_bytes == f.ld_bytes;
+    if (f.row_bytes == f.ld_bytes && f.width == 16) {
+        u32x4* p = reinterpret_cast<u32x4*>(f.p);
+        const u32x4 zero = {0, 0, 0, 0};
+        for (int64_t i = block * 4096 + threadIdx.x; i < total; i += blocks * 4096) {       // (1024 threads, four stores each)
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (i + u * 1024 < total) {
+                    if (f.stream) __builtin_nontemporal_store(zero, p + i + u * 1024);
+                    else p[i + u * 1024] = zero;
+                }
+        }
+        return;
+    }
     for (int64_t i = block * blockDim.x + threadIdx.x; i < total; i += blocks * blockDim.x) {
-        int64_t at = i * f.width;
-        if (!flat) { const int64_t r = i / per_row; at = r * f.ld_bytes + (i - r * per_row) * f.width; }
+        const int64_t r = i / per_row, at = r * f.ld_bytes + (i - r * per_row) * f.width;
         if (f.width == 16) *reinterpret_cast<u32x4*>(f.p + at) = (u32x4){0, 0, 0, 0};
         else if (f.width == 4) *reinterpret_cast<uint32_t*>(f.p + at) = 0;
         else *reinterpret_cast<uint16_t*>(f.p + at) = 0;
@@ -192,14 +269,14 @@ __global__ __launch_bounds__(1024) void embedding_sort_small_kernel(const void* 
         return;
     }
     uint32_t* cnt = reinterpret_cast<uint32_t*>(smem);                       // [16][MAX_BINS]
-    uint32_t* tot = cnt + 16 * MAX_BINS;                                     // [16]
-    uint32_t* lkey = tot + 16;                                               // [N]
-    uint16_t* lpos = reinterpret_cast<uint16_t*>(lkey + N);                  // [N]
+    uint32_t* lkey = cnt + 16 * MAX_BINS;                                    // [max(N, 16)]
+    uint32_t* tot = lkey;                                                    // [16]: in use between the keys' reading and the next writing of them only
+    uint16_t* lpos = reinterpret_cast<uint16_t*>(lkey + (N > 16 ? N : 16)); // [N]
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int n_e = (N + 1023) >> 10;                                        // elements per thread: wave w owns [w n_e 64, (w + 1) n_e 64)
     const int i0 = wave * n_e * 64 + lane;
     const uint32_t mask = (1u << bits) - 1u;
-    if (threadIdx.x == 0) *list_n = 0;
+    if (threadIdx.x < 2) list_n[threadIdx.x] = 0;
     uint32_t key[E], rank[E], valid = 0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -234,10 +311,15 @@ __global__ __launch_bounds__(1024) void embedding_sort_small_kernel(const void* 
     }
 }
 
-// tiled sort, digit counts of each tile: hist[digit][tile]
+// tiled sort, digit counts of each tile: hist[tile][digit]. Workgroups behind the last tile write the zero rows.
 __global__ __launch_bounds__(1024) void embedding_sort_count_kernel(const void* __restrict__ ids, int ids_i64, int64_t N, int64_t V, int64_t pad, const uint32_t* __restrict__ keys, int shift, int bits,
-                                                                    uint32_t* __restrict__ hist) {
+                                                                    int tiles, uint32_t* __restrict__ hist, uint32_t* __restrict__ list_n, const Fill f) {
+    if ((int)blockIdx.x >= tiles) {
+        fill_zero(f, blockIdx.x - tiles, gridDim.x - tiles);
+        return;
+    }
     __shared__ uint32_t cnt[MAX_BINS];
+    if (list_n && blockIdx.x == 0 && threadIdx.x < 2) list_n[threadIdx.x] = 0;
     for (int i = threadIdx.x; i < MAX_BINS; i += 1024) cnt[i] = 0;
     __syncthreads();
 #pragma unroll
@@ -249,38 +331,17 @@ __global__ __launch_bounds__(1024) void embedding_sort_count_kernel(const void* 
         }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < (1 << bits); i += 1024) hist[(int64_t)i * gridDim.x + blockIdx.x] = cnt[i];
+    for (int i = threadIdx.x; i < (1 << bits); i += 1024) hist[((int64_t)blockIdx.x << bits) + i] = cnt[i];
 }
 
-// exclusive prefix over all entries of hist in place (workgroup 0); the others write the zero rows
-__global__ __launch_bounds__(1024) void embedding_sort_scan_kernel(uint32_t* __restrict__ hist, int64_t n, uint32_t* __restrict__ list_n, const Fill f) {
-    __shared__ uint32_t tot[16];
-    if (blockIdx.x > 0) {
-        fill_zero(f, blockIdx.x - 1, gridDim.x - 1);
-        return;
-    }
-    if (list_n && threadIdx.x == 0) *list_n = 0;
-    uint32_t carry = 0;
-    for (int64_t base = 0; base < n; base += 8192) {
-        uint32_t c[8], sum = 0;
-        const int64_t at = base + threadIdx.x * 8;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) { c[j] = at + j < n ? hist[at + j] : 0u; sum += c[j]; }
-        uint32_t total;
-        uint32_t x = carry + block_exclusive(sum, tot, total);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            if (at + j < n) hist[at + j] = x;
-            x += c[j];
-        }
-        carry += total;
-    }
-}
-
+// Each tile forms the first rank of its elements of every digit itself, from all tiles' counts: tokens of smaller digits plus those of the same digit in earlier tiles. (A scan by one
+// workgroup in between measured 13 - 16 us and a launch at 200 003 tokens; the counts of all tiles are 50 KB there and sit in the L2.)
 __global__ __launch_bounds__(1024) void embedding_sort_scatter_kernel(const void* __restrict__ ids, int ids_i64, int64_t N, int64_t V, int64_t pad, const uint32_t* __restrict__ keys,
-                                                                      const uint32_t* __restrict__ poss, int shift, int bits, const uint32_t* __restrict__ hist, uint32_t* __restrict__ sid,
-                                                                      uint32_t* __restrict__ spos) {
+                                                                      const uint32_t* __restrict__ poss, int shift, int bits, int tiles, const uint32_t* __restrict__ hist,
+                                                                      uint32_t* __restrict__ sid, uint32_t* __restrict__ spos) {
     __shared__ uint32_t cnt[16 * MAX_BINS];
+    __shared__ uint32_t sums[2 * 1024];
+    __shared__ uint32_t tot[16];
     constexpr int E = TILE / 1024;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     uint32_t key[E], pos[E], rank[E], valid = 0;
@@ -294,10 +355,24 @@ __global__ __launch_bounds__(1024) void embedding_sort_scatter_kernel(const void
             valid |= 1u << e;
         }
     }
+    // counts of digit threadIdx.x % bins: over every `groups`-th tile, all of them and the earlier ones
+    const int bins = 1 << bits, groups = 1024 >> bits, dgt = threadIdx.x & (bins - 1);
+    uint32_t all = 0, earlier = 0;
+#pragma unroll 8
+    for (int t = threadIdx.x >> bits; t < tiles; t += groups) {
+        const uint32_t h = hist[((int64_t)t << bits) + dgt];
+        all += h;
+        earlier += t < (int)blockIdx.x ? h : 0u;
+    }
+    sums[threadIdx.x] = all;
+    sums[1024 + threadIdx.x] = earlier;
     rank_digits<E>(key, valid, shift, bits, cnt, rank, E);
-    // counts per wave -> the tile's first rank of each digit plus the waves before
-    if (threadIdx.x < (1 << bits)) {
-        uint32_t at = hist[(int64_t)threadIdx.x * gridDim.x + blockIdx.x];
+    all = earlier = 0;
+    if ((int)threadIdx.x < bins)
+        for (int g = 0; g < groups; ++g) { all += sums[g * bins + threadIdx.x]; earlier += sums[1024 + g * bins + threadIdx.x]; }
+    uint32_t total;
+    uint32_t at = block_exclusive(all, tot, total) + earlier;
+    if ((int)threadIdx.x < bins) {
 #pragma unroll
         for (int w = 0; w < 16; ++w) {
             const uint32_t c = cnt[w * MAX_BINS + threadIdx.x];
@@ -309,9 +384,9 @@ __global__ __launch_bounds__(1024) void embedding_sort_scatter_kernel(const void
 #pragma unroll
     for (int e = 0; e < E; ++e)
         if ((valid >> e) & 1u) {
-            const uint32_t at = cnt[wave * MAX_BINS + ((key[e] >> shift) & ((1u << bits) - 1u))] + rank[e];
-            sid[at] = key[e];
-            spos[at] = pos[e];
+            const uint32_t to = cnt[wave * MAX_BINS + ((key[e] >> shift) & (bins - 1))] + rank[e];
+            sid[to] = key[e];
+            spos[to] = pos[e];
         }
 }
 
@@ -321,7 +396,7 @@ struct SumArgs {
     int64_t N, V, d, ld_dout, ld_grad;
     const void* dout; void* grad;
     float* part;                 // [windows][2][d]: 0 = the run that came into the window, 1 = the run that goes out of it (and started in it)
-    uint32_t* list; uint32_t* list_n;
+    uint32_t* list; uint32_t* list_n;      // [windows]: short runs from the front, long ones from the back; their two counts
     float scale;
     int accumulate, S, chunks;
     int64_t windows;
@@ -342,8 +417,11 @@ __device__ __forceinline__ void write_row(const SumArgs& a, uint32_t id, int64_t
     Io<GT, W>::store(a.grad, at, y);
 }
 
+// dout is read once and past the caches: 200 003 rows of 2 KB 94 us, through the caches 133 (the loads evict what the launches before left dirty there).
+// A wave holds its window's ids and positions in its lanes (one load each), picks them by lane number, and keeps two groups of GROUP rows: one being added, the next one in flight.
 template <typename DT, typename GT, int W>
 __global__ __launch_bounds__(256) void embedding_sum_kernel(const SumArgs a) {
+    constexpr int GROUP = 8;
     const int lane = threadIdx.x & 63;
     const int64_t item = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t w = item / a.chunks;
@@ -352,72 +430,115 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(const SumArgs a) {
     const bool in = c < a.d;                                    // (d % W == 0 wherever W > 1)
     const int64_t i0 = w * a.S, i1 = i0 + a.S < a.N ? i0 + a.S : a.N;
     const uint32_t none = (uint32_t)a.V;
-    uint32_t cur = a.sid[i0];
-    bool came_in = i0 > 0 && a.sid[i0 - 1] == cur;
+    uint32_t ids = none, poss = 0;
+    if (i0 + lane < i1) { ids = a.sid[i0 + lane]; poss = a.spos[i0 + lane]; }
+    const uint32_t before = i0 > 0 ? a.sid[i0 - 1] : none, after = i1 < a.N ? a.sid[i1] : none;
+    const int n = (int)__popcll(__ballot(ids != none));         // (sorted: the tokens without a gradient are the last ones)
+    if (n == 0) return;
+    const DT* dout = reinterpret_cast<const DT*>(a.dout) + (in ? c : 0);
+    uint32_t cur = (uint32_t)__builtin_amdgcn_readlane((int)ids, 0);
+    bool came_in = before == cur;
     float acc[W];
 #pragma unroll
     for (int j = 0; j < W; ++j) acc[j] = 0.f;
     float* part = a.part + w * 2 * a.d + c;
-    for (int64_t i = i0; i < i1 && cur != none; i += 8) {
-        uint32_t id[8];
-        float x[8][W];
+    Raw<DT, W> now[GROUP], next[GROUP];
+    auto fetch = [&](Raw<DT, W>(&x)[GROUP], int i) {
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            const int64_t at = i + u < i1 ? i + u : i1 - 1;      // (beyond the window: the last token again, not used)
-            id[u] = i + u < i1 ? a.sid[at] : none;
-            if (in) Io<DT, W>::load(a.dout, (int64_t)a.spos[at] * a.ld_dout + c, x[u]);
+        for (int u = 0; u < GROUP; ++u) {
+            const int at = i + u < n ? i + u : n - 1;            // (beyond the end: the last token again, not used)
+            x[u].template load<true>(dout + (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)poss, at) * a.ld_dout);
         }
+    };
+    auto add = [&](const Raw<DT, W>(&x)[GROUP], int i) {
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            if (i + u >= i1) break;
-            if (id[u] != cur) {                                  // (uniform) the run of `cur` ends here, inside the window
+        for (int u = 0; u < GROUP; ++u) {
+            if (i + u >= n) break;
+            const uint32_t id = (uint32_t)__builtin_amdgcn_readlane((int)ids, i + u);
+            if (id != cur) {                                     // (uniform) the run of `cur` ends here, inside the window
                 if (in) {
                     if (came_in) Io<float, W>::store(part, 0, acc);
                     else write_row<GT, W>(a, cur, c, acc);
                 }
-                cur = id[u];
+                cur = id;
                 came_in = false;
 #pragma unroll
                 for (int j = 0; j < W; ++j) acc[j] = 0.f;
-                if (cur == none) break;
             }
 #pragma unroll
-            for (int j = 0; j < W; ++j) acc[j] += x[u][j];
+            for (int j = 0; j < W; ++j) acc[j] += x[u].at(j);
         }
+    };
+    fetch(now, 0);
+    for (int i = 0; i < n; i += 2 * GROUP) {
+        if (i + GROUP < n) fetch(next, i + GROUP);
+        add(now, i);
+        if (i + GROUP >= n) break;
+        if (i + 2 * GROUP < n) fetch(now, i + 2 * GROUP);
+        add(next, i + GROUP);
     }
-    if (cur == none) return;
-    const bool goes_on = i1 < a.N && a.sid[i1] == cur;
-    if (!in) return;
-    if (came_in) Io<float, W>::store(part, 0, acc);
-    else if (goes_on) {
-        Io<float, W>::store(part, a.d, acc);
-        if (c == 0) a.list[atomicAdd(a.list_n, 1u)] = (uint32_t)w;      // (the list's order shows nowhere: each entry is a whole run)
-    } else write_row<GT, W>(a, cur, c, acc);
+    const bool goes_on = after == cur;
+    if (in) {
+        if (came_in) Io<float, W>::store(part, 0, acc);
+        else if (goes_on) Io<float, W>::store(part, a.d, acc);
+        else write_row<GT, W>(a, cur, c, acc);
+    }
+    // the window in which a crossing run starts goes on a list (whose order shows nowhere: each entry is a whole run): LONG of runs that cover more than JOIN_SHORT windows behind it
+    if (goes_on && !came_in && c == 0) {
+        const int64_t far = i1 + (int64_t)JOIN_SHORT * a.S;
+        if (far < a.N && a.sid[far] == cur) a.list[a.windows - 1 - atomicAdd(a.list_n + 1, 1u)] = (uint32_t)w;
+        else a.list[atomicAdd(a.list_n, 1u)] = (uint32_t)w;
+    }
 }
 
-// the run that starts in window list[k] and goes on: tail partial of that window, then the head partials of the following ones up to the window where it ends. Four waves take a
-// quarter of the windows each, in order, and are joined in order.
-template <typename GT>
-__global__ __launch_bounds__(256) void embedding_join_kernel(const SumArgs a, int chunks) {
-    __shared__ float sums[4][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t items = (int64_t)*a.list_n * chunks;
-    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const int64_t w = a.list[item / chunks];
+// number of windows behind w that the run of `id` reaches into, given that it goes on behind w: 64 windows looked at per step
+__device__ __forceinline__ int64_t run_windows(const SumArgs& a, int64_t w, uint32_t id) {
+    const int lane = threadIdx.x & 63;
+    for (int64_t n = 1;; n += 64) {
+        const int64_t end = (w + n + lane + 1) * a.S;             // does the run go on behind window w + n + lane?
+        const uint64_t stops = __ballot(!(end < a.N && a.sid[end] == id));
+        if (stops) return n + __ffsll((unsigned long long)stops) - 1;
+    }
+}
+
+// The runs that cross window borders: tail partial of the window where the run starts, then the head partials of the following windows, in order. Short runs: a wave each per 256
+// columns. Long ones: a workgroup per 64 columns, its 16 waves take a sixteenth of the windows each and are joined in order.
+template <typename GT, int W>
+__global__ __launch_bounds__(1024) void embedding_join_kernel(const SumArgs a, int long_blocks) {
+    __shared__ float sums[16][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if ((int)blockIdx.x >= long_blocks) {
+        const int chunks = (int)((a.d + 64 * W - 1) / (64 * W));
+        const int64_t items = (int64_t)a.list_n[0] * chunks, step = (int64_t)(gridDim.x - long_blocks) * 16;
+        for (int64_t item = (int64_t)(blockIdx.x - long_blocks) * 16 + wave; item < items; item += step) {
+            const int64_t w = a.list[item / chunks];
+            const int64_t c = (item % chunks) * (64 * W) + lane * W;
+            const uint32_t id = a.sid[(w + 1) * a.S];
+            const int n = (int)run_windows(a, w, id);
+            if (c >= a.d) continue;
+            const float* part = a.part + w * 2 * a.d + c;
+            float s[W];
+            Io<float, W>::load(part, a.d, s);
+#pragma unroll 4
+            for (int k = 1; k <= n; ++k) {
+                float x[W];
+                Io<float, W>::load(part, (int64_t)k * 2 * a.d, x);
+#pragma unroll
+                for (int j = 0; j < W; ++j) s[j] += x[j];
+            }
+            write_row<GT, W>(a, id, c, s);
+        }
+        return;
+    }
+    const int chunks = (int)((a.d + 63) / 64);
+    const int64_t items = (int64_t)a.list_n[1] * chunks;
+    for (int64_t item = blockIdx.x; item < items; item += long_blocks) {
+        const int64_t w = a.list[a.windows - 1 - item / chunks];
         const int64_t c = (item % chunks) * 64 + lane;
         const bool in = c < a.d;
         const uint32_t id = a.sid[(w + 1) * a.S];
-        int64_t last = w + 1;                                     // the window in which the run ends
-        for (;;) {                                                // 64 windows at a time: does the run go on behind window last + lane?
-            const int64_t k = last + lane;
-            const int64_t end = (k + 1) * a.S;
-            const bool on = end < a.N && a.sid[end] == id;
-            const uint64_t stops = __ballot(!on);
-            if (stops) { last += __ffsll((unsigned long long)stops) - 1; break; }
-            last += 64;
-        }
-        const int64_t n = last - w;                               // head partials of windows w + 1 .. last
-        const int64_t k0 = w + 1 + n * wave / 4, k1 = w + 1 + n * (wave + 1) / 4;
+        const int64_t n = run_windows(a, w, id);
+        const int64_t k0 = w + 1 + n * wave / 16, k1 = w + 1 + n * (wave + 1) / 16;
         float s = wave == 0 && in ? a.part[w * 2 * a.d + a.d + c] : 0.f;
         if (in) {
 #pragma unroll 8
@@ -426,7 +547,9 @@ __global__ __launch_bounds__(256) void embedding_join_kernel(const SumArgs a, in
         sums[wave][lane] = s;
         __syncthreads();
         if (wave == 0 && in) {
-            const float t[1] = {((sums[0][lane] + sums[1][lane]) + sums[2][lane]) + sums[3][lane]};
+            float t[1] = {sums[0][lane]};
+#pragma unroll
+            for (int v = 1; v < 16; ++v) t[0] += sums[v][lane];
             write_row<GT, 1>(a, id, c, t);
         }
         __syncthreads();
@@ -469,28 +592,44 @@ inline Plan plan_for(int64_t N, int64_t V, int64_t d) {
 template <int E>
 void launch_sort_small(const void* ids, int ids_i64, int N, int64_t V, int64_t pad, int passes, int bits, uint32_t* sid, uint32_t* spos, uint32_t* list_n, const Fill& f, unsigned fill_blocks,
                        hipStream_t st) {
-    const size_t fixed = (16 * MAX_BINS + 16) * 4;
+    const size_t fixed = 16 * MAX_BINS * 4;                       // (8192 tokens: 80 KB, two workgroups per CU write zeros)
     (void)hipFuncSetAttribute((const void*)embedding_sort_small_kernel<E>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)(fixed + E * 1024 * 6));
-    hipLaunchKernelGGL(embedding_sort_small_kernel<E>, dim3(1 + fill_blocks), dim3(1024), fixed + (size_t)N * 6, st, ids, ids_i64, N, V, pad, passes, bits, sid, spos, list_n, f);
+    hipLaunchKernelGGL(embedding_sort_small_kernel<E>, dim3(1 + fill_blocks), dim3(1024), fixed + (size_t)(N > 16 ? N : 16) * 6, st, ids, ids_i64, N, V, pad, passes, bits, sid, spos, list_n, f);
 }
 
 template <typename DT, typename GT>
 void launch_sum(const SumArgs& a, int W, hipStream_t st) {
     const unsigned blocks = (unsigned)((a.windows * a.chunks + 3) / 4);
-    if (W == 8) hipLaunchKernelGGL((embedding_sum_kernel<DT, GT, 8>), dim3(blocks), dim3(256), 0, st, a);
+    constexpr int WIDE = 16 / sizeof(DT);                          // 16 bytes of dout per lane
+    if (W == 8 && WIDE == 8) hipLaunchKernelGGL((embedding_sum_kernel<DT, GT, WIDE>), dim3(blocks), dim3(256), 0, st, a);
     else if (W == 4) hipLaunchKernelGGL((embedding_sum_kernel<DT, GT, 4>), dim3(blocks), dim3(256), 0, st, a);
     else hipLaunchKernelGGL((embedding_sum_kernel<DT, GT, 1>), dim3(blocks), dim3(256), 0, st, a);
 }
 
+template <typename TT, typename OT, int W>
+void launch_fwd_w(const void* ids, int ids_i64, int64_t N, const void* table, int64_t V, int64_t d, int64_t ld_table, float scale, void* out, int64_t ld_out, hipStream_t st) {
+    if (d <= 32 * W) {
+        int lpr = 0;
+        while (((int64_t)W << lpr) < d) ++lpr;
+        const int64_t rows = 256 >> lpr, want = (N + rows - 1) / rows;
+        hipLaunchKernelGGL((embedding_fwd_narrow_kernel<TT, OT, W>), dim3((unsigned)(want < 65536 ? want : 65536)), dim3(256), 0, st, ids, ids_i64, N, (const TT*)table, V, d, ld_table, scale, (OT*)out,
+                           ld_out, lpr);
+        return;
+    }
+    if (N >= 4 * 4096) {       // enough tokens that four per wave still fill the chip
+        const int64_t waves = (N + 3) / 4;
+        hipLaunchKernelGGL((embedding_fwd_kernel<TT, OT, W, 4>), dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, st, ids, ids_i64, N, (const TT*)table, V, d, ld_table, scale, (OT*)out, ld_out, 1);
+        return;
+    }
+    int64_t split = (d + 64 * W - 1) / (64 * W);
+    while (split > 1 && N * split > 16384) split = (split + 1) / 2;
+    hipLaunchKernelGGL((embedding_fwd_kernel<TT, OT, W, 1>), dim3((unsigned)((N * split + 3) / 4)), dim3(256), 0, st, ids, ids_i64, N, (const TT*)table, V, d, ld_table, scale, (OT*)out, ld_out, (int)split);
+}
 template <typename TT, typename OT>
 void launch_fwd(const void* ids, int ids_i64, int64_t N, const void* table, int64_t V, int64_t d, int64_t ld_table, float scale, void* out, int64_t ld_out, int W, hipStream_t st) {
-    int lpr = 0;
-    while (lpr < 6 && ((int64_t)W << lpr) < d) ++lpr;
-    const int64_t rows = 256 >> lpr, want = (N + rows - 1) / rows;
-    const unsigned blocks = (unsigned)(want < 65536 ? want : 65536);
-    if (W == 8) hipLaunchKernelGGL((embedding_fwd_kernel<TT, OT, 8>), dim3(blocks), dim3(256), 0, st, ids, ids_i64, N, (const TT*)table, V, d, ld_table, scale, (OT*)out, ld_out, lpr);
-    else if (W == 4) hipLaunchKernelGGL((embedding_fwd_kernel<TT, OT, 4>), dim3(blocks), dim3(256), 0, st, ids, ids_i64, N, (const TT*)table, V, d, ld_table, scale, (OT*)out, ld_out, lpr);
-    else hipLaunchKernelGGL((embedding_fwd_kernel<TT, OT, 1>), dim3(blocks), dim3(256), 0, st, ids, ids_i64, N, (const TT*)table, V, d, ld_table, scale, (OT*)out, ld_out, lpr);
+    if (W == 8 && sizeof(TT) == 2 && sizeof(OT) == 2) launch_fwd_w<TT, OT, (sizeof(TT) == 2 && sizeof(OT) == 2) ? 8 : 4>(ids, ids_i64, N, table, V, d, ld_table, scale, out, ld_out, st);
+    else if (W == 4) launch_fwd_w<TT, OT, 4>(ids, ids_i64, N, table, V, d, ld_table, scale, out, ld_out, st);
+    else launch_fwd_w<TT, OT, 1>(ids, ids_i64, N, table, V, d, ld_table, scale, out, ld_out, st);
 }
 
 inline bool dtype_ok(int t) { return t == MTL_F32 || t == MTL_BF16; }
@@ -537,15 +676,16 @@ extern "C" int mtl_embedding_bwd(const void* ids, int ids_i64, int64_t N, const 
     if (N > 0 && workspace_bytes < mtl_embedding_bwd_workspace_bytes(N, V, d)) return MTL_ERR_WORKSPACE;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     if (padding_idx < 0) padding_idx = -1;
-    Fill f = {(char*)grad, accumulate ? 0 : V, d * gs, ld_grad * gs, 2};
+    Fill f = {(char*)grad, accumulate ? 0 : V, d * gs, ld_grad * gs, 2, V * d * gs > CACHE_BYTES};
     for (int w : {4, 16})
         if (f.row_bytes % w == 0 && f.ld_bytes % w == 0 && ((uintptr_t)grad & (w - 1)) == 0) f.width = w;
     const int64_t fill_items = f.rows * (f.row_bytes / f.width);
-    const unsigned fill_blocks = (unsigned)(fill_items == 0 ? 0 : ((fill_items + 1023) / 1024 < 1024 ? (fill_items + 1023) / 1024 : 1024));
+    const int64_t fill_want = (fill_items + 4095) / 4096, fill_most = f.stream ? 128 : 512;
+    const unsigned fill_blocks = (unsigned)(fill_want < fill_most ? fill_want : fill_most);
     char* ws = reinterpret_cast<char*>(workspace);
     if (N == 0) {
-        // no token: zeros only, through the scan kernel with an empty histogram (its counter lives in a workspace that may be NULL here)
-        hipLaunchKernelGGL(embedding_sort_scan_kernel, dim3(1 + fill_blocks), dim3(1024), 0, st, (uint32_t*)nullptr, (int64_t)0, (uint32_t*)nullptr, f);
+        // no token: zeros only (no tile to count)
+        hipLaunchKernelGGL(embedding_sort_count_kernel, dim3(fill_blocks), dim3(1024), 0, st, ids, ids_i64, N, V, padding_idx, (const uint32_t*)nullptr, 0, 1, 0, (uint32_t*)nullptr, (uint32_t*)nullptr, f);
         MTL_CHECK_LAUNCH();
         return MTL_OK;
     }
@@ -556,8 +696,7 @@ extern "C" int mtl_embedding_bwd(const void* ids, int ids_i64, int64_t N, const 
     const int passes = passes_for(V), bits = bits_per_pass(V);
     if (N <= SORT_MAX) {
         if (N <= 4096) launch_sort_small<4>(ids, ids_i64, (int)N, V, padding_idx, passes, bits, sid, spos, list_n, f, fill_blocks, st);
-        else if (N <= 8192) launch_sort_small<8>(ids, ids_i64, (int)N, V, padding_idx, passes, bits, sid, spos, list_n, f, fill_blocks, st);
-        else launch_sort_small<16>(ids, ids_i64, (int)N, V, padding_idx, passes, bits, sid, spos, list_n, f, fill_blocks, st);
+        else launch_sort_small<8>(ids, ids_i64, (int)N, V, padding_idx, passes, bits, sid, spos, list_n, f, fill_blocks, st);
         MTL_CHECK_LAUNCH();
     } else {
         uint32_t* hist = reinterpret_cast<uint32_t*>(ws + p.hist);
@@ -569,17 +708,15 @@ extern "C" int mtl_embedding_bwd(const void* ids, int ids_i64, int64_t N, const 
             const bool to_first = ((passes - 1 - q) & 1) == 0;                 // the last pass ends in sid / spos
             uint32_t* ko = to_first ? sid : other_id;
             uint32_t* po = to_first ? spos : other_pos;
-            hipLaunchKernelGGL(embedding_sort_count_kernel, dim3(tiles), dim3(1024), 0, st, ids, ids_i64, N, V, padding_idx, kin, q * bits, bits, hist);
-            const Fill none = {nullptr, 0, 16, 16, 16};
-            hipLaunchKernelGGL(embedding_sort_scan_kernel, dim3(1 + (q == 0 ? fill_blocks : 0)), dim3(1024), 0, st, hist, (int64_t)tiles << bits, list_n, q == 0 ? f : none);
-            hipLaunchKernelGGL(embedding_sort_scatter_kernel, dim3(tiles), dim3(1024), 0, st, ids, ids_i64, N, V, padding_idx, kin, pin, q * bits, bits, hist, ko, po);
+            hipLaunchKernelGGL(embedding_sort_count_kernel, dim3(tiles + (q == 0 ? fill_blocks : 0)), dim3(1024), 0, st, ids, ids_i64, N, V, padding_idx, kin, q * bits, bits, (int)tiles, hist, list_n, f);
+            hipLaunchKernelGGL(embedding_sort_scatter_kernel, dim3(tiles), dim3(1024), 0, st, ids, ids_i64, N, V, padding_idx, kin, pin, q * bits, bits, (int)tiles, hist, ko, po);
             MTL_CHECK_LAUNCH();
             kin = ko; pin = po;
         }
     }
     int W = 1;
     for (int c : {4, 8})
-        if (d > 64 * (c / 4) && fits(dout, ld_dout, dout_dtype, d, c) && fits(grad, ld_grad, grad_dtype, d, c) && (c == 4 || d % 512 == 0 || d >= 2048)) W = c;
+        if (d > 64 * (c / 4) && fits(dout, ld_dout, dout_dtype, d, c) && fits(grad, ld_grad, grad_dtype, d, c) && (c == 4 || (dout_dtype == MTL_BF16 && (d % 512 == 0 || d >= 2048)))) W = c;
     SumArgs a;
     a.sid = sid; a.spos = spos; a.N = N; a.V = V; a.d = d; a.ld_dout = ld_dout; a.ld_grad = ld_grad; a.dout = dout; a.grad = grad;
     a.part = reinterpret_cast<float*>(ws + p.part); a.list = reinterpret_cast<uint32_t*>(ws + p.list); a.list_n = list_n;
@@ -595,11 +732,13 @@ extern "C" int mtl_embedding_bwd(const void* ids, int ids_i64, int64_t N, const 
     else launch_sum<float, float>(a, W, st);
     MTL_CHECK_LAUNCH();
     if (a.windows > 1) {
-        const int jc = (int)chunks_of(d, 1);
-        const int64_t most = (a.windows - 1) * jc;
-        const unsigned blocks = (unsigned)(most < 2048 ? most : 2048);
-        if (g16) hipLaunchKernelGGL(embedding_join_kernel<bf16_t>, dim3(blocks), dim3(256), 0, st, a, jc);
-        else hipLaunchKernelGGL(embedding_join_kernel<float>, dim3(blocks), dim3(256), 0, st, a, jc);
+        const int64_t most = ((a.windows - 1) * chunks_of(d, W > 4 ? 4 : W) + 15) / 16;      // waves of 16 short runs' column chunks
+        const int64_t most_long = (a.windows / (JOIN_SHORT + 1)) * chunks_of(d, 1);           // a long run takes at least that many windows
+        const unsigned lb = (unsigned)(most_long < 256 ? most_long : 256), sb = (unsigned)(most < 256 ? most : 256);
+        if (W > 1 && g16) hipLaunchKernelGGL((embedding_join_kernel<bf16_t, 4>), dim3(lb + sb), dim3(1024), 0, st, a, (int)lb);
+        else if (W > 1) hipLaunchKernelGGL((embedding_join_kernel<float, 4>), dim3(lb + sb), dim3(1024), 0, st, a, (int)lb);
+        else if (g16) hipLaunchKernelGGL((embedding_join_kernel<bf16_t, 1>), dim3(lb + sb), dim3(1024), 0, st, a, (int)lb);
+        else hipLaunchKernelGGL((embedding_join_kernel<float, 1>), dim3(lb + sb), dim3(1024), 0, st, a, (int)lb);
         MTL_CHECK_LAUNCH();
     }
     return MTL_OK;

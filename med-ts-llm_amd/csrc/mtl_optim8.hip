@@ -20,8 +20,11 @@ namespace {
 
 constexpr int MAX_T = MTL_ADAM8_MAX_TENSORS;
 constexpr int THREADS = 256;
-constexpr int ITERS = 4;                                       // 4 elements per lane and iteration: all loads of a chunk are in flight before the first use
-constexpr int CHUNK = THREADS * 4 * ITERS;                     // elements per workgroup: a whole number of 64-element blocks
+// 4 elements per lane and iteration; all loads of a workgroup's iterations are in flight before the first use. Iterations, measured at 512 M elements: fp32 step 1 / 2 / 4: 1351 / 1475 /
+// 1413 us (6.1 TB/s); bf16 step 1066 / 968 / 1046 (5.3 TB/s: half of the bytes per element, the arithmetic shows); read-back 594 / 502 / 541.
+constexpr int ITERS_F32 = 1, ITERS_B16 = 2, ITERS_STATE = 2;
+constexpr int chunk_of(int iters) { return THREADS * 4 * iters; }      // elements per workgroup: a whole number of 64-element blocks
+inline int step_chunk(int64_t dtype) { return chunk_of(dtype == MTL_BF16 ? ITERS_B16 : ITERS_F32); }
 
 struct Adam8Table {
     mtl_adam8_tensor t[MAX_T];
@@ -50,19 +53,34 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v) {
     v = row_max_step<0x124>(v);
     return row_max_step<0x128>(v);
 }
+__device__ __forceinline__ uint32_t max4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) { const uint32_t x = a > b ? a : b, y = c > d ? c : d; return x > y ? x : y; }
+__device__ __forceinline__ uint32_t min4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) { const uint32_t x = a < b ? a : b, y = c < d ? c : d; return x < y ? x : y; }
+constexpr uint32_t INF_BITS = 0x7f800000u;
 // bits of |x|, 0 where it is not finite: ordered like the values
 __device__ __forceinline__ uint32_t finite_bits(float x) {
     const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
-    return b < 0x7f800000u ? b : 0u;
+    return b < INF_BITS ? b : 0u;
 }
 __device__ __forceinline__ int scale_exp(uint32_t top_bits, int below) {
     const int e = (int)(top_bits >> 23) - 127 - below;
     return e < -126 ? -126 : e;                                // (the largest is 127 - 7)
 }
+__device__ __forceinline__ bool has_zero_byte(uint32_t x) { return ((x - 0x01010101u) & ~x & 0x80808080u) != 0; }
 
-__device__ __forceinline__ void decode4(uint32_t cm, uint32_t cr, float sm, float sr, float (&m)[4], float (&r)[4]) {
+// The general forms of decoding and encoding handle every value; the step is bound by its arithmetic with them (bf16: 180 vector operations per element, 4.2 TB/s). What almost every wave
+// meets are finite values within 2^13 of their block's largest, and for those the codes are fields of the fp32 numbers: u44(c) 2^er = bits (c + 2080 + 16 er) << 19 for c >= 16, and
+// the threshold is added below the four mantissa bits that stay. A wave takes that path where all its values allow it (a uniform branch), with the same bits.
+__device__ __forceinline__ void decode4(uint32_t cm, uint32_t cr, int em, int er, float (&m)[4], float (&r)[4]) {
+    const float sm = pow2i(em);
     m[0] = __builtin_amdgcn_cvt_f32_fp8((int)cm, 0) * sm; m[1] = __builtin_amdgcn_cvt_f32_fp8((int)cm, 1) * sm;
     m[2] = __builtin_amdgcn_cvt_f32_fp8((int)cm, 2) * sm; m[3] = __builtin_amdgcn_cvt_f32_fp8((int)cm, 3) * sm;
+    if (!__any(has_zero_byte(cr & 0xf0f0f0f0u) || has_zero_byte(~cr))) {      // no code below 16, no 255
+        const uint32_t k = (uint32_t)(130 * 16 + 16 * er);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] = __uint_as_float((((cr >> (8 * e)) & 0xffu) + k) << 19);
+        return;
+    }
+    const float sr = pow2i(er);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         const uint32_t c = (cr >> (8 * e)) & 0xffu;
@@ -78,29 +96,59 @@ __device__ __forceinline__ uint32_t encode_root(float r, float inv, uint32_t u) 
     const uint32_t small = (uint32_t)__builtin_floorf(y + (float)(u >> 8) * 0x1p-24f);
     uint32_t c = y >= 16.0f ? large : small;
     c = (r > 0.f && c < 1u) ? 1u : c;
-    return (__float_as_uint(r) & 0x7f800000u) == 0x7f800000u ? 255u : c;
+    return (__float_as_uint(r) & INF_BITS) == INF_BITS ? 255u : c;
 }
 
-// codes of 4 elements and the block's exponents (the same in the 16 lanes of a block); every lane of the wave is active
-__device__ __forceinline__ void encode4(const float (&m)[4], const float (&r)[4], uint32_t idx, uint32_t t_thr, uint32_t& cm, uint32_t& cr, uint32_t& ex) {
-    uint32_t tm = 0, tr = 0;
+// square root, rounded to nearest, of 0 and of x >= 2^-96: the hardware's estimate is off by at most one unit in the last place; the residuals of its two neighbours decide
+__device__ __forceinline__ float sqrt_near(float x) {
+    float s = __builtin_amdgcn_sqrtf(x);
+    const float down = __uint_as_float(__float_as_uint(s) - 1u), up = __uint_as_float(__float_as_uint(s) + 1u);
+    const float rd = __builtin_fmaf(-down, s, x), ru = __builtin_fmaf(-up, s, x);
+    s = rd <= 0.f ? down : s;
+    return ru > 0.f ? up : s;
+}
+
+constexpr uint32_t DITHER_I = 0xC13FA9A9u;
+
+// Codes of 4 elements and the block's exponents (the same in the 16 lanes of a block) from m and v; r[] receives sqrt(v). Every lane of the wave is active.
+__device__ __forceinline__ void encode4(const float (&m)[4], const float (&v)[4], float (&r)[4], uint32_t idx, uint32_t t_thr, uint32_t& cm, uint32_t& cr, uint32_t& ex) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const uint32_t a = finite_bits(m[e]), b = finite_bits(r[e]);
-        tm = a > tm ? a : tm;
-        tr = b > tr ? b : tr;
+    for (int e = 0; e < 4; ++e) r[e] = sqrt_near(v[e]);
+    uint32_t mb[4], rb[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { mb[e] = __float_as_uint(m[e]) & 0x7fffffffu; rb[e] = __float_as_uint(r[e]); }
+    uint32_t tm = row_max(max4(mb[0], mb[1], mb[2], mb[3])), tr = row_max(max4(rb[0], rb[1], rb[2], rb[3]));
+    int em = scale_exp(tm, 7), er = scale_exp(tr, 17);
+    const uint32_t u0 = idx * DITHER_I + t_thr;
+    // 16 in the block's scale, and 2^-48: smaller roots come from v < 2^-96, for which sqrt_near is not exact
+    const uint32_t least = (uint32_t)(131 + er) << 23, lo = least > 0x27800000u ? least : 0x27800000u;
+    if (__any(tm >= INF_BITS || tr >= INF_BITS || min4(rb[0], rb[1], rb[2], rb[3]) < lo)) {
+        tm = tr = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            r[e] = __builtin_sqrtf(v[e]);
+            const uint32_t a = finite_bits(m[e]), b = finite_bits(r[e]);
+            tm = a > tm ? a : tm;
+            tr = b > tr ? b : tr;
+        }
+        em = scale_exp(row_max(tm), 7); er = scale_exp(row_max(tr), 17);
+        cr = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) cr |= encode_root(r[e], pow2i(-er), u0 + (uint32_t)e * DITHER_I) << (8 * e);
+    } else {
+        const uint32_t k = (uint32_t)(130 * 16 + 16 * er);
+        cr = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) cr |= (((rb[e] + ((u0 + (uint32_t)e * DITHER_I) >> 13)) >> 19) - k) << (8 * e);
     }
-    const int em = scale_exp(row_max(tm), 7), er = scale_exp(row_max(tr), 17);
-    const float im = pow2i(-em), ir = pow2i(-er);
+    const float im = pow2i(-em);
     int pk = __builtin_amdgcn_cvt_pk_fp8_f32(m[0] * im, m[1] * im, 0, false);
     pk = __builtin_amdgcn_cvt_pk_fp8_f32(m[2] * im, m[3] * im, pk, true);
     cm = (uint32_t)pk;
-    cr = 0;
+    if (__any(max4(mb[0], mb[1], mb[2], mb[3]) >= INF_BITS))
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        if ((__float_as_uint(m[e]) & 0x7f800000u) == 0x7f800000u) cm = (cm & ~(0xffu << (8 * e))) | (0x7fu << (8 * e));
-        cr |= encode_root(r[e], ir, (idx + (uint32_t)e) * 0xC13FA9A9u + t_thr) << (8 * e);
-    }
+        for (int e = 0; e < 4; ++e)
+            if (mb[e] >= INF_BITS) cm = (cm & ~(0xffu << (8 * e))) | (0x7fu << (8 * e));
     ex = ((uint32_t)em & 0xffu) | (((uint32_t)er & 0xffu) << 8);
 }
 
@@ -120,18 +168,17 @@ __device__ __forceinline__ void store_codes(uint8_t* p, uint32_t c, int nv, bool
         if (e < nv) p[e] = (uint8_t)(c >> (8 * e));
 }
 
-__device__ __forceinline__ void adam8_one(float& p, float g, float& m, float& r, const Adam8Hyper& h) {
-    float v = r * r;
+// new moments (v: the second moment itself), and the update once their root is known
+__device__ __forceinline__ void adam8_moments_of(float& p, float g, float& m, float r, float& v, const Adam8Hyper& h) {
+    v = r * r;
     if (h.mode == 2) p = p * h.decay;
     else if (h.mode == 1) g = g + p * h.wd;
     m = m + (g - m) * h.om_b1;
     v = v * h.b2 + (g * g) * h.om_b2;
-    r = __builtin_sqrtf(v);
-    const float denom = r * h.inv_bc2 + h.eps;
-    p = p - (m / denom) * h.step_size;
 }
+__device__ __forceinline__ float adam8_update(float p, float m, float r, const Adam8Hyper& h) { return p - (m / (r * h.inv_bc2 + h.eps)) * h.step_size; }
 
-// HBM-bound: fp32 16 + 2/32 B per element (p read and written, g read, two code bytes read and written, two exponent bytes per 64 elements each way), bf16 10 + 2/32.
+// HBM-bound: fp32 16 + 4/64 B per element (p read and written, g read, two code bytes read and written, two exponent bytes per 64 elements each way), bf16 10 + 4/64.
 template <bool P16>
 __device__ __forceinline__ void adam8_chunk(const mtl_adam8_tensor& t, int64_t base, const Adam8Hyper& h) {
     float* p32 = reinterpret_cast<float*>(t.p);
@@ -140,6 +187,7 @@ __device__ __forceinline__ void adam8_chunk(const mtl_adam8_tensor& t, int64_t b
     const bf16_t* g16 = reinterpret_cast<const bf16_t*>(t.g);
     const bool vec = (((uintptr_t)t.p | (uintptr_t)t.g) & (P16 ? 7 : 15)) == 0;
     const bool vec8 = (((uintptr_t)t.m8 | (uintptr_t)t.r8) & 3) == 0;
+    constexpr int ITERS = P16 ? ITERS_B16 : ITERS_F32;
     float pp[ITERS][4], gg[ITERS][4];
     uint32_t cm[ITERS], cr[ITERS], ex[ITERS];
 #pragma unroll
@@ -181,15 +229,17 @@ __device__ __forceinline__ void adam8_chunk(const mtl_adam8_tensor& t, int64_t b
         const int64_t e0 = base + ((int64_t)i * THREADS + threadIdx.x) * 4;
         const int64_t left = t.n - e0;
         const int nv = left >= 4 ? 4 : (left > 0 ? (int)left : 0);
-        float m[4], r[4];
-        decode4(cm[i], cr[i], pow2i((int8_t)(ex[i] & 0xffu)), pow2i((int8_t)(ex[i] >> 8)), m, r);
+        float m[4], r[4], v[4];
+        decode4(cm[i], cr[i], (int8_t)(ex[i] & 0xffu), (int8_t)(ex[i] >> 8), m, r);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            adam8_one(pp[i][e], gg[i][e], m[e], r[e], h);
-            if (e >= nv) m[e] = r[e] = 0.f;                     // (elements behind the tensor's end have no part in their block's scales)
+            adam8_moments_of(pp[i][e], gg[i][e], m[e], r[e], v[e], h);
+            if (e >= nv) m[e] = v[e] = 0.f;                     // (elements behind the tensor's end have no part in their block's scales)
         }
         uint32_t nm, nr, nx;
-        encode4(m, r, (uint32_t)e0, h.t_thr, nm, nr, nx);
+        encode4(m, v, r, (uint32_t)e0, h.t_thr, nm, nr, nx);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) pp[i][e] = adam8_update(pp[i][e], m[e], r[e], h);
         if (nv == 0) continue;                                  // (no cross-lane operation below)
         store_codes(t.m8 + e0, nm, nv, vec8);
         store_codes(t.r8 + e0, nr, nv, vec8);
@@ -226,9 +276,9 @@ __global__ __launch_bounds__(THREADS) void adam8_step_kernel(const Adam8Table ta
     const int b = blockIdx.x;
     while (ti + 1 < tab.count && b >= tab.first_block[ti + 1]) ++ti;
     const mtl_adam8_tensor t = tab.t[ti];
-    const int64_t base = (int64_t)(b - tab.first_block[ti]) * CHUNK;
-    if (t.param_dtype == MTL_BF16) adam8_chunk<true>(t, base, h);
-    else adam8_chunk<false>(t, base, h);
+    const int64_t at = b - tab.first_block[ti];
+    if (t.param_dtype == MTL_BF16) adam8_chunk<true>(t, at * chunk_of(ITERS_B16), h);
+    else adam8_chunk<false>(t, at * chunk_of(ITERS_F32), h);
 }
 
 __device__ __forceinline__ void store_moment(void* dst, int64_t e0, int nv, const float (&x)[4], bool b16) {
@@ -253,16 +303,28 @@ __global__ __launch_bounds__(THREADS) void adam8_moments_kernel(const State8Tabl
     const int b = blockIdx.x;
     while (ti + 1 < tab.count && b >= tab.first_block[ti + 1]) ++ti;
     const mtl_adam8_state t = tab.t[ti];
-    const int64_t base = (int64_t)(b - tab.first_block[ti]) * CHUNK;
+    constexpr int ITERS = ITERS_STATE;
+    const int64_t base = (int64_t)(b - tab.first_block[ti]) * chunk_of(ITERS);
     const bool vec8 = (((uintptr_t)t.m8 | (uintptr_t)t.r8) & 3) == 0;
+    uint32_t cm[ITERS], cr[ITERS], ex[ITERS];
 #pragma unroll
     for (int i = 0; i < ITERS; ++i) {
-        const int64_t e0 = base + ((int64_t)i * THREADS + threadIdx.x) * 4;
-        if (e0 >= t.n) break;
-        const int nv = t.n - e0 >= 4 ? 4 : (int)(t.n - e0);
-        const uint32_t ex = *reinterpret_cast<const uint16_t*>(t.ex + (e0 >> 6) * 2);
+        const int64_t e0 = base + ((int64_t)i * THREADS + threadIdx.x) * 4, left = t.n - e0;
+        const int nv = left >= 4 ? 4 : (left > 0 ? (int)left : 0);
+        cm[i] = cr[i] = ex[i] = 0;
+        if (nv > 0) {
+            ex[i] = *reinterpret_cast<const uint16_t*>(t.ex + (e0 >> 6) * 2);
+            cm[i] = load_codes(t.m8 + e0, nv, vec8);
+            cr[i] = load_codes(t.r8 + e0, nv, vec8);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < ITERS; ++i) {
+        const int64_t e0 = base + ((int64_t)i * THREADS + threadIdx.x) * 4, left = t.n - e0;
+        const int nv = left >= 4 ? 4 : (left > 0 ? (int)left : 0);
+        if (nv == 0) break;
         float m[4], r[4], v[4];
-        decode4(load_codes(t.m8 + e0, nv, vec8), load_codes(t.r8 + e0, nv, vec8), pow2i((int8_t)(ex & 0xffu)), pow2i((int8_t)(ex >> 8)), m, r);
+        decode4(cm[i], cr[i], (int8_t)(ex[i] & 0xffu), (int8_t)(ex[i] >> 8), m, r);
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = r[e] * r[e];
         store_moment(t.m, e0, nv, m, t.dtype == MTL_BF16);
@@ -276,7 +338,8 @@ __global__ __launch_bounds__(THREADS) void adam8_quantize_kernel(const State8Tab
     const int b = blockIdx.x;
     while (ti + 1 < tab.count && b >= tab.first_block[ti + 1]) ++ti;
     const mtl_adam8_state t = tab.t[ti];
-    const int64_t base = (int64_t)(b - tab.first_block[ti]) * CHUNK;
+    constexpr int ITERS = ITERS_STATE;
+    const int64_t base = (int64_t)(b - tab.first_block[ti]) * chunk_of(ITERS);
     const bool vec8 = (((uintptr_t)t.m8 | (uintptr_t)t.r8) & 3) == 0;
     const float* ms = reinterpret_cast<const float*>(t.m);
     const float* vs = reinterpret_cast<const float*>(t.v);
@@ -285,14 +348,14 @@ __global__ __launch_bounds__(THREADS) void adam8_quantize_kernel(const State8Tab
         const int64_t e0 = base + ((int64_t)i * THREADS + threadIdx.x) * 4;
         const int64_t left = t.n - e0;
         const int nv = left >= 4 ? 4 : (left > 0 ? (int)left : 0);
-        float m[4], r[4];
+        float m[4], v[4], r[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             m[e] = e < nv ? ms[e0 + e] : 0.f;
-            r[e] = e < nv ? __builtin_sqrtf(vs[e0 + e]) : 0.f;
+            v[e] = e < nv ? vs[e0 + e] : 0.f;
         }
         uint32_t nm, nr, nx;
-        encode4(m, r, (uint32_t)e0, t_thr, nm, nr, nx);
+        encode4(m, v, r, (uint32_t)e0, t_thr, nm, nr, nx);
         if (nv == 0) continue;
         store_codes(t.m8 + e0, nm, nv, vec8);
         store_codes(t.r8 + e0, nr, nv, vec8);
@@ -318,7 +381,7 @@ int for_tables(const mtl_adam8_state* states, int count, bool read_back, Launch 
         int64_t blocks = 0;
         for (; i < count && tab.count < MAX_T; ++i) {
             if (states[i].n == 0) continue;
-            const int64_t nb = (states[i].n + CHUNK - 1) / CHUNK;
+            const int64_t nb = (states[i].n + chunk_of(ITERS_STATE) - 1) / chunk_of(ITERS_STATE);
             if (nb > 0x7fffffff) return MTL_ERR_UNSUPPORTED;
             if (blocks + nb > 0x7fffffff) break;                // (this one goes into the next launch)
             tab.t[tab.count] = states[i];
@@ -361,7 +424,7 @@ extern "C" int mtl_adam8_step(const mtl_adam8_tensor* tensors, int count, double
         for (; i < count && tab.count < MAX_T; ++i) {
             const mtl_adam8_tensor& t = tensors[i];
             if (t.n == 0) continue;
-            const int64_t nb = (t.n + CHUNK - 1) / CHUNK;
+            const int64_t nb = (t.n + step_chunk(t.param_dtype) - 1) / step_chunk(t.param_dtype);
             if (nb > 0x7fffffff) return MTL_ERR_UNSUPPORTED;
             if (blocks + nb > 0x7fffffff) break;
             tab.t[tab.count] = t;

@@ -4,8 +4,9 @@
 //   u = Rot^T dy,  dw = sum u n,  a = u w,  dx = r (a - n mean_j(a_j n_j))
 //
 // HBM-bound: the forward reads and writes (Hq + Hkv) D elements per row, the backward reads two and writes one (r is recomputed from x, which it reads anyway: nothing is saved).
-// Layout: a wave owns a row (one token) and walks its heads; a group of LPH lanes owns a head, each lane W consecutive PAIRS, i.e. W elements of each half: the rotation needs no
-// exchange between lanes, the two sums take log2(LPH) DPP steps, and what the heads of a row share (cos, sin, both weights) is loaded once per row or wave and stays in registers.
+// Layout: a wave owns the queries OR the keys of a row (one token; blockIdx.y says which: with both, the two weights and their gradients double the registers and halve the waves in
+// flight) and walks their heads; a group of LPH lanes owns a head, each lane W consecutive PAIRS, i.e. W elements of each half: the rotation needs no exchange between lanes, the two
+// sums take log2(LPH) DPP steps, and what the heads of a row share (cos, sin, the weight) is loaded once per row or wave and stays in registers.
 // Pairs beyond R/2 (elements R .. D-1, split in halves the same way) are rotated by angle 0. All arithmetic fp32, one rounding at the store.
 #include "mtl_common.h"
 
@@ -160,23 +161,39 @@ __device__ __forceinline__ void heads_fwd(const T* __restrict__ x, T* y, int h0,
     }
 }
 
+// one side of a call: the queries (0) or the keys (1)
+struct Side {
+    const void *x, *dy, *w;
+    void* y;
+    int64_t x_bs, x_ts, dy_bs, dy_ts, y_bs, y_ts;
+    int H;
+};
+__device__ __forceinline__ Side side_of(const mtl_qk_norm_rope_args& a, bool keys) {
+    Side s;
+    s.x = keys ? a.k : a.q; s.x_bs = keys ? a.k_bs : a.q_bs; s.x_ts = keys ? a.k_ts : a.q_ts;
+    s.dy = keys ? a.dk_out : a.dq_out; s.dy_bs = keys ? a.dko_bs : a.dqo_bs; s.dy_ts = keys ? a.dko_ts : a.dqo_ts;
+    s.y = keys ? a.k_out : a.q_out; s.y_bs = keys ? a.ko_bs : a.qo_bs; s.y_ts = keys ? a.ko_ts : a.qo_ts;
+    s.w = keys ? a.wk : a.wq;
+    s.H = (int)(keys ? a.Hkv : a.Hq);
+    return s;
+}
+
 template <typename T, int W, int LPH, int C>
 __global__ __launch_bounds__(WAVES * 64) void qk_norm_rope_fwd_kernel(const mtl_qk_norm_rope_args a, int hq_per, int hk_per) {
     const Lane<W, LPH, C> L((int)a.D, (int)a.R);
     const int64_t rows = a.B * a.T;
     const float inv_d = 1.0f / (float)a.D;
-    float ql[C][W], qh[C][W], kl[C][W], kh[C][W];
-    load_weights(a.wq, a.w_dtype, L, ql, qh);
-    load_weights(a.wk, a.w_dtype, L, kl, kh);
-    const int part = blockIdx.y;                       // few rows: a row's heads are spread over gridDim.y waves
-    const int q0 = part * hq_per, q1 = q0 + hq_per < a.Hq ? q0 + hq_per : (int)a.Hq;
-    const int k0 = part * hk_per, k1 = k0 + hk_per < a.Hkv ? k0 + hk_per : (int)a.Hkv;
+    const Side s = side_of(a, blockIdx.y == 1);
+    const int per = blockIdx.y ? hk_per : hq_per;                 // few rows: a row's heads are spread over gridDim.z waves
+    const int h0 = blockIdx.z * per, h1 = h0 + per < s.H ? h0 + per : s.H;
+    if (h0 >= h1) return;
+    float wl[C][W], wh[C][W];
+    load_weights(s.w, a.w_dtype, L, wl, wh);
     for (int64_t row = (int64_t)blockIdx.x * WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); row < rows; row += (int64_t)gridDim.x * WAVES) {
         const int64_t b = row / a.T, t = row - b * a.T;
         float cs[C][W], sn[C][W];
         load_turn(a, b, t, L, cs, sn);
-        heads_fwd<T, W, LPH, C>((const T*)a.q + b * a.q_bs + t * a.q_ts, (T*)a.q_out + b * a.qo_bs + t * a.qo_ts, q0, q1, (int)a.D, a.eps, inv_d, L, ql, qh, cs, sn);
-        heads_fwd<T, W, LPH, C>((const T*)a.k + b * a.k_bs + t * a.k_ts, (T*)a.k_out + b * a.ko_bs + t * a.ko_ts, k0, k1, (int)a.D, a.eps, inv_d, L, kl, kh, cs, sn);
+        heads_fwd<T, W, LPH, C>((const T*)s.x + b * s.x_bs + t * s.x_ts, (T*)s.y + b * s.y_bs + t * s.y_ts, h0, h1, (int)a.D, a.eps, inv_d, L, wl, wh, cs, sn);
     }
 }
 
@@ -233,51 +250,44 @@ __device__ __forceinline__ void heads_bwd(const T* __restrict__ x, const T* dy, 
     }
 }
 
-// part [gridDim.x][2][D] (DW): every workgroup's weight gradients, summed over its waves and lane groups in a fixed order
+// part [2][gridDim.x][D] (DW): every workgroup's weight gradient, summed over its waves and lane groups in a fixed order
 template <typename T, int W, int LPH, int C, bool DW>
 __global__ __launch_bounds__(WAVES * 64) void qk_norm_rope_bwd_kernel(const mtl_qk_norm_rope_args a, float* __restrict__ part) {
     const Lane<W, LPH, C> L((int)a.D, (int)a.R);
     const int64_t rows = a.B * a.T;
     const float inv_d = 1.0f / (float)a.D;
-    float ql[C][W], qh[C][W], kl[C][W], kh[C][W], gql[C][W], gqh[C][W], gkl[C][W], gkh[C][W];
-    load_weights(a.wq, a.w_dtype, L, ql, qh);
-    load_weights(a.wk, a.w_dtype, L, kl, kh);
+    const Side s = side_of(a, blockIdx.y == 1);
+    float wl[C][W], wh[C][W], gl[C][W], gh[C][W];
+    load_weights(s.w, a.w_dtype, L, wl, wh);
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
-        for (int j = 0; j < W; ++j) gql[c][j] = gqh[c][j] = gkl[c][j] = gkh[c][j] = 0.f;
+        for (int j = 0; j < W; ++j) gl[c][j] = gh[c][j] = 0.f;
     for (int64_t row = (int64_t)blockIdx.x * WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); row < rows; row += (int64_t)gridDim.x * WAVES) {
         const int64_t b = row / a.T, t = row - b * a.T;
         float cs[C][W], sn[C][W];
         load_turn(a, b, t, L, cs, sn);
-        heads_bwd<T, W, LPH, C, DW>((const T*)a.q + b * a.q_bs + t * a.q_ts, (const T*)a.dq_out + b * a.dqo_bs + t * a.dqo_ts, (T*)a.q_out + b * a.qo_bs + t * a.qo_ts, (int)a.Hq, (int)a.D, a.eps, inv_d,
-                                    L, ql, qh, cs, sn, gql, gqh);
-        heads_bwd<T, W, LPH, C, DW>((const T*)a.k + b * a.k_bs + t * a.k_ts, (const T*)a.dk_out + b * a.dko_bs + t * a.dko_ts, (T*)a.k_out + b * a.ko_bs + t * a.ko_ts, (int)a.Hkv, (int)a.D, a.eps, inv_d,
-                                    L, kl, kh, cs, sn, gkl, gkh);
+        heads_bwd<T, W, LPH, C, DW>((const T*)s.x + b * s.x_bs + t * s.x_ts, (const T*)s.dy + b * s.dy_bs + t * s.dy_ts, (T*)s.y + b * s.y_bs + t * s.y_ts, s.H, (int)a.D, a.eps, inv_d, L, wl, wh, cs, sn,
+                                    gl, gh);
     }
     if (!DW) return;
-    // lane groups of a wave, then the waves: [WAVES * 64 / LPH][D] in LDS, one weight at a time
     constexpr int G = 64 / LPH;
-    __shared__ float sums[WAVES * G * 2 * LPH * C * W];
+    __shared__ float sums[WAVES * G * 2 * LPH * C * W];           // [waves * lane groups][D]
     const int slot = (threadIdx.x >> 6) * G + (threadIdx.x & 63) / LPH, D = (int)a.D;
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-        __syncthreads();
+    for (int c = 0; c < C; ++c)
+        if (L.on[c])
 #pragma unroll
-        for (int c = 0; c < C; ++c)
-            if (L.on[c])
-#pragma unroll
-                for (int j = 0; j < W; ++j) {
-                    sums[slot * D + L.lo[c] + j] = which ? gkl[c][j] : gql[c][j];
-                    sums[slot * D + L.hi[c] + j] = which ? gkh[c][j] : gqh[c][j];
-                }
-        __syncthreads();
-        for (int i = threadIdx.x; i < D; i += WAVES * 64) {
-            float s = 0.f;
+            for (int j = 0; j < W; ++j) {
+                sums[slot * D + L.lo[c] + j] = gl[c][j];
+                sums[slot * D + L.hi[c] + j] = gh[c][j];
+            }
+    __syncthreads();
+    for (int i = threadIdx.x; i < D; i += WAVES * 64) {
+        float x = 0.f;
 #pragma unroll 8
-            for (int k = 0; k < WAVES * G; ++k) s += sums[k * D + i];
-            part[((int64_t)blockIdx.x * 2 + which) * D + i] = s;
-        }
+        for (int k = 0; k < WAVES * G; ++k) x += sums[k * D + i];
+        part[((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * D + i] = x;
     }
 }
 
@@ -290,7 +300,7 @@ __global__ __launch_bounds__(1024) void qk_norm_rope_dw_kernel(const float* __re
     if (i < D) {
         const int k0 = n * wave / 16, k1 = n * (wave + 1) / 16;
 #pragma unroll 8
-        for (int k = k0; k < k1; ++k) s += part[((int64_t)k * 2 + which) * D + i];
+        for (int k = k0; k < k1; ++k) s += part[((int64_t)which * n + k) * D + i];
     }
     sums[wave][lane] = s;
     __syncthreads();
@@ -303,7 +313,7 @@ __global__ __launch_bounds__(1024) void qk_norm_rope_dw_kernel(const float* __re
 }
 
 inline unsigned fwd_blocks(int64_t rows) { const int64_t b = (rows + WAVES - 1) / WAVES; return (unsigned)(b < 2048 ? b : 2048); }
-inline unsigned bwd_blocks(int64_t rows) { const int64_t b = (rows + WAVES - 1) / WAVES; return (unsigned)(b < 1024 ? b : 1024); }
+inline unsigned bwd_blocks(int64_t rows) { const int64_t b = (rows + WAVES - 1) / WAVES; return (unsigned)(b < 768 ? b : 768); }
 
 template <typename T, int W, int LPH, int C>
 int launch(const mtl_qk_norm_rope_args& a, bool bwd, hipStream_t st) {
@@ -316,18 +326,18 @@ int launch(const mtl_qk_norm_rope_args& a, bool bwd, hipStream_t st) {
         while (parts < steps && rows * parts < 4096) parts *= 2;
         if (parts > steps) parts = (int)steps;
         const int hq = (int)(((a.Hq + parts - 1) / parts + G - 1) / G * G), hk = (int)(((a.Hkv + parts - 1) / parts + G - 1) / G * G);
-        hipLaunchKernelGGL((qk_norm_rope_fwd_kernel<T, W, LPH, C>), dim3(fwd_blocks(rows), parts), dim3(WAVES * 64), 0, st, a, hq, hk);
+        hipLaunchKernelGGL((qk_norm_rope_fwd_kernel<T, W, LPH, C>), dim3(fwd_blocks(rows), 2, parts), dim3(WAVES * 64), 0, st, a, hq, hk);
         MTL_CHECK_LAUNCH();
         return MTL_OK;
     }
     const unsigned blocks = bwd_blocks(rows);
     float* part = reinterpret_cast<float*>(a.workspace);
     if (!a.dwq) {
-        hipLaunchKernelGGL((qk_norm_rope_bwd_kernel<T, W, LPH, C, false>), dim3(blocks), dim3(WAVES * 64), 0, st, a, part);
+        hipLaunchKernelGGL((qk_norm_rope_bwd_kernel<T, W, LPH, C, false>), dim3(blocks, 2), dim3(WAVES * 64), 0, st, a, part);
         MTL_CHECK_LAUNCH();
         return MTL_OK;
     }
-    hipLaunchKernelGGL((qk_norm_rope_bwd_kernel<T, W, LPH, C, true>), dim3(blocks), dim3(WAVES * 64), 0, st, a, part);
+    hipLaunchKernelGGL((qk_norm_rope_bwd_kernel<T, W, LPH, C, true>), dim3(blocks, 2), dim3(WAVES * 64), 0, st, a, part);
     MTL_CHECK_LAUNCH();
     hipLaunchKernelGGL(qk_norm_rope_dw_kernel, dim3((unsigned)((a.D + 63) / 64), 2), dim3(1024), 0, st, part, (int)blocks, (int)a.D, a.dwq, a.dwk);
     MTL_CHECK_LAUNCH();

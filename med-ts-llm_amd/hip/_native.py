@@ -231,8 +231,9 @@ _HERE_AND_NOW = contextlib.nullcontext()
 
 def on_device(t):
     """context in which the current device is the tensor's own (launches and `stream()` follow the current device)"""
-    return _HERE_AND_NOW if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return _HERE_AND_NOW if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def stream():
-    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    # (the raw handle: building a torch.cuda.Stream object for it costs more than a launch)
+    return C.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))

@@ -405,39 +405,53 @@ def assemble_bwd(dh0, n_tok, drop=(0.0, 0)):
 
 
 # ---- token table: lookup with scaling, gradient by sorted tokens
+# (The checks of these entry points are one condition on the way through; what is wrong is worked out only where it fails: the calls are short enough for the host's time to count.)
+_TYPES = {F32: N.MTL_F32, BF16: N.MTL_BF16}
+_ID_TYPES = {torch.int32: 0, torch.int64: 1}
+
+
 def _req_gpu(*tensors):
     """all on one GPU (the last check of an entry point: what is wrong with shapes and types is said on any machine)"""
-    _req(all(t.is_cuda for t in tensors), "the HIP path needs tensors on the GPU (no CPU fallback)")
-    _req(all(t.device == tensors[0].device for t in tensors), "tensors on different devices")
+    dev = tensors[0].get_device()
+    for t in tensors:
+        if t.get_device() != dev or dev < 0:
+            raise ValueError("the HIP path needs all tensors on one GPU (no CPU fallback)")
 
 
 def _rows(x, d):
     """[..., d] as rows of unit inner stride (a copy where strides do not allow it, e.g. the expanded gradient of a sum)"""
     x = x.reshape(-1, d)
-    return x if (d == 1 or x.stride(1) == 1) and (x.shape[0] <= 1 or x.stride(0) >= d) else x.contiguous()
+    n, (rs, cs) = x.shape[0], x.stride()
+    return x if (d == 1 or cs == 1) and (n <= 1 or rs >= d) else x.contiguous()
 
 
 def _ids(ids):
-    _req(ids.dtype in (torch.int32, torch.int64), f"embedding: ids must be int32 or int64, got {ids.dtype}")
-    return ids.reshape(-1).contiguous()
+    if ids.dtype not in _ID_TYPES:
+        raise ValueError(f"embedding: ids must be int32 or int64, got {ids.dtype}")
+    return ids if ids.is_contiguous() else ids.contiguous()
 
 
-def _ld(x):
-    return x.stride(0) if x.shape[0] > 1 else max(x.stride(0), x.shape[1])
+def _table_ld(t, what):
+    """row stride of a [V, d] table whose rows have unit inner stride and do not overlap"""
+    (V, d), (rs, cs) = t.shape, t.stride()
+    if V < 1 or d < 1 or (d > 1 and cs != 1) or (V > 1 and rs < d):
+        raise ValueError(f"embedding: {what} needs rows of unit inner stride that do not overlap")
+    return rs if V > 1 else max(rs, d)
 
 
 def embedding_fwd(ids, table, scale=1.0, out_dtype=None):
     """scale * table[ids]: ids int32 / int64 of any shape, table [V, d] f32 / bf16 (rows of unit inner stride), out_dtype f32 / bf16 (default: the table's).
     An id outside [0, V) gives a row of zeros."""
     out_dtype = table.dtype if out_dtype is None else out_dtype
-    _req(table.dim() == 2 and table.dtype in (F32, BF16) and out_dtype in (F32, BF16), "embedding: table [V, d] of f32 or bf16, output f32 or bf16")
+    if table.dim() != 2 or table.dtype not in _TYPES or out_dtype not in _TYPES:
+        raise ValueError("embedding: table [V, d] of f32 or bf16, output f32 or bf16")
+    ld = _table_ld(table, "the table")
     V, d = table.shape
-    _req(V >= 1 and d >= 1 and (d == 1 or table.stride(1) == 1) and (V == 1 or table.stride(0) >= d), "embedding: the table needs rows of unit inner stride that do not overlap")
     flat = _ids(ids)
     _req_gpu(table, flat)
     with N.on_device(table):
-        out = torch.empty((*ids.shape, d), dtype=out_dtype, device=table.device)
-        check(lib().mtl_embedding_fwd(ptr(flat), flat.element_size() // 8, flat.numel(), ptr(table), _dt(table), V, d, _ld(table), float(scale), ptr(out), _dt(out), d, stream()),
+        out = table.new_empty((*ids.shape, d), dtype=out_dtype)
+        check(lib().mtl_embedding_fwd(flat.data_ptr(), _ID_TYPES[flat.dtype], flat.numel(), table.data_ptr(), _TYPES[table.dtype], V, d, ld, scale, out.data_ptr(), _TYPES[out_dtype], d, stream()),
               "mtl_embedding_fwd")
     return out
 
@@ -445,55 +459,73 @@ def embedding_fwd(ids, table, scale=1.0, out_dtype=None):
 def embedding_bwd(dout, ids, V, scale=1.0, padding_idx=None, out=None, accumulate=False, out_dtype=F32):
     """gradient of embedding_fwd's table: [V, d], row v = scale * sum of the dout rows whose id is v (padding_idx and ids outside [0, V): none). Sums in fp32 in the order
     of the tokens: the same bits every time. out: write there (f32 / bf16 [V, d]); accumulate: add to it, touching only the rows that occur."""
+    if dout.dim() < 1 or dout.dtype not in _TYPES or dout.shape[:-1] != ids.shape or dout.shape[-1] < 1:
+        raise ValueError("embedding_bwd: dout [*ids.shape, d] of f32 or bf16")
+    if V < 1 or (padding_idx is not None and not 0 <= padding_idx < V):
+        raise ValueError("embedding_bwd: padding_idx outside [0, V)")
     d = dout.shape[-1]
-    _req(dout.dim() >= 1 and d >= 1 and dout.dtype in (F32, BF16) and tuple(dout.shape[:-1]) == tuple(ids.shape), "embedding_bwd: dout [*ids.shape, d] of f32 or bf16")
-    _req(V >= 1 and (padding_idx is None or 0 <= padding_idx < V), "embedding_bwd: padding_idx outside [0, V)")
-    _req(out is not None or not accumulate, "embedding_bwd: accumulate needs out")
     if out is None:
-        _req(out_dtype in (F32, BF16), "embedding_bwd: gradient of f32 or bf16")
+        if accumulate or out_dtype not in _TYPES:
+            raise ValueError("embedding_bwd: accumulate needs out" if accumulate else "embedding_bwd: gradient of f32 or bf16")
+        ld = d
     else:
-        _req(tuple(out.shape) == (V, d) and out.dtype in (F32, BF16) and (d == 1 or out.stride(1) == 1) and (V == 1 or out.stride(0) >= d),
-             "embedding_bwd: out must be f32 or bf16 [V, d] with rows of unit inner stride that do not overlap")
+        if tuple(out.shape) != (V, d) or out.dtype not in _TYPES:
+            raise ValueError("embedding_bwd: out must be f32 or bf16 [V, d]")
+        ld, out_dtype = _table_ld(out, "out"), out.dtype
     flat, rows = _ids(ids), _rows(dout, d)
     _req_gpu(rows, flat, *(() if out is None else (out,)))
+    n = rows.shape[0]
     with N.on_device(rows):
         if out is None:
-            out = torch.empty((V, d), dtype=out_dtype, device=rows.device)
-        nbytes = lib().mtl_embedding_bwd_workspace_bytes(flat.numel(), V, d)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=rows.device)
-        check(lib().mtl_embedding_bwd(ptr(flat), flat.element_size() // 8, flat.numel(), ptr(rows), _dt(rows), _ld(rows) if rows.shape[0] else d, V, d,
-                                      -1 if padding_idx is None else int(padding_idx), float(scale), ptr(out), _dt(out), _ld(out), 1 if accumulate else 0, ptr(ws), nbytes, stream()),
-              "mtl_embedding_bwd")
+            out = rows.new_empty((V, d), dtype=out_dtype)
+        nbytes = lib().mtl_embedding_bwd_workspace_bytes(n, V, d)
+        ws = rows.new_empty(nbytes, dtype=torch.uint8)
+        check(lib().mtl_embedding_bwd(flat.data_ptr(), _ID_TYPES[flat.dtype], n, rows.data_ptr(), _TYPES[rows.dtype], rows.stride(0) if n > 1 else d, V, d, -1 if padding_idx is None else padding_idx,
+                                      scale, out.data_ptr(), _TYPES[out_dtype], ld, 1 if accumulate else 0, ws.data_ptr(), nbytes, stream()), "mtl_embedding_bwd")
     return out
 
 
 # ---- query / key norm per head + rotary embedding
-def _qk_args(q, k, wq, wk, cos, sin, Hq, Hkv, D, eps, positions, pos0):
+def _qk_complain(q, k, wq, wk, cos, sin, Hq, Hkv, D, positions, pos0):
     _req(q.dim() == 3 and k.dim() == 3 and q.shape[:2] == k.shape[:2], "qk_norm_rope: q [B, T, Hq * D] and k [B, T, Hkv * D]")
     _req(Hq >= 1 and Hkv >= 1 and q.shape[2] == Hq * D and k.shape[2] == Hkv * D, "qk_norm_rope: head counts and widths")
     _req(D % 2 == 0 and 2 <= D <= 512, "qk_norm_rope: an even head width of at most 512")
-    _req(q.dtype == k.dtype and q.dtype in (F32, BF16) and q.stride(2) == 1 and k.stride(2) == 1, "qk_norm_rope: q and k both f32 or both bf16, unit inner stride")
-    _req(tuple(wq.shape) == (D,) == tuple(wk.shape) and wq.dtype == wk.dtype and wq.dtype in (F32, BF16), "qk_norm_rope: weights [D], both f32 or both bf16")
+    _req(q.dtype == k.dtype and q.dtype in _TYPES and q.stride(2) == 1 and k.stride(2) == 1, "qk_norm_rope: q and k both f32 or both bf16, unit inner stride")
+    _req(tuple(wq.shape) == (D,) == tuple(wk.shape) and wq.dtype == wk.dtype and wq.dtype in _TYPES, "qk_norm_rope: weights [D], both f32 or both bf16")
     _req(cos.dim() == 2 and cos.shape == sin.shape and cos.dtype == F32 == sin.dtype and cos.is_contiguous() and sin.is_contiguous(), "qk_norm_rope: cos / sin f32 [positions, R], contiguous")
-    P, R = cos.shape
-    _req(2 <= R <= D and R % 2 == 0 and P >= 1, "qk_norm_rope: an even rotated width of at most D")
-    B, T = q.shape[:2]
+    _req(2 <= cos.shape[1] <= D and cos.shape[1] % 2 == 0 and cos.shape[0] >= 1, "qk_norm_rope: an even rotated width of at most D")
     if positions is None:
-        _req(0 <= pos0 and pos0 + T <= P, f"qk_norm_rope: rows {pos0} .. {pos0 + T - 1} of a table of {P} positions")
-    else:
-        _req(positions.dtype in (torch.int32, torch.int64) and tuple(positions.shape) in ((T,), (B, T)) and pos0 == 0, "qk_norm_rope: positions int32 / int64 [B, T] or [T], without pos0")
-        if T > 1 and positions.stride(-1) != 1:
-            positions = positions.contiguous()
-    wq, wk = wq.contiguous(), wk.contiguous()
-    a = N.QkNormRopeArgs()
-    a.q, a.q_bs, a.q_ts = q.data_ptr(), q.stride(0), q.stride(1)
-    a.k, a.k_bs, a.k_ts = k.data_ptr(), k.stride(0), k.stride(1)
-    a.wq, a.wk, a.w_dtype = wq.data_ptr(), wk.data_ptr(), _dt(wq)
-    a.cos_t, a.sin_t, a.n_pos = cos.data_ptr(), sin.data_ptr(), P
-    if positions is not None:
-        a.positions, a.pos_i64, a.pos_bs = positions.data_ptr(), positions.element_size() // 8, positions.stride(0) if positions.dim() == 2 else 0
-    a.pos0, a.B, a.T, a.Hq, a.Hkv, a.D, a.R, a.eps, a.dtype = int(pos0), B, T, Hq, Hkv, D, R, float(eps), _dt(q)
-    return a, (q, k, wq, wk, cos, sin) + (() if positions is None else (positions,))
+        _req(0 <= pos0 and pos0 + q.shape[1] <= cos.shape[0], f"qk_norm_rope: rows {pos0} .. {pos0 + q.shape[1] - 1} of a table of {cos.shape[0]} positions")
+    _req(positions is None or pos0 == 0, "qk_norm_rope: positions without pos0")
+    raise ValueError("qk_norm_rope: positions int32 / int64 [B, T] or [T]")
+
+
+def _qk_args(q, k, wq, wk, cos, sin, Hq, Hkv, D, eps, positions, pos0):
+    """the C structure of a checked call (without outputs and gradients), and the tensors its pointers stand on"""
+    fine = q.dim() == 3 == k.dim() and cos.dim() == 2 and wq.dim() == 1 and wk.dim() == 1
+    if fine:
+        (B, T, nq), (Bk, Tk, nk), (P, R), (q_bs, q_ts, q_cs), (k_bs, k_ts, k_cs) = q.shape, k.shape, cos.shape, q.stride(), k.stride()
+        fine = (B == Bk and T == Tk and Hq >= 1 and Hkv >= 1 and nq == Hq * D and nk == Hkv * D and D % 2 == 0 and 2 <= D <= 512 and q.dtype is k.dtype and q.dtype in _TYPES and q_cs == 1 == k_cs
+                and wq.shape[0] == D == wk.shape[0] and wq.dtype is wk.dtype and wq.dtype in _TYPES and cos.shape == sin.shape and cos.dtype is F32 is sin.dtype and cos.is_contiguous()
+                and sin.is_contiguous() and 2 <= R <= D and R % 2 == 0 and P >= 1)
+    pp, p64, pbs = None, 0, 0
+    if fine and positions is None:
+        fine = 0 <= pos0 and pos0 + T <= P
+    elif fine:
+        p64 = _ID_TYPES.get(positions.dtype)
+        fine = p64 is not None and positions.shape in ((B, T), (T,)) and pos0 == 0
+        if fine:
+            if not positions.is_contiguous():
+                positions = positions.contiguous()
+            pp, pbs = positions.data_ptr(), T if positions.dim() == 2 else 0
+    if not fine:
+        _qk_complain(q, k, wq, wk, cos, sin, Hq, Hkv, D, positions, pos0)
+    if not (wq.is_contiguous() and wk.is_contiguous()):
+        wq, wk = wq.contiguous(), wk.contiguous()
+    dt = _TYPES[q.dtype]
+    a = N.QkNormRopeArgs(q.data_ptr(), q_bs, q_ts, k.data_ptr(), k_bs, k_ts, None, 0, 0, None, 0, 0, wq.data_ptr(), wk.data_ptr(), _TYPES[wq.dtype], cos.data_ptr(), sin.data_ptr(), P, pp, p64, pbs, pos0,
+                         B, T, Hq, Hkv, D, R, eps, dt)
+    return a, (q, k, wq, wk, cos, sin) if positions is None else (q, k, wq, wk, cos, sin, positions)
 
 
 def _row_views(t, like, name):
@@ -509,9 +541,8 @@ def _same_view(a, b):
     return a.data_ptr() == b.data_ptr() and a.stride() == b.stride()
 
 
-def _qk_outputs(q, k, out):
-    if out is None:
-        return torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
+def _check_qk_outputs(q, k, out):
+    """given outputs: rows that do not overlap, and either memory of their own or their input's, exactly"""
     qo, ko = out
     _row_views(qo, q, "the query output")
     _row_views(ko, k, "the key output")
@@ -523,51 +554,63 @@ def _qk_outputs(q, k, out):
             ts, off = a.stride(1), (b.data_ptr() - a.data_ptr()) // a.element_size()
             _req(a.stride() == b.stride() and ts > 0 and off % ts >= a.shape[2] and off % ts <= ts - b.shape[2] and (a.shape[0] <= 1 or a.stride(0) % ts == 0),
                  "qk_norm_rope: queries and keys in one buffer have to be separate column ranges of it")
-    return qo, ko
+
+
+def _new(t):
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def qk_norm_rope_fwd(q, k, wq, wk, cos, sin, Hq, Hkv, D, eps=1e-6, positions=None, pos0=0, out=None):
     """rotate(w * x / rms(x)) for every head of q [B, T, Hq * D] and k [B, T, Hkv * D] (f32 or bf16; strided views, e.g. of a fused qkv buffer). cos / sin f32 [positions, R] as
     rope_inplace takes them (R <= D: the first R elements of a head are rotated). positions [B, T] or [T]: the rows' positions (a row whose position is not in the table comes out
     as NaN), default pos0 + 0 .. T - 1. out = (q', k'): write there; the inputs themselves for in place."""
+    return _qk_fwd(q, k, wq, wk, cos, sin, Hq, Hkv, D, eps, positions, pos0, out)[:2]
+
+
+def _qk_fwd(q, k, wq, wk, cos, sin, Hq, Hkv, D, eps, positions, pos0, out=None):
+    """(q', k', the call's C structure, the tensors it points to)"""
     a, keep = _qk_args(q, k, wq, wk, cos, sin, Hq, Hkv, D, eps, positions, pos0)
-    qo, ko = _qk_outputs(q, k, out) if out is not None else (None, None)
+    if out is not None:
+        _check_qk_outputs(q, k, out)
     _req_gpu(*keep, *(out or ()))
     with N.on_device(q):
-        if out is None:
-            qo, ko = _qk_outputs(q, k, None)
-        a.q_out, a.qo_bs, a.qo_ts = qo.data_ptr(), qo.stride(0), qo.stride(1)
-        a.k_out, a.ko_bs, a.ko_ts = ko.data_ptr(), ko.stride(0), ko.stride(1)
+        qo, ko = out if out is not None else (_new(q), _new(k))
+        a.q_out, a.k_out = qo.data_ptr(), ko.data_ptr()
+        (a.qo_bs, a.qo_ts, _), (a.ko_bs, a.ko_ts, _) = qo.stride(), ko.stride()
         check(lib().mtl_qk_norm_rope_fwd(C.byref(a), stream()), "mtl_qk_norm_rope_fwd")
-    return qo, ko
+    return qo, ko, a, keep
 
 
 def qk_norm_rope_bwd(dq_out, dk_out, q, k, wq, wk, cos, sin, Hq, Hkv, D, eps=1e-6, positions=None, pos0=0, want_dw=True, out=None):
     """(dq, dk, dwq, dwk) from the gradients of qk_norm_rope_fwd's outputs and its inputs (the norms are recomputed). dq / dk in the inputs' type (out = (dq, dk): written there,
     e.g. column ranges of one d(qkv) buffer, or over dq_out / dk_out themselves), dwq / dwk f32 [D] or None (want_dw False)."""
     a, keep = _qk_args(q, k, wq, wk, cos, sin, Hq, Hkv, D, eps, positions, pos0)
-    _req(dq_out.shape == q.shape and dk_out.shape == k.shape and dq_out.dtype == q.dtype == dk_out.dtype, "qk_norm_rope_bwd: gradients of the outputs' shapes and type")
-    dq_out, dk_out = (t if t.stride(2) == 1 else t.contiguous() for t in (dq_out, dk_out))
+    return _qk_bwd(dq_out, dk_out, a, keep, want_dw, out)
+
+
+def _qk_bwd(dq_out, dk_out, a, keep, want_dw, out=None):
+    q, k, wq, wk = keep[:4]
+    if dq_out.shape != q.shape or dk_out.shape != k.shape or not dq_out.dtype is q.dtype is dk_out.dtype:
+        raise ValueError("qk_norm_rope_bwd: gradients of the outputs' shapes and type")
+    if dq_out.stride(2) != 1 or dk_out.stride(2) != 1:
+        dq_out, dk_out = dq_out.contiguous(), dk_out.contiguous()
     if out is not None:
         ins = {t.untyped_storage().data_ptr() for t in (q, k)}
         _req(all(o.untyped_storage().data_ptr() not in ins for o in out), "qk_norm_rope_bwd: out must not share memory with q or k")
-        _qk_outputs(dq_out, dk_out, out)
+        _check_qk_outputs(dq_out, dk_out, out)
     _req_gpu(*keep, dq_out, dk_out, *(out or ()))
     with N.on_device(q):
-        dq, dk = _qk_outputs(q, k, None) if out is None else out
-        a.q_out, a.qo_bs, a.qo_ts = dq.data_ptr(), dq.stride(0), dq.stride(1)
-        a.k_out, a.ko_bs, a.ko_ts = dk.data_ptr(), dk.stride(0), dk.stride(1)
-        a.dq_out, a.dqo_bs, a.dqo_ts = dq_out.data_ptr(), dq_out.stride(0), dq_out.stride(1)
-        a.dk_out, a.dko_bs, a.dko_ts = dk_out.data_ptr(), dk_out.stride(0), dk_out.stride(1)
-        dw = ws = None
+        dq, dk = out if out is not None else (_new(q), _new(k))
+        a.q_out, a.k_out, a.dq_out, a.dk_out = dq.data_ptr(), dk.data_ptr(), dq_out.data_ptr(), dk_out.data_ptr()
+        (a.qo_bs, a.qo_ts, _), (a.ko_bs, a.ko_ts, _), (a.dqo_bs, a.dqo_ts, _), (a.dko_bs, a.dko_ts, _) = dq.stride(), dk.stride(), dq_out.stride(), dk_out.stride()
+        dwq = dwk = None
         if want_dw:
-            dw = torch.empty((2, D), dtype=F32, device=q.device)
-            a.dwq, a.dwk = dw[0].data_ptr(), dw[1].data_ptr()
-            nbytes = lib().mtl_qk_norm_rope_bwd_workspace_bytes(a.B, a.T, D)
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-            a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
+            nbytes = lib().mtl_qk_norm_rope_bwd_workspace_bytes(a.B, a.T, a.D)
+            ws = q.new_empty(nbytes, dtype=torch.uint8)
+            dwq, dwk = torch.empty_like(wq, dtype=F32), torch.empty_like(wk, dtype=F32)
+            a.dwq, a.dwk, a.workspace, a.workspace_bytes = dwq.data_ptr(), dwk.data_ptr(), ws.data_ptr(), nbytes
         check(lib().mtl_qk_norm_rope_bwd(C.byref(a), stream()), "mtl_qk_norm_rope_bwd")
-    return dq, dk, (dw[0] if want_dw else None), (dw[1] if want_dw else None)
+    return dq, dk, dwq, dwk
 
 
 # =============================================================================================== autograd ops
@@ -941,7 +984,7 @@ class EmbeddingFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, table, scale=1.0, padding_idx=None, out_dtype=None):
         _req(padding_idx is None or 0 <= padding_idx < table.shape[0], "EmbeddingFn: padding_idx outside [0, V)")
-        out = embedding_fwd(ids, table.detach(), scale, out_dtype)
+        out = embedding_fwd(ids, table, scale, out_dtype)
         ctx.save_for_backward(ids)
         ctx.meta = (table.shape[0], float(scale), padding_idx, table.dtype)
         return out
@@ -960,19 +1003,28 @@ class QkNormRopeFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, wq, wk, cos, sin, Hq, Hkv, D, eps=1e-6, positions=None, pos0=0):
-        qo, ko = qk_norm_rope_fwd(q.detach(), k.detach(), wq.detach(), wk.detach(), cos, sin, Hq, Hkv, D, eps, positions, pos0)
-        ctx.save_for_backward(q, k, wq, wk, cos, sin, positions)
+        qo, ko, ctx.args, keep = _qk_fwd(q, k, wq, wk, cos, sin, Hq, Hkv, D, eps, positions, pos0)
+        ctx.save_for_backward(*keep)
         ctx.meta = (Hq, Hkv, D, eps, pos0)
         return qo, ko
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dqo, dko):
-        q, k, wq, wk, cos, sin, positions = ctx.saved_tensors
-        Hq, Hkv, D, eps, pos0 = ctx.meta
-        need = ctx.needs_input_grad
-        dq, dk, dwq, dwk = qk_norm_rope_bwd(dqo, dko, q, k, wq, wk, cos, sin, Hq, Hkv, D, eps, positions, pos0, want_dw=need[2] or need[3])
-        return (dq if need[0] else None, dk if need[1] else None, dwq.to(wq.dtype) if need[2] else None, dwk.to(wk.dtype) if need[3] else None) + (None,) * 8
+        keep, need, a = ctx.saved_tensors, ctx.needs_input_grad, ctx.args
+        q, k, wq, wk, cos, sin = keep[:6]
+        positions = keep[6] if len(keep) > 6 else None
+        # the forward's checked structure serves again as long as the saved tensors are where they were (a saved-tensor hook may have moved them)
+        if (a.q, a.k, a.wq, a.wk, a.cos_t, a.sin_t, a.positions) == (q.data_ptr(), k.data_ptr(), wq.data_ptr(), wk.data_ptr(), cos.data_ptr(), sin.data_ptr(), None if positions is None else positions.data_ptr()) \
+                and (a.q_bs, a.q_ts) == q.stride()[:2] and (a.k_bs, a.k_ts) == k.stride()[:2]:
+            a = N.QkNormRopeArgs.from_buffer_copy(a)
+        else:
+            Hq, Hkv, D, eps, pos0 = ctx.meta
+            a, keep = _qk_args(q, k, wq, wk, cos, sin, Hq, Hkv, D, eps, positions, pos0)
+        dq, dk, dwq, dwk = _qk_bwd(dqo, dko, a, keep, need[2] or need[3])
+        if dwq is not None and wq.dtype is not F32:
+            dwq, dwk = dwq.to(wq.dtype), dwk.to(wk.dtype)
+        return dq if need[0] else None, dk if need[1] else None, dwq if need[2] else None, dwk if need[3] else None, None, None, None, None, None, None, None, None
 
 
 def dropout_f32(x, p, seed, out=None):

@@ -32,18 +32,27 @@ Adam8State.__doc__ = """moments in 8 bits: uint8 codes of the first moment and o
 consecutive elements, uint8 [ceil(n / 64), 2]"""
 
 
-def _check_state8(st, what):
-    n = st.exp_avg.numel()
-    ok = all(t.dtype == torch.uint8 and t.is_contiguous() for t in st) and st.exp_avg.shape == st.exp_avg_sq.shape and tuple(st.exponents.shape) == ((n + N.ADAM8_BLOCK - 1) // N.ADAM8_BLOCK, 2)
-    if not ok:
-        raise ValueError(f"{what}: an 8-bit state is contiguous uint8: two code tensors of one shape and exponents [ceil(n / 64), 2]")
+_PARAM_TYPES = {torch.float32: N.MTL_F32, torch.bfloat16: N.MTL_BF16}
+
+
+def _state8_row(st, what):
+    """(codes, codes, exponents, n) as pointers and the element count of a checked state"""
+    m8, r8, ex = st
+    n = m8.numel()
+    u8 = torch.uint8
+    if not (m8.dtype is u8 and r8.dtype is u8 and ex.dtype is u8 and r8.numel() == n and ex.numel() == (n + N.ADAM8_BLOCK - 1) // N.ADAM8_BLOCK * 2
+            and m8.is_contiguous() and r8.is_contiguous() and ex.is_contiguous()):
+        raise ValueError(f"{what}: an 8-bit state is contiguous uint8: two code tensors of one size and two exponents for every 64 of their elements")
+    return m8.data_ptr(), r8.data_ptr(), ex.data_ptr(), n
 
 
 def _one_gpu(tensors, what):
-    if not all(t.is_cuda for t in tensors):
+    dev = tensors[0].get_device()
+    if dev < 0:
         raise N.MtlError(f"{what} needs tensors on the GPU (no CPU fallback)")
-    if any(t.device != tensors[0].device for t in tensors):
-        raise ValueError(f"{what}: tensors on different devices")
+    for t in tensors:
+        if t.get_device() != dev:
+            raise ValueError(f"{what}: tensors on different devices")
 
 
 def adam8_state(p):
@@ -60,58 +69,61 @@ def adam8_step(params, grads, states, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-
     shadows = [None] * len(params) if shadows is None else list(shadows)
     if not len(params) == len(grads) == len(states) == len(shadows):
         raise ValueError("adam8_step: as many gradients, states and shadows as parameters")
-    step, (b1, b2) = int(step), betas
+    step, (b1, b2), lr, eps, weight_decay = int(step), map(float, betas), float(lr), float(eps), float(weight_decay)
     if step < 1 or not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and eps >= 0.0 and weight_decay >= 0.0):
         raise ValueError("adam8_step: step >= 1, betas in [0, 1), eps and weight_decay not negative")
     if not params:
         return
-    arr = (N.Adam8Tensor * len(params))()
-    for i, (p, g, st, sh) in enumerate(zip(params, grads, states, shadows)):
-        if p.dtype not in (torch.float32, torch.bfloat16) or not p.is_contiguous() or g.dtype != p.dtype or g.shape != p.shape or not g.is_contiguous():
+    rows, touched, read = [], [], []
+    for p, g, st, sh in zip(params, grads, states, shadows):
+        dt = p.dtype
+        if dt not in _PARAM_TYPES or g.dtype is not dt or g.shape != p.shape or not p.is_contiguous() or not g.is_contiguous():
             raise ValueError("adam8_step: contiguous f32 or bf16 parameters with gradients of the same type and shape")
-        _check_state8(st, "adam8_step")
-        if st.exp_avg.numel() != p.numel():
+        m8, r8, ex, n = _state8_row(st, "adam8_step")
+        if n != p.numel():
             raise ValueError("adam8_step: a state of another size than its parameter")
-        a = arr[i]
-        a.p, a.g, a.m8, a.r8, a.ex, a.n = p.data_ptr(), g.data_ptr(), st.exp_avg.data_ptr(), st.exp_avg_sq.data_ptr(), st.exponents.data_ptr(), p.numel()
-        a.param_dtype = N.MTL_BF16 if p.dtype == torch.bfloat16 else N.MTL_F32
+        rows += (p.data_ptr(), g.data_ptr(), m8, r8, ex, n)
+        rows += (0, 0, 0) if sh is None else (sh.tensor.data_ptr(), p.shape[1], sh.tensor.stride(0))
+        rows.append(_PARAM_TYPES[dt])
+        touched += (p, *st)
+        read.append(g)
         if sh is not None:
-            a.shadow, a.cols, a.ld_shadow = sh.tensor.data_ptr(), p.shape[1], sh.tensor.stride(0)
-    for name, ptrs in (("parameter", [p.data_ptr() for p in params if p.numel()]), ("state", [st.exp_avg.data_ptr() for st in states if st.exp_avg.numel()])):
+            read.append(sh.tensor)
+    for name, at in (("parameter", 0), ("state", 2)):
+        ptrs = [x for x, n in zip(rows[at::10], rows[5::10]) if n]
         if len(set(ptrs)) < len(ptrs):
             raise ValueError(f"adam8_step: the same {name} twice in one step")
-    _one_gpu([t for p, g, st, sh in zip(params, grads, states, shadows) for t in (p, g, *st, *(() if sh is None else (sh.tensor,)))], "adam8_step")
+    _one_gpu(touched + read, "adam8_step")
     with N.on_device(params[0]):
-        N.check(N.lib().mtl_adam8_step(arr, len(params), float(lr), float(b1), float(b2), float(eps), float(weight_decay), 1 if decoupled_weight_decay else 0, step, N.stream()), "mtl_adam8_step")
-    for p, st, sh in zip(params, states, shadows):   # the kernel wrote through raw pointers: bump the autograd versions like an in-place op
-        torch.autograd.graph.increment_version((p, *st))
+        N.check(N.lib().mtl_adam8_step((N.i64 * len(rows))(*rows), len(params), lr, b1, b2, eps, weight_decay, 1 if decoupled_weight_decay else 0, step, N.stream()), "mtl_adam8_step")
+    torch.autograd.graph.increment_version(touched)   # the kernel wrote through raw pointers: bump the autograd versions like an in-place op
+    for p, sh in zip(params, shadows):
         if sh is not None:
             sh.version = p._version
 
 
-def _state8_array(states, ms, vs):
-    arr = (N.Adam8State * len(states))()
-    for a, st, m, v in zip(arr, states, ms, vs):
-        a.m8, a.r8, a.ex, a.n = st.exp_avg.data_ptr(), st.exp_avg_sq.data_ptr(), st.exponents.data_ptr(), st.exp_avg.numel()
-        a.m, a.v, a.dtype = m.data_ptr(), v.data_ptr(), N.MTL_BF16 if m.dtype == torch.bfloat16 else N.MTL_F32
-    return arr
+def _state8_rows(rows, ms, vs):
+    """mtl_adam8_state structures (7 64-bit words each)"""
+    flat = []
+    for (m8, r8, ex, n), m, v in zip(rows, ms, vs):
+        flat += (m8, r8, ex, n, m.data_ptr(), v.data_ptr(), _PARAM_TYPES[m.dtype])
+    return (N.i64 * len(flat))(*flat)
 
 
 @torch.no_grad()
 def adam8_moments(states, dtype=torch.float32):
     """[(exp_avg, exp_avg_sq)] that the states' codes stand for: exact in f32; in bf16 the first moment is exact, the second rounded once"""
     states = list(states)
-    if dtype not in (torch.float32, torch.bfloat16):
+    if dtype not in _PARAM_TYPES:
         raise ValueError("adam8_moments: f32 or bf16")
-    for st in states:
-        _check_state8(st, "adam8_moments")
+    rows = [_state8_row(st, "adam8_moments") for st in states]
     if not states:
         return []
     _one_gpu([t for st in states for t in st], "adam8_moments")
     with N.on_device(states[0].exp_avg):
-        out = [(torch.empty(st.exp_avg.shape, dtype=dtype, device=st.exp_avg.device), torch.empty(st.exp_avg.shape, dtype=dtype, device=st.exp_avg.device)) for st in states]
-        N.check(N.lib().mtl_adam8_moments(_state8_array(states, *zip(*out)), len(states), N.stream()), "mtl_adam8_moments")
-    return out
+        ms, vs = ([torch.empty_like(st.exp_avg, dtype=dtype) for st in states] for _ in range(2))
+        N.check(N.lib().mtl_adam8_moments(_state8_rows(rows, ms, vs), len(rows), N.stream()), "mtl_adam8_moments")
+    return list(zip(ms, vs))
 
 
 @torch.no_grad()
@@ -123,7 +135,7 @@ def adam8_quantize(exp_avg, exp_avg_sq, step=0):
     _one_gpu([m, v], "adam8_quantize")
     with N.on_device(m):
         st = adam8_state(m)
-        N.check(N.lib().mtl_adam8_quantize(_state8_array([st], [m], [v]), 1, int(step), N.stream()), "mtl_adam8_quantize")
+        N.check(N.lib().mtl_adam8_quantize(_state8_rows([_state8_row(st, "adam8_quantize")], [m], [v]), 1, int(step), N.stream()), "mtl_adam8_quantize")
     return st
 
 
