@@ -20,70 +20,36 @@ constexpr int SORT_MAX = 8192;
 constexpr int TILE = 4096;               // tokens per workgroup of the tiled sort
 constexpr int64_t CACHE_BYTES = (int64_t)256 << 20;      // the Infinity Cache
 constexpr int JOIN_SHORT = 16;           // windows behind its first one up to which a crossing run is joined by one wave
+constexpr unsigned SELF_TILES = 256;     // tiles up to which each sums all tiles' counts itself
 constexpr int MAX_BINS = 512;            // digits of up to 9 bits: two passes for every vocabulary up to 262143
 
-// ---------------------------------------------------------------- element access: W consecutive elements <-> fp32
-template <typename T, int W>
-struct Io;
-template <>
-struct Io<float, 1> {
-    static __device__ __forceinline__ void load(const void* p, int64_t i, float (&x)[1]) { x[0] = reinterpret_cast<const float*>(p)[i]; }
-    static __device__ __forceinline__ void store(void* p, int64_t i, const float (&x)[1]) { reinterpret_cast<float*>(p)[i] = x[0]; }
-};
-template <>
-struct Io<bf16_t, 1> {
-    static __device__ __forceinline__ void load(const void* p, int64_t i, float (&x)[1]) { x[0] = bf16_to_f32(reinterpret_cast<const bf16_t*>(p)[i]); }
-    static __device__ __forceinline__ void store(void* p, int64_t i, const float (&x)[1]) { reinterpret_cast<bf16_t*>(p)[i] = f32_to_bf16(x[0]); }
-};
-template <int W>
-struct Io<float, W> {
-    static __device__ __forceinline__ void load(const void* p, int64_t i, float (&x)[W]) {
-#pragma unroll
-        for (int j = 0; j < W; j += 4) {
-            const f32x4 v = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(p) + i + j);
-            x[j] = v[0]; x[j + 1] = v[1]; x[j + 2] = v[2]; x[j + 3] = v[3];
-        }
-    }
-    static __device__ __forceinline__ void store(void* p, int64_t i, const float (&x)[W]) {
-#pragma unroll
-        for (int j = 0; j < W; j += 4) *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(p) + i + j) = (f32x4){x[j], x[j + 1], x[j + 2], x[j + 3]};
-    }
-};
-template <int W>
-struct Io<bf16_t, W> {
-    static __device__ __forceinline__ void load(const void* p, int64_t i, float (&x)[W]) {
-        uint32_t w[W / 2];
-        const bf16_t* s = reinterpret_cast<const bf16_t*>(p) + i;
-        if (W == 8) { const u32x4 v = *reinterpret_cast<const u32x4*>(s); w[0] = v[0]; w[1] = v[1]; w[W / 2 - 2] = v[2]; w[W / 2 - 1] = v[3]; }
-        else { const u32x2 v = *reinterpret_cast<const u32x2*>(s); w[0] = v[0]; w[1] = v[1]; }
-#pragma unroll
-        for (int j = 0; j < W / 2; ++j) { x[2 * j] = __uint_as_float(w[j] << 16); x[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u); }
-    }
-    static __device__ __forceinline__ void store(void* p, int64_t i, const float (&x)[W]) {
-        bf16_t* d = reinterpret_cast<bf16_t*>(p) + i;
-        if (W == 8) *reinterpret_cast<u32x4*>(d) = (u32x4){pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[W - 4], x[W - 3]), pack_bf16x2(x[W - 2], x[W - 1])};
-        else *reinterpret_cast<u32x2*>(d) = (u32x2){pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
-    }
-};
+// ---------------------------------------------------------------- element access
+// Vectors of up to 16 bytes at any element's address (global accesses need no more alignment than their type's elements have): rows of odd width take the same path as others. A
+// lane whose W columns would reach beyond the row starts earlier instead (Cols) and computes the columns it shares with its neighbour a second time: the same bits.
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
 
 // W consecutive elements as loaded: held like this until they are used, so that many rows are in flight in few registers
 template <typename T, int W>
 struct Raw {
     static constexpr int WORDS = (W * (int)sizeof(T) + 3) / 4;
     uint32_t w[WORDS];
-    // STREAM: read once, past the caches
     template <bool STREAM, typename V>
     static __device__ __forceinline__ V get(const void* p) {
         const V* v = reinterpret_cast<const V*>(p);
         return STREAM ? __builtin_nontemporal_load(v) : *v;
     }
+    // STREAM: read once, past the caches
     template <bool STREAM>
     __device__ __forceinline__ void load(const T* p) {
-        if constexpr (sizeof(T) * W == 16) {
-            const u32x4 v = get<STREAM, u32x4>(p);
-            w[0] = v[0]; w[1] = v[1]; w[2] = v[2]; w[3] = v[3];
+        if constexpr (sizeof(T) * W >= 16) {
+#pragma unroll
+            for (int i = 0; i < WORDS; i += 4) {
+                const u32x4_any v = get<STREAM, u32x4_any>(reinterpret_cast<const uint32_t*>(p) + i);
+                w[i] = v[0]; w[i + 1] = v[1]; w[i + 2] = v[2]; w[i + 3] = v[3];
+            }
         } else if constexpr (sizeof(T) * W == 8) {
-            const u32x2 v = get<STREAM, u32x2>(p);
+            const u32x2_any v = get<STREAM, u32x2_any>(p);
             w[0] = v[0]; w[1] = v[1];
         } else if constexpr (sizeof(T) == 4) w[0] = get<STREAM, uint32_t>(p);
         else w[0] = get<STREAM, uint16_t>(p);
@@ -93,6 +59,36 @@ struct Raw {
         return __uint_as_float((j & 1) ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16);
     }
 };
+template <typename T, int W>
+__device__ __forceinline__ void load_w(const T* p, float (&x)[W]) {
+    Raw<T, W> r;
+    r.template load<false>(p);
+#pragma unroll
+    for (int j = 0; j < W; ++j) x[j] = r.at(j);
+}
+__device__ __forceinline__ void store_1(float* p, float x) { *p = x; }
+__device__ __forceinline__ void store_1(bf16_t* p, float x) { *p = f32_to_bf16(x); }
+template <typename T, int W>
+__device__ __forceinline__ void store_w(T* p, const float (&x)[W]) {
+    if constexpr (W == 1) store_1(p, x[0]);
+    else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int j = 0; j < W; j += 4)
+            *reinterpret_cast<u32x4_any*>(p + j) = (u32x4_any){__float_as_uint(x[j]), __float_as_uint(x[j + 1]), __float_as_uint(x[j + 2]), __float_as_uint(x[j + 3])};
+    } else if constexpr (W == 4) *reinterpret_cast<u32x2_any*>(p) = (u32x2_any){pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
+    else *reinterpret_cast<u32x4_any*>(p) = (u32x4_any){pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7])};
+}
+
+// a lane's columns at .. at + W - 1 of a row of d >= W; the first `skip` of them are its neighbour's as well; not `in`: it has none (and reads the row's first)
+struct Cols { int64_t at; int skip; bool in; };
+template <int W>
+__device__ __forceinline__ Cols cols_of(int64_t c, int64_t d) {
+    Cols k;
+    k.in = c < d;
+    k.at = !k.in ? 0 : (c <= d - W ? c : d - W);
+    k.skip = k.in ? (int)(c - k.at) : 0;
+    return k;
+}
 
 __device__ __forceinline__ int64_t load_id(const void* ids, int ids_i64, int64_t i) {
     return ids_i64 ? reinterpret_cast<const int64_t*>(ids)[i] : (int64_t)reinterpret_cast<const int32_t*>(ids)[i];
@@ -105,16 +101,16 @@ __global__ __launch_bounds__(256) void embedding_fwd_narrow_kernel(const void* _
                                                                    float scale, OT* __restrict__ out, int64_t ld_out, int lpr_log2) {
     const int lpr = 1 << lpr_log2;
     const int rows_per_block = 256 >> lpr_log2;
-    const int64_t c = (int64_t)(threadIdx.x & (lpr - 1)) * W;
-    if (c >= d) return;
+    const Cols k = cols_of<W>((int64_t)(threadIdx.x & (lpr - 1)) * W, d);
+    if (!k.in) return;
     for (int64_t i = (int64_t)blockIdx.x * rows_per_block + (threadIdx.x >> lpr_log2); i < N; i += (int64_t)gridDim.x * rows_per_block) {
         const int64_t id = load_id(ids, ids_i64, i);
         const bool in = id >= 0 && id < V;
         float x[W];
-        Io<TT, W>::load(table + (in ? id : 0) * ld_table, c, x);
+        load_w<TT, W>(table + (in ? id : 0) * ld_table + k.at, x);
 #pragma unroll
         for (int j = 0; j < W; ++j) x[j] = in ? x[j] * scale : 0.f;
-        Io<OT, W>::store(out + i * ld_out, c, x);
+        store_w<OT, W>(out + i * ld_out + k.at, x);
     }
 }
 
@@ -140,46 +136,48 @@ __global__ __launch_bounds__(256) void embedding_fwd_kernel(const void* __restri
         src[r] = in ? table + id * ld_table : nullptr;
     }
     for (int64_t c = ((item - group * split) * 64 + lane) * W; c < d; c += (int64_t)64 * W * split) {
+        const int64_t at = cols_of<W>(c, d).at;
         Raw<TT, W> x[ROWS];
 #pragma unroll
         for (int r = 0; r < ROWS; ++r)
-            if (src[r]) x[r].template load<false>(src[r] + c);
+            if (src[r]) x[r].template load<false>(src[r] + at);
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
             if (r >= n) break;
             float y[W];
 #pragma unroll
             for (int j = 0; j < W; ++j) y[j] = src[r] ? x[r].at(j) * scale : 0.f;
-            Io<OT, W>::store(out + (i0 + r) * ld_out, c, y);
+            store_w<OT, W>(out + (i0 + r) * ld_out + at, y);
         }
     }
 }
 
 // ---------------------------------------------------------------- zero rows of the dense gradient
-// width: 16, 4 or 2 bytes per store. stream: the gradient is larger than the Infinity Cache (256 MB): non-temporal stores from few workgroups. 2.1 GB: ordinary stores 345 us and the sum
-// behind them 65 us (it evicts their dirty lines), non-temporal from 128 workgroups 353 and 42; 154 MB, which the cache holds: 24 us against 29 and more.
+// rows of row_bytes each, ld_bytes apart (one row where the gradient is contiguous), stores of `width` (16, 4 or 2) bytes and a row's last ones of 2. stream: the gradient is larger than
+// the Infinity Cache (256 MB): non-temporal stores from few workgroups. 2.1 GB: ordinary stores 345 us and the sum behind them 65 us (it evicts their dirty lines), non-temporal from 128
+// workgroups 353 and 42; 154 MB, which the cache holds: 24 us against 29 and more.
 struct Fill { char* p; int64_t rows, row_bytes, ld_bytes; int width, stream; };
 
 __device__ __forceinline__ void fill_zero(const Fill& f, int64_t block, int64_t blocks) {
-    const int64_t per_row = f.row_bytes / f.width, total = f.rows * per_row;
-    if (f.row_bytes == f.ld_bytes && f.width == 16) {
-        u32x4* p = reinterpret_cast<u32x4*>(f.p);
-        const u32x4 zero = {0, 0, 0, 0};
-        for (int64_t i = block * 4096 + threadIdx.x; i < total; i += blocks * 4096) {       // (1024 threads, four stores each)
+    const u32x4 zero = {0, 0, 0, 0};
+    const bool flat = f.rows == 1;
+    for (int64_t r = flat ? 0 : block; r < f.rows; r += flat ? 1 : blocks) {
+        char* row = f.p + r * f.ld_bytes;
+        const int64_t n = f.row_bytes / f.width, first = flat ? block * 4096 : 0, step = flat ? blocks * 4096 : 4096;      // (1024 threads, four stores each)
+        for (int64_t i = first + threadIdx.x; i < n; i += step) {
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-                if (i + u * 1024 < total) {
-                    if (f.stream) __builtin_nontemporal_store(zero, p + i + u * 1024);
-                    else p[i + u * 1024] = zero;
-                }
+            for (int u = 0; u < 4; ++u) {
+                const int64_t at = i + u * 1024;
+                if (at >= n) break;
+                if (f.width == 16) {
+                    if (f.stream) __builtin_nontemporal_store(zero, reinterpret_cast<u32x4*>(row) + at);
+                    else reinterpret_cast<u32x4*>(row)[at] = zero;
+                } else if (f.width == 4) reinterpret_cast<uint32_t*>(row)[at] = 0;
+                else reinterpret_cast<uint16_t*>(row)[at] = 0;
+            }
         }
-        return;
-    }
-    for (int64_t i = block * blockDim.x + threadIdx.x; i < total; i += blocks * blockDim.x) {
-        const int64_t r = i / per_row, at = r * f.ld_bytes + (i - r * per_row) * f.width;
-        if (f.width == 16) *reinterpret_cast<u32x4*>(f.p + at) = (u32x4){0, 0, 0, 0};
-        else if (f.width == 4) *reinterpret_cast<uint32_t*>(f.p + at) = 0;
-        else *reinterpret_cast<uint16_t*>(f.p + at) = 0;
+        const int64_t tail = n * f.width + threadIdx.x * 2;
+        if ((!flat || block == 0) && tail < f.row_bytes) *reinterpret_cast<uint16_t*>(row + tail) = 0;
     }
 }
 
@@ -334,11 +332,41 @@ __global__ __launch_bounds__(1024) void embedding_sort_count_kernel(const void* 
     for (int i = threadIdx.x; i < (1 << bits); i += 1024) hist[((int64_t)blockIdx.x << bits) + i] = cnt[i];
 }
 
-// Each tile forms the first rank of its elements of every digit itself, from all tiles' counts: tokens of smaller digits plus those of the same digit in earlier tiles. (A scan by one
-// workgroup in between measured 13 - 16 us and a launch at 200 003 tokens; the counts of all tiles are 50 KB there and sit in the L2.)
+// More than SELF_TILES tiles: hist[tile][digit] becomes the number of the digit's tokens in earlier tiles, totals[digit] all of them. A workgroup per 64 digits, 16 waves over the tiles.
+__global__ __launch_bounds__(1024) void embedding_sort_scan_kernel(uint32_t* __restrict__ hist, int tiles, int bits, uint32_t* __restrict__ totals) {
+    __shared__ uint32_t sums[16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, dgt = blockIdx.x * 64 + lane;
+    const bool in = dgt < (1 << bits);
+    const int t0 = (int)((int64_t)tiles * wave / 16), t1 = (int)((int64_t)tiles * (wave + 1) / 16);
+    uint32_t s = 0;
+    if (in) {
+#pragma unroll 8
+        for (int t = t0; t < t1; ++t) s += hist[((int64_t)t << bits) + dgt];
+    }
+    sums[wave][lane] = s;
+    __syncthreads();
+    uint32_t at = 0;
+    for (int w = 0; w < wave; ++w) at += sums[w][lane];
+    if (!in) return;
+    if (wave == 15) totals[dgt] = at + s;
+    for (int t = t0; t < t1; t += 8) {
+        uint32_t h[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) h[u] = t + u < t1 ? hist[((int64_t)(t + u) << bits) + dgt] : 0u;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            if (t + u < t1) hist[((int64_t)(t + u) << bits) + dgt] = at;
+            at += h[u];
+        }
+    }
+}
+
+// The first rank of a tile's elements of every digit: tokens of smaller digits plus those of the same digit in earlier tiles. Up to SELF_TILES tiles each tile sums them up itself from
+// all tiles' counts (totals == NULL); above that the work would grow with the square of the tiles, and the scan kernel has done it. Per digit of 50257 ids, scan + scatter against
+// scatter alone: 100 000 tokens 15.1 / 12.1 us, 400 000 17.2 / 13.9, 1 M 22.5 / 20.9, 2 M 33 / 41, and a launch.
 __global__ __launch_bounds__(1024) void embedding_sort_scatter_kernel(const void* __restrict__ ids, int ids_i64, int64_t N, int64_t V, int64_t pad, const uint32_t* __restrict__ keys,
                                                                       const uint32_t* __restrict__ poss, int shift, int bits, int tiles, const uint32_t* __restrict__ hist,
-                                                                      uint32_t* __restrict__ sid, uint32_t* __restrict__ spos) {
+                                                                      const uint32_t* __restrict__ totals, uint32_t* __restrict__ sid, uint32_t* __restrict__ spos) {
     __shared__ uint32_t cnt[16 * MAX_BINS];
     __shared__ uint32_t sums[2 * 1024];
     __shared__ uint32_t tot[16];
@@ -358,11 +386,15 @@ __global__ __launch_bounds__(1024) void embedding_sort_scatter_kernel(const void
     // counts of digit threadIdx.x % bins: over every `groups`-th tile, all of them and the earlier ones
     const int bins = 1 << bits, groups = 1024 >> bits, dgt = threadIdx.x & (bins - 1);
     uint32_t all = 0, earlier = 0;
+    if (totals) {
+        if ((int)threadIdx.x < bins) { all = totals[dgt]; earlier = hist[((int64_t)blockIdx.x << bits) + dgt]; }
+    } else {
 #pragma unroll 8
-    for (int t = threadIdx.x >> bits; t < tiles; t += groups) {
-        const uint32_t h = hist[((int64_t)t << bits) + dgt];
-        all += h;
-        earlier += t < (int)blockIdx.x ? h : 0u;
+        for (int t = threadIdx.x >> bits; t < tiles; t += groups) {
+            const uint32_t h = hist[((int64_t)t << bits) + dgt];
+            all += h;
+            earlier += t < (int)blockIdx.x ? h : 0u;
+        }
     }
     sums[threadIdx.x] = all;
     sums[1024 + threadIdx.x] = earlier;
@@ -403,18 +435,28 @@ struct SumArgs {
 };
 
 template <typename GT, int W>
-__device__ __forceinline__ void write_row(const SumArgs& a, uint32_t id, int64_t c, const float (&acc)[W]) {
-    const int64_t at = (int64_t)id * a.ld_grad + c;
+__device__ __forceinline__ void write_row(const SumArgs& a, uint32_t id, const Cols& k, const float (&acc)[W]) {
+    GT* to = reinterpret_cast<GT*>(a.grad) + (int64_t)id * a.ld_grad + k.at;
     float y[W];
 #pragma unroll
     for (int j = 0; j < W; ++j) y[j] = acc[j] * a.scale;
     if (a.accumulate) {
+        if (W > 1 && k.skip) {                                  // columns shared with a neighbour are added once: by it
+#pragma unroll
+            for (int j = 0; j < W; ++j)
+                if (j >= k.skip) {
+                    float old[1];
+                    load_w<GT, 1>(to + j, old);
+                    store_1(to + j, y[j] + old[0]);
+                }
+            return;
+        }
         float old[W];
-        Io<GT, W>::load(a.grad, at, old);
+        load_w<GT, W>(to, old);
 #pragma unroll
         for (int j = 0; j < W; ++j) y[j] += old[j];
     }
-    Io<GT, W>::store(a.grad, at, y);
+    store_w<GT, W>(to, y);
 }
 
 // dout is read once and past the caches: 200 003 rows of 2 KB 94 us, through the caches 133 (the loads evict what the launches before left dirty there).
@@ -426,8 +468,8 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(const SumArgs a) {
     const int64_t item = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t w = item / a.chunks;
     if (w >= a.windows) return;
-    const int64_t c = (item - w * a.chunks) * (64 * W) + lane * W;
-    const bool in = c < a.d;                                    // (d % W == 0 wherever W > 1)
+    const int64_t chunk = item - w * a.chunks;
+    const Cols k = cols_of<W>(chunk * (64 * W) + lane * W, a.d);
     const int64_t i0 = w * a.S, i1 = i0 + a.S < a.N ? i0 + a.S : a.N;
     const uint32_t none = (uint32_t)a.V;
     uint32_t ids = none, poss = 0;
@@ -435,13 +477,13 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(const SumArgs a) {
     const uint32_t before = i0 > 0 ? a.sid[i0 - 1] : none, after = i1 < a.N ? a.sid[i1] : none;
     const int n = (int)__popcll(__ballot(ids != none));         // (sorted: the tokens without a gradient are the last ones)
     if (n == 0) return;
-    const DT* dout = reinterpret_cast<const DT*>(a.dout) + (in ? c : 0);
+    const DT* dout = reinterpret_cast<const DT*>(a.dout) + k.at;
     uint32_t cur = (uint32_t)__builtin_amdgcn_readlane((int)ids, 0);
     bool came_in = before == cur;
     float acc[W];
 #pragma unroll
     for (int j = 0; j < W; ++j) acc[j] = 0.f;
-    float* part = a.part + w * 2 * a.d + c;
+    float* part = a.part + w * 2 * a.d + k.at;
     Raw<DT, W> now[GROUP], next[GROUP];
     auto fetch = [&](Raw<DT, W>(&x)[GROUP], int i) {
 #pragma unroll
@@ -456,9 +498,9 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(const SumArgs a) {
             if (i + u >= n) break;
             const uint32_t id = (uint32_t)__builtin_amdgcn_readlane((int)ids, i + u);
             if (id != cur) {                                     // (uniform) the run of `cur` ends here, inside the window
-                if (in) {
-                    if (came_in) Io<float, W>::store(part, 0, acc);
-                    else write_row<GT, W>(a, cur, c, acc);
+                if (k.in) {
+                    if (came_in) store_w<float, W>(part, acc);
+                    else write_row<GT, W>(a, cur, k, acc);
                 }
                 cur = id;
                 came_in = false;
@@ -478,13 +520,13 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(const SumArgs a) {
         add(next, i + GROUP);
     }
     const bool goes_on = after == cur;
-    if (in) {
-        if (came_in) Io<float, W>::store(part, 0, acc);
-        else if (goes_on) Io<float, W>::store(part, a.d, acc);
-        else write_row<GT, W>(a, cur, c, acc);
+    if (k.in) {
+        if (came_in) store_w<float, W>(part, acc);
+        else if (goes_on) store_w<float, W>(part + a.d, acc);
+        else write_row<GT, W>(a, cur, k, acc);
     }
     // the window in which a crossing run starts goes on a list (whose order shows nowhere: each entry is a whole run): LONG of runs that cover more than JOIN_SHORT windows behind it
-    if (goes_on && !came_in && c == 0) {
+    if (goes_on && !came_in && chunk == 0 && lane == 0) {
         const int64_t far = i1 + (int64_t)JOIN_SHORT * a.S;
         if (far < a.N && a.sid[far] == cur) a.list[a.windows - 1 - atomicAdd(a.list_n + 1, 1u)] = (uint32_t)w;
         else a.list[atomicAdd(a.list_n, 1u)] = (uint32_t)w;
@@ -512,21 +554,21 @@ __global__ __launch_bounds__(1024) void embedding_join_kernel(const SumArgs a, i
         const int64_t items = (int64_t)a.list_n[0] * chunks, step = (int64_t)(gridDim.x - long_blocks) * 16;
         for (int64_t item = (int64_t)(blockIdx.x - long_blocks) * 16 + wave; item < items; item += step) {
             const int64_t w = a.list[item / chunks];
-            const int64_t c = (item % chunks) * (64 * W) + lane * W;
+            const Cols k = cols_of<W>((item % chunks) * (64 * W) + lane * W, a.d);
             const uint32_t id = a.sid[(w + 1) * a.S];
             const int n = (int)run_windows(a, w, id);
-            if (c >= a.d) continue;
-            const float* part = a.part + w * 2 * a.d + c;
+            if (!k.in) continue;
+            const float* part = a.part + w * 2 * a.d + k.at;
             float s[W];
-            Io<float, W>::load(part, a.d, s);
+            load_w<float, W>(part + a.d, s);
 #pragma unroll 4
-            for (int k = 1; k <= n; ++k) {
+            for (int i = 1; i <= n; ++i) {
                 float x[W];
-                Io<float, W>::load(part, (int64_t)k * 2 * a.d, x);
+                load_w<float, W>(part + (int64_t)i * 2 * a.d, x);
 #pragma unroll
                 for (int j = 0; j < W; ++j) s[j] += x[j];
             }
-            write_row<GT, W>(a, id, c, s);
+            write_row<GT, W>(a, id, k, s);
         }
         return;
     }
@@ -550,7 +592,7 @@ __global__ __launch_bounds__(1024) void embedding_join_kernel(const SumArgs a, i
             float t[1] = {sums[0][lane]};
 #pragma unroll
             for (int v = 1; v < 16; ++v) t[0] += sums[v][lane];
-            write_row<GT, 1>(a, id, c, t);
+            write_row<GT, 1>(a, id, cols_of<1>(c, a.d), t);
         }
         __syncthreads();
     }
@@ -573,7 +615,8 @@ inline int64_t chunks_of(int64_t d, int W) { return (d + 64 * W - 1) / (64 * W);
 struct Plan { int64_t sid, spos, sid2, spos2, hist, list, part, total; };
 inline Plan plan_for(int64_t N, int64_t V, int64_t d) {
     Plan p;
-    int64_t at = 256;                                             // list_n
+    int64_t at = 8 + 4 * MAX_BINS;                                // two list counts, the scan's digit totals
+    at = up(at, 256);
     auto take = [&](int64_t bytes) { const int64_t here = at; at += up(bytes, 256); return here; };
     const bool small = N <= SORT_MAX;
     const int64_t tiles = (N + TILE - 1) / TILE, windows = (N + 7) / 8;      // (8: the shortest window)
@@ -634,12 +677,6 @@ void launch_fwd(const void* ids, int ids_i64, int64_t N, const void* table, int6
 
 inline bool dtype_ok(int t) { return t == MTL_F32 || t == MTL_BF16; }
 inline int size_of(int t) { return t == MTL_BF16 ? 2 : 4; }
-// W columns per lane are possible for this operand: W * size <= 16 B accesses, aligned
-inline bool fits(const void* p, int64_t ld, int dtype, int64_t d, int W) {
-    const int64_t a = (int64_t)W * size_of(dtype) < 16 ? (int64_t)W * size_of(dtype) : 16;
-    return d % W == 0 && (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0 && (ld * size_of(dtype)) % a == 0;
-}
-
 }  // namespace
 
 extern "C" int mtl_embedding_fwd(const void* ids, int ids_i64, int64_t N, const void* table, int table_dtype, int64_t V, int64_t d, int64_t ld_table, float scale, void* out, int out_dtype,
@@ -649,10 +686,8 @@ extern "C" int mtl_embedding_fwd(const void* ids, int ids_i64, int64_t N, const 
     if (!ids || !table || !out) return MTL_ERR_ARG;
     if (((uintptr_t)ids & (ids_i64 ? 7 : 3)) || ((uintptr_t)table & (size_of(table_dtype) - 1)) || ((uintptr_t)out & (size_of(out_dtype) - 1))) return MTL_ERR_ALIGN;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    // 16-byte accesses of the wider operand's type where both allow it
-    int W = 1;
-    for (int c : {4, 8})
-        if (fits(table, ld_table, table_dtype, d, c) && fits(out, ld_out, out_dtype, d, c) && (c == 4 || (table_dtype == MTL_BF16 && out_dtype == MTL_BF16))) W = c;
+    // 16-byte accesses of the wider type (8 columns only where both are bf16), one column where the row is shorter
+    const int W = table_dtype == MTL_BF16 && out_dtype == MTL_BF16 && d >= 8 ? 8 : (d >= 4 ? 4 : 1);
     if (table_dtype == MTL_F32 && out_dtype == MTL_F32) launch_fwd<float, float>(ids, ids_i64, N, table, V, d, ld_table, scale, out, ld_out, W, st);
     else if (table_dtype == MTL_F32) launch_fwd<float, bf16_t>(ids, ids_i64, N, table, V, d, ld_table, scale, out, ld_out, W, st);
     else if (out_dtype == MTL_F32) launch_fwd<bf16_t, float>(ids, ids_i64, N, table, V, d, ld_table, scale, out, ld_out, W, st);
@@ -677,11 +712,11 @@ extern "C" int mtl_embedding_bwd(const void* ids, int ids_i64, int64_t N, const 
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     if (padding_idx < 0) padding_idx = -1;
     Fill f = {(char*)grad, accumulate ? 0 : V, d * gs, ld_grad * gs, 2, V * d * gs > CACHE_BYTES};
+    if (!accumulate && ld_grad == d) { f.rows = 1; f.row_bytes = V * d * gs; }
     for (int w : {4, 16})
-        if (f.row_bytes % w == 0 && f.ld_bytes % w == 0 && ((uintptr_t)grad & (w - 1)) == 0) f.width = w;
-    const int64_t fill_items = f.rows * (f.row_bytes / f.width);
-    const int64_t fill_want = (fill_items + 4095) / 4096, fill_most = f.stream ? 128 : 512;
-    const unsigned fill_blocks = (unsigned)(fill_want < fill_most ? fill_want : fill_most);
+        if (((uintptr_t)grad & (w - 1)) == 0 && (f.rows == 1 || f.ld_bytes % w == 0)) f.width = w;
+    const int64_t fill_want = f.rows == 1 ? (f.row_bytes / f.width + 4095) / 4096 : f.rows, fill_most = f.stream ? 128 : 512;
+    const unsigned fill_blocks = (unsigned)(fill_want < fill_most ? (f.rows > 0 && fill_want < 1 ? 1 : fill_want) : fill_most);
     char* ws = reinterpret_cast<char*>(workspace);
     if (N == 0) {
         // no token: zeros only (no tile to count)
@@ -709,14 +744,16 @@ extern "C" int mtl_embedding_bwd(const void* ids, int ids_i64, int64_t N, const 
             uint32_t* ko = to_first ? sid : other_id;
             uint32_t* po = to_first ? spos : other_pos;
             hipLaunchKernelGGL(embedding_sort_count_kernel, dim3(tiles + (q == 0 ? fill_blocks : 0)), dim3(1024), 0, st, ids, ids_i64, N, V, padding_idx, kin, q * bits, bits, (int)tiles, hist, list_n, f);
-            hipLaunchKernelGGL(embedding_sort_scatter_kernel, dim3(tiles), dim3(1024), 0, st, ids, ids_i64, N, V, padding_idx, kin, pin, q * bits, bits, (int)tiles, hist, ko, po);
+            uint32_t* totals = tiles > SELF_TILES ? list_n + 2 : nullptr;          // (MAX_BINS words behind the two list counts)
+            if (totals) hipLaunchKernelGGL(embedding_sort_scan_kernel, dim3(((1u << bits) + 63) / 64), dim3(1024), 0, st, hist, (int)tiles, bits, totals);
+            hipLaunchKernelGGL(embedding_sort_scatter_kernel, dim3(tiles), dim3(1024), 0, st, ids, ids_i64, N, V, padding_idx, kin, pin, q * bits, bits, (int)tiles, hist, totals, ko, po);
             MTL_CHECK_LAUNCH();
             kin = ko; pin = po;
         }
     }
-    int W = 1;
-    for (int c : {4, 8})
-        if (d > 64 * (c / 4) && fits(dout, ld_dout, dout_dtype, d, c) && fits(grad, ld_grad, grad_dtype, d, c) && (c == 4 || (dout_dtype == MTL_BF16 && (d % 512 == 0 || d >= 2048)))) W = c;
+    // columns per lane: 16 bytes of dout, less where that would leave a good part of the wave without columns
+    int W = d > 64 ? 4 : 1;
+    if (dout_dtype == MTL_BF16 && d > 256 && (d + 511) / 512 * 512 <= d + d / 3) W = 8;
     SumArgs a;
     a.sid = sid; a.spos = spos; a.N = N; a.V = V; a.d = d; a.ld_dout = ld_dout; a.ld_grad = ld_grad; a.dout = dout; a.grad = grad;
     a.part = reinterpret_cast<float*>(ws + p.part); a.list = reinterpret_cast<uint32_t*>(ws + p.list); a.list_n = list_n;
@@ -732,7 +769,7 @@ extern "C" int mtl_embedding_bwd(const void* ids, int ids_i64, int64_t N, const 
     else launch_sum<float, float>(a, W, st);
     MTL_CHECK_LAUNCH();
     if (a.windows > 1) {
-        const int64_t most = ((a.windows - 1) * chunks_of(d, W > 4 ? 4 : W) + 15) / 16;      // waves of 16 short runs' column chunks
+        const int64_t most = ((a.windows - 1) * chunks_of(d, W > 1 ? 4 : 1) + 15) / 16;      // waves of 16 short runs' column chunks
         const int64_t most_long = (a.windows / (JOIN_SHORT + 1)) * chunks_of(d, 1);           // a long run takes at least that many windows
         const unsigned lb = (unsigned)(most_long < 256 ? most_long : 256), sb = (unsigned)(most < 256 ? most : 256);
         if (W > 1 && g16) hipLaunchKernelGGL((embedding_join_kernel<bf16_t, 4>), dim3(lb + sb), dim3(1024), 0, st, a, (int)lb);

@@ -118,7 +118,7 @@ __device__ __forceinline__ void load_turn(const mtl_qk_norm_rope_args& a, int64_
 
 // heads [h0, h1) of one row: forward
 template <typename T, int W, int LPH, int C>
-__device__ __forceinline__ void heads_fwd(const T* __restrict__ x, T* y, int h0, int h1, int D, float eps, float inv_d, const Lane<W, LPH, C>& L, const float (&wl)[C][W], const float (&wh)[C][W],
+__device__ __forceinline__ void heads_fwd(const T* x, T* y, int h0, int h1, int D, float eps, float inv_d, const Lane<W, LPH, C>& L, const float (&wl)[C][W], const float (&wh)[C][W],
                                           const float (&cs)[C][W], const float (&sn)[C][W]) {
     constexpr int G = 64 / LPH, U = (W == 8 && C == 1) ? 2 : 1;      // heads per step of the wave, steps whose loads are in flight together
     const int g = (threadIdx.x & 63) / LPH;
@@ -199,7 +199,7 @@ __global__ __launch_bounds__(WAVES * 64) void qk_norm_rope_fwd_kernel(const mtl_
 
 // all heads of one row: backward; gl / gh accumulate dw
 template <typename T, int W, int LPH, int C, bool DW>
-__device__ __forceinline__ void heads_bwd(const T* __restrict__ x, const T* dy, T* dx, int h1, int D, float eps, float inv_d, const Lane<W, LPH, C>& L, const float (&wl)[C][W],
+__device__ __forceinline__ void heads_bwd(const T* x, const T* dy, T* dx, int h1, int D, float eps, float inv_d, const Lane<W, LPH, C>& L, const float (&wl)[C][W],
                                           const float (&wh)[C][W], const float (&cs)[C][W], const float (&sn)[C][W], float (&gl)[C][W], float (&gh)[C][W]) {
     constexpr int G = 64 / LPH;
     const int g = (threadIdx.x & 63) / LPH;

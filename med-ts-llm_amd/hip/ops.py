@@ -473,8 +473,13 @@ def embedding_bwd(dout, ids, V, scale=1.0, padding_idx=None, out=None, accumulat
             raise ValueError("embedding_bwd: out must be f32 or bf16 [V, d]")
         ld, out_dtype = _table_ld(out, "out"), out.dtype
     flat, rows = _ids(ids), _rows(dout, d)
-    _req_gpu(rows, flat, *(() if out is None else (out,)))
     n = rows.shape[0]
+    if out is not None and n:
+        a0, b0 = out.data_ptr(), rows.data_ptr()
+        a1, b1 = a0 + ((V - 1) * ld + d) * out.element_size(), b0 + ((n - 1) * rows.stride(0) + d) * rows.element_size()
+        if a0 < b1 and b0 < a1:
+            raise ValueError("embedding_bwd: out and dout share memory")
+    _req_gpu(rows, flat, *(() if out is None else (out,)))
     with N.on_device(rows):
         if out is None:
             out = rows.new_empty((V, d), dtype=out_dtype)

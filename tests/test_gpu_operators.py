@@ -89,7 +89,7 @@ EMBED = [  # N, V, d, dout, grad, pad
     (0, 3, 8, F32, F32, None), (1, 1, 1, F32, F32, None), (7, 5, 3, BF16, F32, 2), (8, 100, 64, BF16, BF16, None), (9, 2, 65, F32, F32, 0), (64, 10, 66, F32, BF16, None),
     (1000, 7, 200, BF16, F32, 3), (1025, 513, 128, BF16, BF16, None), (4096, 262143, 20, F32, F32, None), (4097, 511, 96, F32, F32, 5), (5000, 50257, 768, BF16, F32, 11),
     (8192, 1, 512, BF16, F32, None), (8193, 262144, 24, F32, F32, None), (16384, 100, 2048, BF16, BF16, 4), (16385, 300001, 33, BF16, F32, None), (40000, 2, 130, F32, F32, None),
-    (50001, 32000, 256, BF16, BF16, 31999), (300000, 70000, 40, BF16, F32, 1), (200003, 3, 520, BF16, F32, None)]
+    (1100000, 5000, 4, F32, F32, 7), (50001, 32000, 256, BF16, BF16, 31999), (300000, 70000, 40, BF16, F32, 1), (200003, 3, 520, BF16, F32, None)]
 
 
 @pytest.mark.parametrize("N,V,d,dt,gt,pad", EMBED)
@@ -140,6 +140,33 @@ def test_embedding_gradient_layouts(ops):
     assert bool(ops.embedding_bwd(masked, ids2, 50).isfinite().all())
     got = ops.embedding_bwd(masked, ids, 50).isfinite().all(1)
     assert not got[ids[0, 5]] and int((~got).sum()) == 1
+
+
+def test_embedding_offsets_beyond_32_bits(ops):
+    """table, output and gradient of more than 2^31 elements (4.6 GB each in bf16): rows at both ends, looked up, summed and zeroed"""
+    V, d, N = 140000, 16384, 140001
+    g = gen(13)
+    table = torch.zeros(V, d, dtype=BF16, device="cuda")
+    table[-3:] = randn(g, 3, d, dtype=BF16)
+    ids = torch.randint(V // 2, V - 10, (N,), generator=g, device="cuda")
+    ids[-1], ids[0], ids[N // 2] = V - 1, V - 2, V - 1
+    out = ops.embedding_fwd(ids, table)
+    assert torch.equal(out[-1], table[-1]) and torch.equal(out[0], table[-2]) and torch.equal(out[N // 2], table[-1]) and not out[1:1000].any()
+    out.fill_(1.0)
+    out[-1] = randn(g, d, dtype=BF16)
+    want = (out[-1].double() + 1.0)
+    grad = ops.embedding_bwd(out, ids, V, out_dtype=BF16, out=table)
+    within(grad[-1], want, 3 * U * (want.abs() + 1) + HALF[BF16] * (want.abs() + 3 * U))
+    assert bool((grad[-2] == 1).all()) and not grad[:V // 2].any() and not grad[-10:-2].any()
+    n = torch.bincount(ids, minlength=V).double()
+    assert torch.equal(grad[V // 2:V - 2, -1].double(), n[V // 2:V - 2].to(BF16).double())
+
+
+def test_embedding_refuses_shared_memory(ops):
+    x = torch.zeros(64, 8, device="cuda")
+    with pytest.raises(ValueError):
+        ops.embedding_bwd(x[:10], torch.zeros(10, dtype=torch.int64, device="cuda"), 20, out=x[5:25])
+    assert ops.embedding_bwd(x[:10], torch.zeros(10, dtype=torch.int64, device="cuda"), 20, out=x[10:30]).shape == (20, 8)
 
 
 def test_embedding_function_against_differences(ops):
