@@ -18,7 +18,6 @@ namespace {
 // Tokens that one workgroup sorts in its LDS: 4096 14 us, 8192 24 us (16 keys per thread spill: 16384 tokens 117 us, against 29 us and three more launches in tiles).
 constexpr int SORT_MAX = 8192;
 constexpr int TILE = 4096;               // tokens per workgroup of the tiled sort
-constexpr int64_t CACHE_BYTES = (int64_t)256 << 20;      // the Infinity Cache
 constexpr int JOIN_SHORT = 16;           // windows behind its first one up to which a crossing run is joined by one wave
 constexpr unsigned SELF_TILES = 256;     // tiles up to which each sums all tiles' counts itself
 constexpr int MAX_BINS = 512;            // digits of up to 9 bits: two passes for every vocabulary up to 262143
@@ -153,10 +152,9 @@ __global__ __launch_bounds__(256) void embedding_fwd_kernel(const void* __restri
 }
 
 // ---------------------------------------------------------------- zero rows of the dense gradient
-// rows of row_bytes each, ld_bytes apart (one row where the gradient is contiguous), stores of `width` (16, 4 or 2) bytes and a row's last ones of 2. stream: the gradient is larger than
-// the Infinity Cache (256 MB): non-temporal stores from few workgroups. 2.1 GB: ordinary stores 345 us and the sum behind them 65 us (it evicts their dirty lines), non-temporal from 128
-// workgroups 353 and 42; 154 MB, which the cache holds: 24 us against 29 and more.
-struct Fill { char* p; int64_t rows, row_bytes, ld_bytes; int width, stream; };
+// rows of row_bytes each, ld_bytes apart (one row where the gradient is contiguous), stores of `width` (16, 4 or 2) bytes and a row's last ones of 2. Ordinary stores from 512
+// workgroups: 2.1 GB in 345 us (6.1 TB/s). Non-temporal ones spare the sum behind them the eviction of dirty lines (65 -> 42 us) and take that longer themselves: equal at 2.1 GB, worse below.
+struct Fill { char* p; int64_t rows, row_bytes, ld_bytes; int width; };
 
 __device__ __forceinline__ void fill_zero(const Fill& f, int64_t block, int64_t blocks) {
     const u32x4 zero = {0, 0, 0, 0};
@@ -169,10 +167,8 @@ __device__ __forceinline__ void fill_zero(const Fill& f, int64_t block, int64_t 
             for (int u = 0; u < 4; ++u) {
                 const int64_t at = i + u * 1024;
                 if (at >= n) break;
-                if (f.width == 16) {
-                    if (f.stream) __builtin_nontemporal_store(zero, reinterpret_cast<u32x4*>(row) + at);
-                    else reinterpret_cast<u32x4*>(row)[at] = zero;
-                } else if (f.width == 4) reinterpret_cast<uint32_t*>(row)[at] = 0;
+                if (f.width == 16) reinterpret_cast<u32x4*>(row)[at] = zero;
+                else if (f.width == 4) reinterpret_cast<uint32_t*>(row)[at] = 0;
                 else reinterpret_cast<uint16_t*>(row)[at] = 0;
             }
         }
@@ -711,11 +707,11 @@ extern "C" int mtl_embedding_bwd(const void* ids, int ids_i64, int64_t N, const 
     if (N > 0 && workspace_bytes < mtl_embedding_bwd_workspace_bytes(N, V, d)) return MTL_ERR_WORKSPACE;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     if (padding_idx < 0) padding_idx = -1;
-    Fill f = {(char*)grad, accumulate ? 0 : V, d * gs, ld_grad * gs, 2, V * d * gs > CACHE_BYTES};
+    Fill f = {(char*)grad, accumulate ? 0 : V, d * gs, ld_grad * gs, 2};
     if (!accumulate && ld_grad == d) { f.rows = 1; f.row_bytes = V * d * gs; }
     for (int w : {4, 16})
         if (((uintptr_t)grad & (w - 1)) == 0 && (f.rows == 1 || f.ld_bytes % w == 0)) f.width = w;
-    const int64_t fill_want = f.rows == 1 ? (f.row_bytes / f.width + 4095) / 4096 : f.rows, fill_most = f.stream ? 128 : 512;
+    const int64_t fill_want = f.rows == 1 ? (f.row_bytes / f.width + 4095) / 4096 : f.rows, fill_most = 512;
     const unsigned fill_blocks = (unsigned)(fill_want < fill_most ? (f.rows > 0 && fill_want < 1 ? 1 : fill_want) : fill_most);
     char* ws = reinterpret_cast<char*>(workspace);
     if (N == 0) {

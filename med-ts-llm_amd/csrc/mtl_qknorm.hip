@@ -30,59 +30,66 @@ __device__ __forceinline__ float group_sum(float v) {
     return v;
 }
 
+// vectors at any element's address (global accesses need no more alignment than their elements have)
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 template <typename T, int W>
-__device__ __forceinline__ void load_w(const T* p, float (&x)[W]);
-template <>
-__device__ __forceinline__ void load_w<float, 8>(const float* p, float (&x)[8]) {
-    const f32x4 a = reinterpret_cast<const f32x4*>(p)[0], b = reinterpret_cast<const f32x4*>(p)[1];
+__device__ __forceinline__ void load_w(const T* p, float (&x)[W]) {
+    if constexpr (W == 1) {
+        if constexpr (sizeof(T) == 4) x[0] = *p;
+        else x[0] = bf16_to_f32(*p);
+    } else if constexpr (sizeof(T) == 4) {
+        const u32x4_any a = reinterpret_cast<const u32x4_any*>(p)[0], b = reinterpret_cast<const u32x4_any*>(p)[1];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) { x[j] = a[j]; x[4 + j] = b[j]; }
-}
-template <>
-__device__ __forceinline__ void load_w<bf16_t, 8>(const bf16_t* p, float (&x)[8]) {
-    const u32x4 a = *reinterpret_cast<const u32x4*>(p);
+        for (int j = 0; j < 4; ++j) { x[j] = __uint_as_float(a[j]); x[4 + j] = __uint_as_float(b[j]); }
+    } else {
+        const u32x4_any a = *reinterpret_cast<const u32x4_any*>(p);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) { x[2 * j] = __uint_as_float(a[j] << 16); x[2 * j + 1] = __uint_as_float(a[j] & 0xffff0000u); }
+        for (int j = 0; j < 4; ++j) { x[2 * j] = __uint_as_float(a[j] << 16); x[2 * j + 1] = __uint_as_float(a[j] & 0xffff0000u); }
+    }
 }
-template <>
-__device__ __forceinline__ void load_w<float, 1>(const float* p, float (&x)[1]) { x[0] = *p; }
-template <>
-__device__ __forceinline__ void load_w<bf16_t, 1>(const bf16_t* p, float (&x)[1]) { x[0] = bf16_to_f32(*p); }
-__device__ __forceinline__ void store_w(float* p, const float (&x)[8]) {
-    reinterpret_cast<f32x4*>(p)[0] = (f32x4){x[0], x[1], x[2], x[3]};
-    reinterpret_cast<f32x4*>(p)[1] = (f32x4){x[4], x[5], x[6], x[7]};
+template <typename T, int W>
+__device__ __forceinline__ void store_w(T* p, const float (&x)[W]) {
+    if constexpr (W == 1) {
+        if constexpr (sizeof(T) == 4) *p = x[0];
+        else *p = f32_to_bf16(x[0]);
+    } else if constexpr (sizeof(T) == 4) {
+        reinterpret_cast<u32x4_any*>(p)[0] = (u32x4_any){__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])};
+        reinterpret_cast<u32x4_any*>(p)[1] = (u32x4_any){__float_as_uint(x[4]), __float_as_uint(x[5]), __float_as_uint(x[6]), __float_as_uint(x[7])};
+    } else *reinterpret_cast<u32x4_any*>(p) = (u32x4_any){pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7])};
 }
-__device__ __forceinline__ void store_w(bf16_t* p, const float (&x)[8]) {
-    *reinterpret_cast<u32x4*>(p) = (u32x4){pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7])};
-}
-__device__ __forceinline__ void store_w(float* p, const float (&x)[1]) { *p = x[0]; }
-__device__ __forceinline__ void store_w(bf16_t* p, const float (&x)[1]) { *p = f32_to_bf16(x[0]); }
 
-// where a lane's C chunks of W pairs sit: lo[c] / hi[c] = the elements of the two halves, turn[c] = index of the first pair in the cos / sin row or -1 (not rotated), on[c] = in the head
-template <int W, int LPH, int C>
+// Where a lane's C chunks of W pairs sit: lo[c] / hi[c] = the elements of the two halves, turn[c] = index of the first pair in the cos / sin row or -1 (not rotated), on[c] = in the head.
+// The rotated pairs and the others are cut into chunks apart. SHIFT: a number of pairs that W does not divide; the last chunk starts earlier and computes skip[c] of its neighbour's pairs a
+// second time (the same bits), which then count in no sum.
+template <int W, int LPH, int C, bool SHIFT>
 struct Lane {
-    int lo[C], hi[C], turn[C];
+    int lo[C], hi[C], turn[C], skip[C];
     bool on[C];
     __device__ __forceinline__ Lane(int D, int R) {
-        const int l = threadIdx.x & (LPH - 1), rp = R >> 1, pairs = D >> 1;
+        const int l = threadIdx.x & (LPH - 1), rp = R >> 1, rest = (D - R) >> 1, nrot = (rp + W - 1) / W, nrest = (rest + W - 1) / W;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            const int j = (c * LPH + l) * W;
-            on[c] = j < pairs;
-            const int jj = on[c] ? j : 0;
-            const bool rot = jj < rp;
-            lo[c] = rot ? jj : R + (jj - rp);
-            hi[c] = rot ? jj + rp : R + (jj - rp) + ((D - R) >> 1);
-            turn[c] = rot ? jj : -1;
+            int i = c * LPH + l;
+            on[c] = i < nrot + nrest;
+            if (!on[c]) i = 0;
+            const bool rot = i < nrot;
+            const int j = (rot ? i : i - nrot) * W, pairs = rot ? rp : rest;
+            const int at = SHIFT && j > pairs - W ? pairs - W : j;
+            skip[c] = j - at;
+            lo[c] = rot ? at : R + at;
+            hi[c] = lo[c] + pairs;
+            turn[c] = rot ? at : -1;
         }
     }
+    // x where pair j of chunk c counts, 0 where it is a neighbour's
+    __device__ __forceinline__ float own(int c, int j, float x) const { return SHIFT && j < skip[c] ? 0.f : x; }
 };
 
 __device__ __forceinline__ float weight_at(const void* w, int dtype, int i) {
     return dtype == MTL_BF16 ? bf16_to_f32(reinterpret_cast<const bf16_t*>(w)[i]) : reinterpret_cast<const float*>(w)[i];
 }
-template <int W, int LPH, int C>
-__device__ __forceinline__ void load_weights(const void* w, int dtype, const Lane<W, LPH, C>& L, float (&lo)[C][W], float (&hi)[C][W]) {
+template <int W, int LPH, int C, bool S>
+__device__ __forceinline__ void load_weights(const void* w, int dtype, const Lane<W, LPH, C, S>& L, float (&lo)[C][W], float (&hi)[C][W]) {
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
@@ -93,8 +100,8 @@ __device__ __forceinline__ void load_weights(const void* w, int dtype, const Lan
 }
 
 // cos / sin of a row's pairs; a position outside the table turns every element of the row into NaN
-template <int W, int LPH, int C>
-__device__ __forceinline__ void load_turn(const mtl_qk_norm_rope_args& a, int64_t b, int64_t t, const Lane<W, LPH, C>& L, float (&cs)[C][W], float (&sn)[C][W]) {
+template <int W, int LPH, int C, bool S>
+__device__ __forceinline__ void load_turn(const mtl_qk_norm_rope_args& a, int64_t b, int64_t t, const Lane<W, LPH, C, S>& L, float (&cs)[C][W], float (&sn)[C][W]) {
     int64_t pos = a.pos0 + t;
     if (a.positions) pos = a.pos_i64 ? reinterpret_cast<const int64_t*>(a.positions)[b * a.pos_bs + t] : (int64_t)reinterpret_cast<const int32_t*>(a.positions)[b * a.pos_bs + t];
     const bool in = pos >= 0 && pos < a.n_pos;
@@ -117,10 +124,10 @@ __device__ __forceinline__ void load_turn(const mtl_qk_norm_rope_args& a, int64_
 }
 
 // heads [h0, h1) of one row: forward
-template <typename T, int W, int LPH, int C>
-__device__ __forceinline__ void heads_fwd(const T* x, T* y, int h0, int h1, int D, float eps, float inv_d, const Lane<W, LPH, C>& L, const float (&wl)[C][W], const float (&wh)[C][W],
+template <typename T, int W, int LPH, int C, bool S>
+__device__ __forceinline__ void heads_fwd(const T* x, T* y, int h0, int h1, int D, float eps, float inv_d, const Lane<W, LPH, C, S>& L, const float (&wl)[C][W], const float (&wh)[C][W],
                                           const float (&cs)[C][W], const float (&sn)[C][W]) {
-    constexpr int G = 64 / LPH, U = (W == 8 && C == 1) ? 2 : 1;      // heads per step of the wave, steps whose loads are in flight together
+    constexpr int G = 64 / LPH, U = W == 8 ? 2 : 1;      // heads per step of the wave, steps whose loads are in flight together
     const int g = (threadIdx.x & 63) / LPH;
     for (int h = h0; h < h1; h += G * U) {
         float lo[U][C][W], hi[U][C][W];
@@ -144,7 +151,7 @@ __device__ __forceinline__ void heads_fwd(const T* x, T* y, int h0, int h1, int 
 #pragma unroll
             for (int c = 0; c < C; ++c)
 #pragma unroll
-                for (int j = 0; j < W; ++j) ss += lo[u][c][j] * lo[u][c][j] + hi[u][c][j] * hi[u][c][j];
+                for (int j = 0; j < W; ++j) ss += L.own(c, j, lo[u][c][j]) * lo[u][c][j] + L.own(c, j, hi[u][c][j]) * hi[u][c][j];
             ss = group_sum<LPH>(ss);
             const float r = 1.0f / __builtin_sqrtf(ss * inv_d + eps);
 #pragma unroll
@@ -178,9 +185,9 @@ __device__ __forceinline__ Side side_of(const mtl_qk_norm_rope_args& a, bool key
     return s;
 }
 
-template <typename T, int W, int LPH, int C>
+template <typename T, int W, int LPH, int C, bool S>
 __global__ __launch_bounds__(WAVES * 64) void qk_norm_rope_fwd_kernel(const mtl_qk_norm_rope_args a, int hq_per, int hk_per) {
-    const Lane<W, LPH, C> L((int)a.D, (int)a.R);
+    const Lane<W, LPH, C, S> L((int)a.D, (int)a.R);
     const int64_t rows = a.B * a.T;
     const float inv_d = 1.0f / (float)a.D;
     const Side s = side_of(a, blockIdx.y == 1);
@@ -193,13 +200,13 @@ __global__ __launch_bounds__(WAVES * 64) void qk_norm_rope_fwd_kernel(const mtl_
         const int64_t b = row / a.T, t = row - b * a.T;
         float cs[C][W], sn[C][W];
         load_turn(a, b, t, L, cs, sn);
-        heads_fwd<T, W, LPH, C>((const T*)s.x + b * s.x_bs + t * s.x_ts, (T*)s.y + b * s.y_bs + t * s.y_ts, h0, h1, (int)a.D, a.eps, inv_d, L, wl, wh, cs, sn);
+        heads_fwd<T, W, LPH, C, S>((const T*)s.x + b * s.x_bs + t * s.x_ts, (T*)s.y + b * s.y_bs + t * s.y_ts, h0, h1, (int)a.D, a.eps, inv_d, L, wl, wh, cs, sn);
     }
 }
 
 // all heads of one row: backward; gl / gh accumulate dw
-template <typename T, int W, int LPH, int C, bool DW>
-__device__ __forceinline__ void heads_bwd(const T* x, const T* dy, T* dx, int h1, int D, float eps, float inv_d, const Lane<W, LPH, C>& L, const float (&wl)[C][W],
+template <typename T, int W, int LPH, int C, bool S, bool DW>
+__device__ __forceinline__ void heads_bwd(const T* x, const T* dy, T* dx, int h1, int D, float eps, float inv_d, const Lane<W, LPH, C, S>& L, const float (&wl)[C][W],
                                           const float (&wh)[C][W], const float (&cs)[C][W], const float (&sn)[C][W], float (&gl)[C][W], float (&gh)[C][W]) {
     constexpr int G = 64 / LPH;
     const int g = (threadIdx.x & 63) / LPH;
@@ -226,8 +233,9 @@ __device__ __forceinline__ void heads_bwd(const T* x, const T* dy, T* dx, int h1
                 float ul, uh;
                 rope_pair(al[c][j], ah[c][j], cs[c][j], -sn[c][j], ul, uh);          // the inverse rotation
                 al[c][j] = ul; ah[c][j] = uh;
-                ss += lo[c][j] * lo[c][j] + hi[c][j] * hi[c][j];
-                sa += ul * wl[c][j] * lo[c][j] + uh * wh[c][j] * hi[c][j];
+                const float xl = L.own(c, j, lo[c][j]), xh = L.own(c, j, hi[c][j]);
+                ss += xl * lo[c][j] + xh * hi[c][j];
+                sa += ul * wl[c][j] * xl + uh * wh[c][j] * xh;
             }
         ss = group_sum<LPH>(ss);
         sa = group_sum<LPH>(sa);
@@ -251,9 +259,9 @@ __device__ __forceinline__ void heads_bwd(const T* x, const T* dy, T* dx, int h1
 }
 
 // part [2][gridDim.x][D] (DW): every workgroup's weight gradient, summed over its waves and lane groups in a fixed order
-template <typename T, int W, int LPH, int C, bool DW>
+template <typename T, int W, int LPH, int C, bool S, bool DW>
 __global__ __launch_bounds__(WAVES * 64) void qk_norm_rope_bwd_kernel(const mtl_qk_norm_rope_args a, float* __restrict__ part) {
-    const Lane<W, LPH, C> L((int)a.D, (int)a.R);
+    const Lane<W, LPH, C, S> L((int)a.D, (int)a.R);
     const int64_t rows = a.B * a.T;
     const float inv_d = 1.0f / (float)a.D;
     const Side s = side_of(a, blockIdx.y == 1);
@@ -267,7 +275,7 @@ __global__ __launch_bounds__(WAVES * 64) void qk_norm_rope_bwd_kernel(const mtl_
         const int64_t b = row / a.T, t = row - b * a.T;
         float cs[C][W], sn[C][W];
         load_turn(a, b, t, L, cs, sn);
-        heads_bwd<T, W, LPH, C, DW>((const T*)s.x + b * s.x_bs + t * s.x_ts, (const T*)s.dy + b * s.dy_bs + t * s.dy_ts, (T*)s.y + b * s.y_bs + t * s.y_ts, s.H, (int)a.D, a.eps, inv_d, L, wl, wh, cs, sn,
+        heads_bwd<T, W, LPH, C, S, DW>((const T*)s.x + b * s.x_bs + t * s.x_ts, (const T*)s.dy + b * s.dy_bs + t * s.dy_ts, (T*)s.y + b * s.y_bs + t * s.y_ts, s.H, (int)a.D, a.eps, inv_d, L, wl, wh, cs, sn,
                                     gl, gh);
     }
     if (!DW) return;
@@ -279,6 +287,7 @@ __global__ __launch_bounds__(WAVES * 64) void qk_norm_rope_bwd_kernel(const mtl_
         if (L.on[c])
 #pragma unroll
             for (int j = 0; j < W; ++j) {
+                if (S && j < L.skip[c]) continue;               // (its neighbour has it)
                 sums[slot * D + L.lo[c] + j] = gl[c][j];
                 sums[slot * D + L.hi[c] + j] = gh[c][j];
             }
@@ -315,7 +324,7 @@ __global__ __launch_bounds__(1024) void qk_norm_rope_dw_kernel(const float* __re
 inline unsigned fwd_blocks(int64_t rows) { const int64_t b = (rows + WAVES - 1) / WAVES; return (unsigned)(b < 2048 ? b : 2048); }
 inline unsigned bwd_blocks(int64_t rows) { const int64_t b = (rows + WAVES - 1) / WAVES; return (unsigned)(b < 768 ? b : 768); }
 
-template <typename T, int W, int LPH, int C>
+template <typename T, int W, int LPH, int C, bool S>
 int launch(const mtl_qk_norm_rope_args& a, bool bwd, hipStream_t st) {
     const int64_t rows = a.B * a.T;
     if (!bwd) {
@@ -326,45 +335,42 @@ int launch(const mtl_qk_norm_rope_args& a, bool bwd, hipStream_t st) {
         while (parts < steps && rows * parts < 4096) parts *= 2;
         if (parts > steps) parts = (int)steps;
         const int hq = (int)(((a.Hq + parts - 1) / parts + G - 1) / G * G), hk = (int)(((a.Hkv + parts - 1) / parts + G - 1) / G * G);
-        hipLaunchKernelGGL((qk_norm_rope_fwd_kernel<T, W, LPH, C>), dim3(fwd_blocks(rows), 2, parts), dim3(WAVES * 64), 0, st, a, hq, hk);
+        hipLaunchKernelGGL((qk_norm_rope_fwd_kernel<T, W, LPH, C, S>), dim3(fwd_blocks(rows), 2, parts), dim3(WAVES * 64), 0, st, a, hq, hk);
         MTL_CHECK_LAUNCH();
         return MTL_OK;
     }
     const unsigned blocks = bwd_blocks(rows);
     float* part = reinterpret_cast<float*>(a.workspace);
     if (!a.dwq) {
-        hipLaunchKernelGGL((qk_norm_rope_bwd_kernel<T, W, LPH, C, false>), dim3(blocks, 2), dim3(WAVES * 64), 0, st, a, part);
+        hipLaunchKernelGGL((qk_norm_rope_bwd_kernel<T, W, LPH, C, S, false>), dim3(blocks, 2), dim3(WAVES * 64), 0, st, a, part);
         MTL_CHECK_LAUNCH();
         return MTL_OK;
     }
-    hipLaunchKernelGGL((qk_norm_rope_bwd_kernel<T, W, LPH, C, true>), dim3(blocks, 2), dim3(WAVES * 64), 0, st, a, part);
+    hipLaunchKernelGGL((qk_norm_rope_bwd_kernel<T, W, LPH, C, S, true>), dim3(blocks, 2), dim3(WAVES * 64), 0, st, a, part);
     MTL_CHECK_LAUNCH();
     hipLaunchKernelGGL(qk_norm_rope_dw_kernel, dim3((unsigned)((a.D + 63) / 64), 2), dim3(1024), 0, st, part, (int)blocks, (int)a.D, a.dwq, a.dwk);
     MTL_CHECK_LAUNCH();
     return MTL_OK;
 }
 
-// 8 pairs per lane with 16-byte accesses where every row, head and half starts on a 16-byte border; else one pair per lane and chunk
-inline bool rows_fit(const void* p, int64_t bs, int64_t ts, int size) {
-    return ((uintptr_t)p & 15) == 0 && (bs * size) % 16 == 0 && (ts * size) % 16 == 0;
+// 8 pairs per lane where the rotated pairs and the others are at least 8 (or none); else one pair per lane and chunk
+template <typename T, bool S>
+int dispatch_wide(const mtl_qk_norm_rope_args& a, int chunks, bool bwd, hipStream_t st) {
+    if (chunks <= 4) return launch<T, 8, 4, 1, S>(a, bwd, st);
+    if (chunks <= 8) return launch<T, 8, 8, 1, S>(a, bwd, st);
+    if (chunks <= 16) return launch<T, 8, 16, 1, S>(a, bwd, st);
+    return launch<T, 8, 32, 1, S>(a, bwd, st);
 }
 
 template <typename T>
 int dispatch(const mtl_qk_norm_rope_args& a, bool bwd, hipStream_t st) {
-    const int s = (int)sizeof(T);
-    bool wide = (a.R / 2) % 8 == 0 && ((a.D - a.R) / 2) % 8 == 0 && rows_fit(a.q, a.q_bs, a.q_ts, s) && rows_fit(a.k, a.k_bs, a.k_ts, s) && rows_fit(a.q_out, a.qo_bs, a.qo_ts, s) &&
-                rows_fit(a.k_out, a.ko_bs, a.ko_ts, s) && (((uintptr_t)a.cos_t | (uintptr_t)a.sin_t) & 15) == 0;
-    if (bwd) wide = wide && rows_fit(a.dq_out, a.dqo_bs, a.dqo_ts, s) && rows_fit(a.dk_out, a.dko_bs, a.dko_ts, s);
-    const int pairs = (int)(a.D / 2);
-    if (wide) {
-        if (pairs <= 32) return launch<T, 8, 4, 1>(a, bwd, st);
-        if (pairs <= 64) return launch<T, 8, 8, 1>(a, bwd, st);
-        if (pairs <= 128) return launch<T, 8, 16, 1>(a, bwd, st);
-        return launch<T, 8, 32, 1>(a, bwd, st);
-    }
-    if (pairs <= 64) return launch<T, 1, 64, 1>(a, bwd, st);
-    if (pairs <= 128) return launch<T, 1, 64, 2>(a, bwd, st);
-    return launch<T, 1, 64, 4>(a, bwd, st);
+    const int rp = (int)(a.R / 2), rest = (int)((a.D - a.R) / 2), pairs = rp + rest;
+    const int chunks = (rp + 7) / 8 + (rest + 7) / 8;
+    if (rp >= 8 && (rest == 0 || rest >= 8) && chunks <= 32)
+        return rp % 8 == 0 && rest % 8 == 0 ? dispatch_wide<T, false>(a, chunks, bwd, st) : dispatch_wide<T, true>(a, chunks, bwd, st);
+    if (pairs <= 64) return launch<T, 1, 64, 1, false>(a, bwd, st);
+    if (pairs <= 128) return launch<T, 1, 64, 2, false>(a, bwd, st);
+    return launch<T, 1, 64, 4, false>(a, bwd, st);
 }
 
 int check_args(const mtl_qk_norm_rope_args* a, bool bwd) {

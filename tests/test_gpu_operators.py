@@ -220,7 +220,8 @@ QK = [  # B, T, Hq, Hkv, D, R, type, weights, positions
     (1, 1, 1, 1, 2, 2, F32, F32, None), (2, 3, 3, 1, 6, 4, F32, F32, "i64"), (1, 1, 32, 8, 128, 128, BF16, F32, "i32"), (4, 1, 12, 12, 64, 64, BF16, BF16, "i64"), (2, 17, 12, 4, 64, 32, BF16, F32, "pos0"),
     (3, 5, 5, 3, 80, 32, F32, F32, "row"), (2, 9, 7, 2, 96, 96, BF16, F32, None), (1, 33, 4, 4, 130, 64, F32, F32, "i64"), (1, 5, 3, 1, 256, 256, BF16, BF16, None), (2, 4, 2, 2, 512, 256, F32, F32, "i64"),
     (1, 3, 3, 2, 510, 2, BF16, F32, None), (3, 700, 32, 8, 128, 128, BF16, F32, None), (1, 2049, 9, 9, 32, 32, F32, F32, "i32"), (2, 3, 70, 1, 16, 16, F32, F32, None), (1, 4, 2, 2, 384, 384, BF16, F32, None),
-    (2, 1030, 2, 1, 66, 20, BF16, F32, "i64")]
+    (2, 1030, 2, 1, 66, 20, BF16, F32, "i64"), (2, 5, 3, 3, 100, 100, BF16, F32, "i64"), (1, 7, 2, 1, 156, 34, F32, F32, None), (3, 40, 6, 2, 250, 250, BF16, BF16, None), (1, 9, 2, 2, 510, 254, F32, F32, "i32"),
+    (2, 11, 5, 1, 18, 18, BF16, F32, None), (1, 130, 9, 3, 192, 64, BF16, F32, "pos0")]
 
 
 @pytest.mark.parametrize("fused", [True, False])
