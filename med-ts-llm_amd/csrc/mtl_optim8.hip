@@ -262,10 +262,15 @@ __device__ __forceinline__ void adam8_chunk(const mtl_adam8_tensor& t, int64_t b
         if (sh) {                                               // bf16 copy [n / cols, ld_shadow] of the updated weight
             const uint32_t cols = (uint32_t)t.cols;
             uint32_t row = (uint32_t)e0 / cols, col = (uint32_t)e0 - row * cols;
+            if (nv == 4 && col + 4 <= cols) {                   // one 8-byte store wherever the four sit in one row (2-byte aligned where cols is odd)
+                typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
+                *reinterpret_cast<u32x2_any*>(sh + (int64_t)row * t.ld_shadow + col) = (u32x2_any){pack_bf16x2(pp[i][0], pp[i][1]), pack_bf16x2(pp[i][2], pp[i][3])};
+            } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (e < nv) sh[(int64_t)row * t.ld_shadow + col] = f32_to_bf16(pp[i][e]);
-                if (++col == cols) { col = 0; ++row; }
+                for (int e = 0; e < 4; ++e) {
+                    if (e < nv) sh[(int64_t)row * t.ld_shadow + col] = f32_to_bf16(pp[i][e]);
+                    if (++col == cols) { col = 0; ++row; }
+                }
             }
         }
     }

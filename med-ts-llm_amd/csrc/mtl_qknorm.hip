@@ -321,7 +321,9 @@ __global__ __launch_bounds__(1024) void qk_norm_rope_dw_kernel(const float* __re
     }
 }
 
-inline unsigned fwd_blocks(int64_t rows) { const int64_t b = (rows + WAVES - 1) / WAVES; return (unsigned)(b < 2048 ? b : 2048); }
+// Workgroups per side; more rows are walked by the same ones. Forward 1024 / 2048: 30.1 / 32.0 us at 6656 x (32 + 8) heads of 128 in bf16, equal at 8224 x 64. Backward 512 / 768 / 1536: 102 / 90 / 96 us at
+// 8224 x 64 heads, 50 / 51 / 57 at 6656 x 40 (three of its workgroups fit a CU). Two of a wave's head steps in flight in the forward: 50 us, one 57, four 55.
+inline unsigned fwd_blocks(int64_t rows) { const int64_t b = (rows + WAVES - 1) / WAVES; return (unsigned)(b < 1024 ? b : 1024); }
 inline unsigned bwd_blocks(int64_t rows) { const int64_t b = (rows + WAVES - 1) / WAVES; return (unsigned)(b < 768 ? b : 768); }
 
 template <typename T, int W, int LPH, int C, bool S>

@@ -142,6 +142,39 @@ def test_embedding_gradient_layouts(ops):
     assert not got[ids[0, 5]] and int((~got).sum()) == 1
 
 
+@pytest.mark.parametrize("N", [1, 5000, 20000])
+def test_embedding_without_a_token_that_counts(ops, N):
+    """every token is padding or outside the table: zeros, or what was there with accumulate"""
+    g = gen(N)
+    ids = torch.where(torch.rand(N, generator=g, device="cuda") < 0.5, 7, -1)
+    x = randn(g, N, 33)
+    assert not ops.embedding_bwd(x, ids, 20, padding_idx=7).any()
+    base = randn(g, 20, 33)
+    assert torch.equal(ops.embedding_bwd(x, ids, 20, padding_idx=7, out=base.clone(), accumulate=True), base)
+
+
+def test_calls_on_two_streams_at_once(ops):
+    """gradients of two streams in flight together, each with its own workspace"""
+    g = gen(21)
+    cos, sin = turn_tables(512, 64)
+    w = 1 + randn(g, 64, std=0.1)
+    data = [(torch.randint(0, 400, (20000,), generator=g, device="cuda"), randn(g, 20000, 96), randn(g, 2, 512, 512), randn(g, 2, 512, 128), randn(g, 2, 512, 512), randn(g, 2, 512, 128)) for _ in range(2)]
+
+    def work(ids, x, q, k, dq, dk):
+        return [ops.embedding_bwd(x, ids, 400), ops.embedding_bwd(x[:3000], ids[:3000], 400), *ops.qk_norm_rope_bwd(dq, dk, q, k, w, w, cos, sin, 8, 2, 64)]
+
+    want = [work(*d) for d in data]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in data]
+    for _ in range(3):
+        got = []
+        for st, d in zip(streams, data):
+            with torch.cuda.stream(st):
+                got.append(work(*d))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for x, y in zip(got, want) for a, b in zip(x, y))
+
+
 def test_embedding_offsets_beyond_32_bits(ops):
     """table, output and gradient of more than 2^31 elements (4.6 GB each in bf16): rows at both ends, looked up, summed and zeroed"""
     V, d, N = 140000, 16384, 140001
