@@ -420,7 +420,8 @@ def _req_gpu(*tensors):
 
 def _rows(x, d):
     """[..., d] as rows of unit inner stride (a copy where strides do not allow it, e.g. the expanded gradient of a sum)"""
-    x = x.reshape(-1, d)
+    if x.dim() != 2:
+        x = x.reshape(-1, d)
     n, (rs, cs) = x.shape[0], x.stride()
     return x if (d == 1 or cs == 1) and (n <= 1 or rs >= d) else x.contiguous()
 
@@ -982,25 +983,48 @@ class AssembleFn(torch.autograd.Function):
         return assemble_bwd(dh0, ctx.n_tok, ctx.drop), None, None, None, None, None, None
 
 
+def _embedding_grad(ctx, dout):
+    (ids,) = ctx.saved_tensors
+    V, scale, padding_idx, dtype = ctx.meta
+    return None, embedding_bwd(dout, ids, V, scale, padding_idx, None, False, dtype) if ctx.needs_input_grad[1] else None, None, None, None
+
+
 class EmbeddingFn(torch.autograd.Function):
     """scale * table[ids] with a trainable table (the frozen gather of a prompt is AssembleFn): forward embedding_fwd, backward embedding_bwd in the table's type.
     Tokens of padding_idx and ids outside [0, V) give no gradient."""
 
     @staticmethod
     def forward(ctx, ids, table, scale=1.0, padding_idx=None, out_dtype=None):
-        _req(padding_idx is None or 0 <= padding_idx < table.shape[0], "EmbeddingFn: padding_idx outside [0, V)")
+        if padding_idx is not None and not 0 <= padding_idx < table.shape[0]:
+            raise ValueError("EmbeddingFn: padding_idx outside [0, V)")
         out = embedding_fwd(ids, table, scale, out_dtype)
         ctx.save_for_backward(ids)
-        ctx.meta = (table.shape[0], float(scale), padding_idx, table.dtype)
+        ctx.meta = (table.shape[0], scale, padding_idx, table.dtype)
         return out
 
+    _once = staticmethod(torch.autograd.function.once_differentiable(_embedding_grad))
+
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        (ids,) = ctx.saved_tensors
-        V, scale, padding_idx, dtype = ctx.meta
-        grad = embedding_bwd(dout, ids, V, scale, padding_idx, out_dtype=dtype) if ctx.needs_input_grad[1] else None
-        return None, grad, None, None, None
+        # (once_differentiable's bookkeeping is needed under create_graph only, and costs as much as a launch)
+        return EmbeddingFn._once(ctx, dout) if torch.is_grad_enabled() else _embedding_grad(ctx, dout)
+
+
+def _qk_grad(ctx, dqo, dko):
+    keep, need, a = ctx.saved_tensors, ctx.needs_input_grad, ctx.args
+    q, k, wq, wk, cos, sin = keep[:6]
+    positions = keep[6] if len(keep) > 6 else None
+    # the forward's checked structure serves again as long as the saved tensors are where they were (a saved-tensor hook may have moved them)
+    if (a.q, a.k, a.wq, a.wk, a.cos_t, a.sin_t, a.positions) == (q.data_ptr(), k.data_ptr(), wq.data_ptr(), wk.data_ptr(), cos.data_ptr(), sin.data_ptr(), None if positions is None else positions.data_ptr()) \
+            and (a.q_bs, a.q_ts) == q.stride()[:2] and (a.k_bs, a.k_ts) == k.stride()[:2]:
+        a = N.QkNormRopeArgs.from_buffer_copy(a)
+    else:
+        Hq, Hkv, D, eps, pos0 = ctx.meta
+        a, keep = _qk_args(q, k, wq, wk, cos, sin, Hq, Hkv, D, eps, positions, pos0)
+    dq, dk, dwq, dwk = _qk_bwd(dqo, dko, a, keep, need[2] or need[3])
+    if dwq is not None and wq.dtype is not F32:
+        dwq, dwk = dwq.to(wq.dtype), dwk.to(wk.dtype)
+    return dq if need[0] else None, dk if need[1] else None, dwq if need[2] else None, dwk if need[3] else None, None, None, None, None, None, None, None, None
 
 
 class QkNormRopeFn(torch.autograd.Function):
@@ -1013,23 +1037,11 @@ class QkNormRopeFn(torch.autograd.Function):
         ctx.meta = (Hq, Hkv, D, eps, pos0)
         return qo, ko
 
+    _once = staticmethod(torch.autograd.function.once_differentiable(_qk_grad))
+
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dqo, dko):
-        keep, need, a = ctx.saved_tensors, ctx.needs_input_grad, ctx.args
-        q, k, wq, wk, cos, sin = keep[:6]
-        positions = keep[6] if len(keep) > 6 else None
-        # the forward's checked structure serves again as long as the saved tensors are where they were (a saved-tensor hook may have moved them)
-        if (a.q, a.k, a.wq, a.wk, a.cos_t, a.sin_t, a.positions) == (q.data_ptr(), k.data_ptr(), wq.data_ptr(), wk.data_ptr(), cos.data_ptr(), sin.data_ptr(), None if positions is None else positions.data_ptr()) \
-                and (a.q_bs, a.q_ts) == q.stride()[:2] and (a.k_bs, a.k_ts) == k.stride()[:2]:
-            a = N.QkNormRopeArgs.from_buffer_copy(a)
-        else:
-            Hq, Hkv, D, eps, pos0 = ctx.meta
-            a, keep = _qk_args(q, k, wq, wk, cos, sin, Hq, Hkv, D, eps, positions, pos0)
-        dq, dk, dwq, dwk = _qk_bwd(dqo, dko, a, keep, need[2] or need[3])
-        if dwq is not None and wq.dtype is not F32:
-            dwq, dwk = dwq.to(wq.dtype), dwk.to(wk.dtype)
-        return dq if need[0] else None, dk if need[1] else None, dwq if need[2] else None, dwk if need[3] else None, None, None, None, None, None, None, None, None
+        return QkNormRopeFn._once(ctx, dqo, dko) if torch.is_grad_enabled() else _qk_grad(ctx, dqo, dko)
 
 
 def dropout_f32(x, p, seed, out=None):

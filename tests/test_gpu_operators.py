@@ -353,6 +353,31 @@ def test_qk_norm_rope_function_against_differences(ops):
     assert torch.equal(partial[0], grads[2])
 
 
+def test_second_derivatives_are_refused(ops):
+    """the gradients are not differentiable again: under create_graph the first ones come out, a second pass through them raises"""
+    g = gen(22)
+    cos, sin = turn_tables(4, 8)
+    table, w = randn(g, 6, 8).requires_grad_(), torch.ones(8, device="cuda", requires_grad=True)
+    q = randn(g, 1, 4, 8).requires_grad_()
+    for y, leaf in ((ops.EmbeddingFn.apply(torch.arange(4, device="cuda"), table), table), (ops.QkNormRopeFn.apply(q, q, w, w, cos, sin, 1, 1, 8)[0], q)):
+        (first,) = torch.autograd.grad((y * y).sum(), leaf, create_graph=True)
+        assert first.shape == leaf.shape
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(first.sum(), leaf)
+
+
+def test_saved_tensor_hooks(ops):
+    """activations that a hook moves between forward and backward (here: cloned) give the same gradients"""
+    g = gen(23)
+    cos, sin = turn_tables(5, 16)
+    leaves = [randn(g, 2, 5, 64).requires_grad_(), randn(g, 2, 5, 32).requires_grad_(), (1 + randn(g, 16)).requires_grad_(), (1 + randn(g, 16)).requires_grad_()]
+    c = (randn(g, 2, 5, 64), randn(g, 2, 5, 32))
+    want = torch.autograd.grad(ops.QkNormRopeFn.apply(*leaves, cos, sin, 4, 2, 16), leaves, c)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(), lambda t: t.clone()):
+        y = ops.QkNormRopeFn.apply(*leaves, cos, sin, 4, 2, 16)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, leaves, c), want))
+
+
 # ================================================================================================ 8-bit Adam
 def np_of(t):
     return t.detach().float().cpu().numpy().reshape(-1)
