@@ -720,6 +720,13 @@ extern "C" int mtl_embedding_bwd(const void* ids, int ids_i64, int64_t N, const 
         MTL_CHECK_LAUNCH();
         return MTL_OK;
     }
+    // columns per lane: 16 bytes of dout, less where that would leave a good part of the wave without columns
+    int W = d > 64 ? 4 : 1;
+    if (dout_dtype == MTL_BF16 && d > 256 && (d + 511) / 512 * 512 <= d + d / 3) W = 8;
+    const int64_t chunks = chunks_of(d, W);
+    const int S = window_of(N, chunks);
+    const int64_t windows = (N + S - 1) / S;
+    if (chunks > 0x7fffffff || windows * chunks > (int64_t)0x7fffffff * 4) return MTL_ERR_UNSUPPORTED;      // (one grid)
     const Plan p = plan_for(N, V, d);
     uint32_t* list_n = reinterpret_cast<uint32_t*>(ws);
     uint32_t* sid = reinterpret_cast<uint32_t*>(ws + p.sid);
@@ -747,17 +754,11 @@ extern "C" int mtl_embedding_bwd(const void* ids, int ids_i64, int64_t N, const 
             kin = ko; pin = po;
         }
     }
-    // columns per lane: 16 bytes of dout, less where that would leave a good part of the wave without columns
-    int W = d > 64 ? 4 : 1;
-    if (dout_dtype == MTL_BF16 && d > 256 && (d + 511) / 512 * 512 <= d + d / 3) W = 8;
     SumArgs a;
     a.sid = sid; a.spos = spos; a.N = N; a.V = V; a.d = d; a.ld_dout = ld_dout; a.ld_grad = ld_grad; a.dout = dout; a.grad = grad;
     a.part = reinterpret_cast<float*>(ws + p.part); a.list = reinterpret_cast<uint32_t*>(ws + p.list); a.list_n = list_n;
     a.scale = scale; a.accumulate = accumulate ? 1 : 0;
-    a.chunks = (int)chunks_of(d, W);
-    a.S = window_of(N, a.chunks);
-    a.windows = (N + a.S - 1) / a.S;
-    if (a.windows * a.chunks > (int64_t)0x7fffffff * 4) return MTL_ERR_UNSUPPORTED;
+    a.chunks = (int)chunks; a.S = S; a.windows = windows;
     const bool d16 = dout_dtype == MTL_BF16, g16 = grad_dtype == MTL_BF16;
     if (d16 && g16) launch_sum<bf16_t, bf16_t>(a, W, st);
     else if (d16) launch_sum<bf16_t, float>(a, W, st);

@@ -475,19 +475,24 @@ def embedding_bwd(dout, ids, V, scale=1.0, padding_idx=None, out=None, accumulat
         ld, out_dtype = _table_ld(out, "out"), out.dtype
     flat, rows = _ids(ids), _rows(dout, d)
     n = rows.shape[0]
+    ld_rows = rows.stride(0) if n > 1 else d
     if out is not None and n:
         a0, b0 = out.data_ptr(), rows.data_ptr()
-        a1, b1 = a0 + ((V - 1) * ld + d) * out.element_size(), b0 + ((n - 1) * rows.stride(0) + d) * rows.element_size()
+        a1, b1 = a0 + ((V - 1) * ld + d) * out.element_size(), b0 + ((n - 1) * ld_rows + d) * rows.element_size()
         if a0 < b1 and b0 < a1:
             raise ValueError("embedding_bwd: out and dout share memory")
     _req_gpu(rows, flat, *(() if out is None else (out,)))
+    return _embedding_bwd(rows, ld_rows, flat, n, V, d, scale, padding_idx, out, ld, accumulate, out_dtype)
+
+
+def _embedding_bwd(rows, ld_rows, flat, n, V, d, scale, padding_idx, out, ld, accumulate, out_dtype):
     with N.on_device(rows):
         if out is None:
             out = rows.new_empty((V, d), dtype=out_dtype)
         nbytes = lib().mtl_embedding_bwd_workspace_bytes(n, V, d)
         ws = rows.new_empty(nbytes, dtype=torch.uint8)
-        check(lib().mtl_embedding_bwd(flat.data_ptr(), _ID_TYPES[flat.dtype], n, rows.data_ptr(), _TYPES[rows.dtype], rows.stride(0) if n > 1 else d, V, d, -1 if padding_idx is None else padding_idx,
-                                      scale, out.data_ptr(), _TYPES[out_dtype], ld, 1 if accumulate else 0, ws.data_ptr(), nbytes, stream()), "mtl_embedding_bwd")
+        check(lib().mtl_embedding_bwd(flat.data_ptr(), _ID_TYPES[flat.dtype], n, rows.data_ptr(), _TYPES[rows.dtype], ld_rows, V, d, -1 if padding_idx is None else padding_idx, scale, out.data_ptr(),
+                                      _TYPES[out_dtype], ld, 1 if accumulate else 0, ws.data_ptr(), nbytes, stream()), "mtl_embedding_bwd")
     return out
 
 
@@ -569,7 +574,7 @@ def _new(t):
 def qk_norm_rope_fwd(q, k, wq, wk, cos, sin, Hq, Hkv, D, eps=1e-6, positions=None, pos0=0, out=None):
     """rotate(w * x / rms(x)) for every head of q [B, T, Hq * D] and k [B, T, Hkv * D] (f32 or bf16; strided views, e.g. of a fused qkv buffer). cos / sin f32 [positions, R] as
     rope_inplace takes them (R <= D: the first R elements of a head are rotated). positions [B, T] or [T]: the rows' positions (a row whose position is not in the table comes out
-    as NaN), default pos0 + 0 .. T - 1. out = (q', k'): write there; the inputs themselves for in place."""
+    as NaN, and makes the weights' gradients NaN: give the rows behind a sequence any position of the table), default pos0 + 0 .. T - 1. out = (q', k'): write there; the inputs themselves for in place."""
     return _qk_fwd(q, k, wq, wk, cos, sin, Hq, Hkv, D, eps, positions, pos0, out)[:2]
 
 
@@ -591,11 +596,6 @@ def qk_norm_rope_bwd(dq_out, dk_out, q, k, wq, wk, cos, sin, Hq, Hkv, D, eps=1e-
     """(dq, dk, dwq, dwk) from the gradients of qk_norm_rope_fwd's outputs and its inputs (the norms are recomputed). dq / dk in the inputs' type (out = (dq, dk): written there,
     e.g. column ranges of one d(qkv) buffer, or over dq_out / dk_out themselves), dwq / dwk f32 [D] or None (want_dw False)."""
     a, keep = _qk_args(q, k, wq, wk, cos, sin, Hq, Hkv, D, eps, positions, pos0)
-    return _qk_bwd(dq_out, dk_out, a, keep, want_dw, out)
-
-
-def _qk_bwd(dq_out, dk_out, a, keep, want_dw, out=None):
-    q, k, wq, wk = keep[:4]
     if dq_out.shape != q.shape or dk_out.shape != k.shape or not dq_out.dtype is q.dtype is dk_out.dtype:
         raise ValueError("qk_norm_rope_bwd: gradients of the outputs' shapes and type")
     if dq_out.stride(2) != 1 or dk_out.stride(2) != 1:
@@ -605,6 +605,11 @@ def _qk_bwd(dq_out, dk_out, a, keep, want_dw, out=None):
         _req(all(o.untyped_storage().data_ptr() not in ins for o in out), "qk_norm_rope_bwd: out must not share memory with q or k")
         _check_qk_outputs(dq_out, dk_out, out)
     _req_gpu(*keep, dq_out, dk_out, *(out or ()))
+    return _qk_bwd(dq_out, dk_out, a, keep, want_dw, out)
+
+
+def _qk_bwd(dq_out, dk_out, a, keep, want_dw, out=None):
+    q, k, wq, wk = keep[:4]
     with N.on_device(q):
         dq, dk = out if out is not None else (_new(q), _new(k))
         a.q_out, a.k_out, a.dq_out, a.dk_out = dq.data_ptr(), dk.data_ptr(), dq_out.data_ptr(), dk_out.data_ptr()
@@ -984,9 +989,12 @@ class AssembleFn(torch.autograd.Function):
 
 
 def _embedding_grad(ctx, dout):
+    if not ctx.needs_input_grad[1]:
+        return None, None, None, None, None
     (ids,) = ctx.saved_tensors
-    V, scale, padding_idx, dtype = ctx.meta
-    return None, embedding_bwd(dout, ids, V, scale, padding_idx, None, False, dtype) if ctx.needs_input_grad[1] else None, None, None, None
+    V, d, scale, padding_idx, dtype = ctx.meta
+    flat, dout = _ids(ids), dout.contiguous()            # (autograd has seen to dout's shape, type and device)
+    return None, _embedding_bwd(dout, d, flat, flat.numel(), V, d, scale, padding_idx, None, d, False, dtype), None, None, None
 
 
 class EmbeddingFn(torch.autograd.Function):
@@ -999,7 +1007,7 @@ class EmbeddingFn(torch.autograd.Function):
             raise ValueError("EmbeddingFn: padding_idx outside [0, V)")
         out = embedding_fwd(ids, table, scale, out_dtype)
         ctx.save_for_backward(ids)
-        ctx.meta = (table.shape[0], scale, padding_idx, table.dtype)
+        ctx.meta = (*table.shape, scale, padding_idx, table.dtype)
         return out
 
     _once = staticmethod(torch.autograd.function.once_differentiable(_embedding_grad))
@@ -1021,6 +1029,8 @@ def _qk_grad(ctx, dqo, dko):
     else:
         Hq, Hkv, D, eps, pos0 = ctx.meta
         a, keep = _qk_args(q, k, wq, wk, cos, sin, Hq, Hkv, D, eps, positions, pos0)
+    if dqo.stride(2) != 1 or dko.stride(2) != 1:                # (autograd has seen to the gradients' shapes, types and devices)
+        dqo, dko = dqo.contiguous(), dko.contiguous()
     dq, dk, dwq, dwk = _qk_bwd(dqo, dko, a, keep, need[2] or need[3])
     if dwq is not None and wq.dtype is not F32:
         dwq, dwk = dwq.to(wq.dtype), dwk.to(wk.dtype)

@@ -499,6 +499,22 @@ def test_hip_adam_changes_width_on_load(optim):
         within(back.moments()[q][0], m + (gr - m) * 0.1, 1e-6 * (m.abs() + gr.abs()))
 
 
+def test_hip_adam_with_8_bit_state_on_a_side_stream(optim):
+    """HipAdam.defer with 8-bit state: the deferred parameters' updates run on the side stream and are the same bits"""
+    from med_ts_llm_amd.hip.optim import HipAdam
+    g = gen(31)
+    a = [randn(g, 300, 500).requires_grad_(), randn(g, 70, 11).requires_grad_()]
+    b = [p.detach().clone().requires_grad_() for p in a]
+    late = HipAdam(b, lr=1e-2, state_bits=8)
+    late.defer(b[:1])
+    _run({"lr": 1e-2, "state_bits": 8}, 4, 60, a)
+    for t in range(4):
+        _run(None, 1, 60 + t, b, late)
+        late.wait_deferred()
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
 def test_adam8_refuses_capture_and_large_tensor_indexing(optim):
     """a captured HipAdam step is refused; in a tensor of more than 2^31 elements the ones behind 2^31 get their own thresholds and codes (checked on the last blocks)"""
     from med_ts_llm_amd.hip import _native as N
