@@ -130,6 +130,18 @@ def test_embedding_gradient_layouts(ops):
         within(buf[:50, lo:hi], ref, (n + 2) * U * mag + U * ref.abs())
         buf[:50, lo:hi] = 9.0
         assert bool((buf == 9.0).all())
+    for lo, hi in ((0, 33), (1, 34), (3, 80)):                    # bf16 rows 162 bytes apart: 2-byte aligned
+        x16 = randn(g, 3, 41, hi - lo, dtype=BF16)
+        ref, mag, n = embed_ref(x16, ids, 50, 0.5, 3)
+        buf = torch.full((51, 81), 9.0, dtype=BF16, device="cuda")
+        ops.embedding_bwd(x16, ids, 50, scale=0.5, padding_idx=3, out=buf[:50, lo:hi])
+        within(buf[:50, lo:hi], ref, (n + 2) * U * mag + HALF[BF16] * (ref.abs() + (n + 2) * U * mag))
+        old = buf[:50, lo:hi].clone()
+        ops.embedding_bwd(x16, ids, 50, scale=0.5, padding_idx=3, out=buf[:50, lo:hi], accumulate=True)
+        twice = old.double() + ref
+        within(buf[:50, lo:hi], twice, (n + 3) * U * (mag + old.double().abs()) + HALF[BF16] * (twice.abs() + (n + 3) * U * (mag + old.double().abs())))
+        buf[:50, lo:hi] = 9.0
+        assert bool((buf == 9.0).all())
     table = randn(g, 50, 16).requires_grad_()
     ops.EmbeddingFn.apply(ids, table, 2.0).sum().backward()
     assert torch.equal(table.grad, 2.0 * torch.bincount(ids.reshape(-1), minlength=50).float()[:, None].expand(50, 16))
@@ -330,6 +342,22 @@ def test_qk_norm_rope_positions_outside_the_table_and_masked_values(ops):
     e = ops.qk_norm_rope_bwd(q[:0], k[:0], q[:0], k[:0], w, w, cos, sin, 4, 2, 32)
     assert e[0].shape == (0, 3, 128) and not e[2].any() and not e[3].any()
     assert ops.qk_norm_rope_fwd(q[:, :0], k[:, :0], w, w, cos, sin, 4, 2, 32)[0].shape == (2, 0, 128)
+
+
+def test_qk_norm_rope_into_a_cache(ops):
+    """one token of every sequence at its own position: the keys go straight to their places in a cache, the rest of which stays as it is"""
+    g = gen(41)
+    B, Hq, Hkv, D, L = 5, 8, 2, 64, 37
+    cos, sin = turn_tables(L, D)
+    wq, wk = 1 + randn(g, D, std=0.1), 1 + randn(g, D, std=0.1)
+    q, k = randn(g, B, 1, Hq * D, dtype=BF16), randn(g, B, 1, Hkv * D, dtype=BF16)
+    cache = torch.full((B, L, 2, Hkv * D), 3.0, dtype=BF16, device="cuda")
+    yq, yk = ops.qk_norm_rope_fwd(q, k, wq, wk, cos, sin, Hq, Hkv, D, pos0=11)
+    oq = torch.empty_like(q)
+    ops.qk_norm_rope_fwd(q, k, wq, wk, cos, sin, Hq, Hkv, D, pos0=11, out=(oq, cache[:, 11:12, 0]))
+    assert torch.equal(oq, yq) and torch.equal(cache[:, 11:12, 0], yk)
+    cache[:, 11:12, 0] = 3.0
+    assert bool((cache == 3.0).all())
 
 
 def test_qk_norm_rope_function_against_differences(ops):
@@ -549,6 +577,25 @@ def test_adam8_refuses_capture_and_large_tensor_indexing(optim):
     assert np.array_equal(np_of(big[lo:]), torch.from_numpy(wp).to(BF16).float().numpy())
     assert np.array_equal(st.exp_avg[lo:].cpu().numpy(), wc[0]) and np.array_equal(st.exp_avg_sq[lo:].cpu().numpy(), wc[1])
     assert np.array_equal(st.exponents[lo // 64:].cpu().numpy().view(np.int8), wc[2])
+
+
+def test_adam8_step_captured(optim):
+    """the raw step in a graph repeats the step number it was captured with, on what the tensors hold at the replay"""
+    g = gen(51)
+    p, gr = randn(g, 5000), randn(g, 5000, std=1e-2)
+    st = optim.adam8_state(p)
+    ref, rst = p.clone(), optim.adam8_state(p)
+    optim.adam8_step([p.clone()], [gr], [optim.adam8_state(p)], 7, lr=1e-2)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        optim.adam8_step([p], [gr], [st], 7, lr=1e-2)
+    for i in range(4):
+        gr.copy_(randn(g, 5000, std=1e-2))
+        graph.replay()
+        optim.adam8_step([ref], [gr], [rst], 7, lr=1e-2)
+        torch.cuda.synchronize()
+        assert torch.equal(p, ref) and all(torch.equal(a, b) for a, b in zip(st, rst)), i
 
 
 # ================================================================================================ together
