@@ -113,7 +113,7 @@ __global__ __launch_bounds__(256) void embedding_fwd_narrow_kernel(const void* _
     }
 }
 
-// a wave owns ROWS consecutive tokens and walks their columns: ROWS loads are in flight per step (one row per wave is bound by the latency id -> row -> store). `split` > 1: few tokens,
+// a wave owns ROWS consecutive tokens and walks their columns: ROWS loads are in flight per step. `split` > 1: few tokens,
 // a row's columns are spread over that many waves.
 template <typename TT, typename OT, int W, int ROWS>
 __global__ __launch_bounds__(256) void embedding_fwd_kernel(const void* __restrict__ ids, int ids_i64, int64_t N, const TT* __restrict__ table, int64_t V, int64_t d, int64_t ld_table, float scale,
@@ -600,10 +600,12 @@ inline int passes_for(int64_t V) { return (bits_for(V) + 8) / 9; }
 inline int bits_per_pass(int64_t V) { const int p = passes_for(V); return (bits_for(V) + p - 1) / p; }
 inline int64_t up(int64_t x, int64_t a) { return (x + a - 1) / a * a; }
 
-// window length: enough (window, column chunk) waves to fill the chip, at most 64 tokens (a partial row per window border costs 2 / S of the rows read)
+// Window length: as long as about 2400 (window, column chunk) waves are left, at most 64 tokens; a longer window writes and joins fewer partial rows (2 / S of the rows read), a shorter one
+// shortens the chain of a wave. Gradient as a whole, windows of 8 / 16 / 32 / 64: 2000 x 768 bf16 18.3 / 19.7 / 22.6 / 28.9 us (8 taken); 8192 x 4096 fp32 67 / 63 / 60 / 64 (32);
+// 40 000 x 768 bf16 68 / 62 / 58 / 62 (32); 200 003 x 64 bf16 126 / 94 / 74 / 66 (64); 200 003 x 1024 bf16 199 / 160 / 145 / 141 (64).
 inline int window_of(int64_t N, int64_t chunks) {
     int s = 8;
-    while (s < 64 && N / (2 * s) * chunks >= 8192) s *= 2;
+    while (s < 64 && N / (2 * s) * chunks >= 2400) s *= 2;
     return s;
 }
 inline int64_t chunks_of(int64_t d, int W) { return (d + 64 * W - 1) / (64 * W); }
@@ -620,9 +622,9 @@ inline Plan plan_for(int64_t N, int64_t V, int64_t d) {
     p.sid2 = small ? 0 : take(4 * N); p.spos2 = small ? 0 : take(4 * N);
     p.hist = small ? 0 : take(4 * tiles * MAX_BINS);
     p.list = take(4 * windows);
-    // partials: the window length depends on the columns per wave (64, 256 or 512): the longest list of the three
+    // partials: the window length depends on the columns per wave (64 or 256): the longer list of the two
     int64_t most = 0;
-    for (int W : {1, 4, 8}) { const int64_t s = window_of(N, chunks_of(d, W)); const int64_t w = (N + s - 1) / s; most = w > most ? w : most; }
+    for (int W : {1, 4}) { const int64_t s = window_of(N, chunks_of(d, W)); const int64_t w = (N + s - 1) / s; most = w > most ? w : most; }
     p.part = take(8 * most * d);
     p.total = at;
     return p;
@@ -639,9 +641,7 @@ void launch_sort_small(const void* ids, int ids_i64, int N, int64_t V, int64_t p
 template <typename DT, typename GT>
 void launch_sum(const SumArgs& a, int W, hipStream_t st) {
     const unsigned blocks = (unsigned)((a.windows * a.chunks + 3) / 4);
-    constexpr int WIDE = 16 / sizeof(DT);                          // 16 bytes of dout per lane
-    if (W == 8 && WIDE == 8) hipLaunchKernelGGL((embedding_sum_kernel<DT, GT, WIDE>), dim3(blocks), dim3(256), 0, st, a);
-    else if (W == 4) hipLaunchKernelGGL((embedding_sum_kernel<DT, GT, 4>), dim3(blocks), dim3(256), 0, st, a);
+    if (W == 4) hipLaunchKernelGGL((embedding_sum_kernel<DT, GT, 4>), dim3(blocks), dim3(256), 0, st, a);
     else hipLaunchKernelGGL((embedding_sum_kernel<DT, GT, 1>), dim3(blocks), dim3(256), 0, st, a);
 }
 
@@ -655,13 +655,15 @@ void launch_fwd_w(const void* ids, int ids_i64, int64_t N, const void* table, in
                            ld_out, lpr);
         return;
     }
-    if (N >= 4 * 4096) {       // enough tokens that four per wave still fill the chip
-        const int64_t waves = (N + 3) / 4;
-        hipLaunchKernelGGL((embedding_fwd_kernel<TT, OT, W, 4>), dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, st, ids, ids_i64, N, (const TT*)table, V, d, ld_table, scale, (OT*)out, ld_out, 1);
+    if (N >= 131072) {
+        // two tokens per wave: 200 003 x 1024 bf16 119.6 us, with one 128.2, with four 121.0; 65 536 x 1024 fp32 84.6 against 82.6 with one, 8192 x 4096 fp32 51 against 42
+        const int64_t waves = (N + 1) / 2;
+        hipLaunchKernelGGL((embedding_fwd_kernel<TT, OT, W, 2>), dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, st, ids, ids_i64, N, (const TT*)table, V, d, ld_table, scale, (OT*)out, ld_out, 1);
         return;
     }
+    // few tokens: a row's columns go to several waves, up to 8192 in all. 133 x 768 fp32 2.4 us (one wave per row 2.8), 1000 x 4096 5.8 (9.3); up to 16384 waves: 6.4, and 4096 x 768 5.7 against 5.0
     int64_t split = (d + 64 * W - 1) / (64 * W);
-    while (split > 1 && N * split > 16384) split = (split + 1) / 2;
+    while (split > 1 && N * split > 8192) split = (split + 1) / 2;
     hipLaunchKernelGGL((embedding_fwd_kernel<TT, OT, W, 1>), dim3((unsigned)((N * split + 3) / 4)), dim3(256), 0, st, ids, ids_i64, N, (const TT*)table, V, d, ld_table, scale, (OT*)out, ld_out, (int)split);
 }
 template <typename TT, typename OT>
@@ -720,9 +722,9 @@ extern "C" int mtl_embedding_bwd(const void* ids, int ids_i64, int64_t N, const 
         MTL_CHECK_LAUNCH();
         return MTL_OK;
     }
-    // columns per lane: 16 bytes of dout, less where that would leave a good part of the wave without columns
-    int W = d > 64 ? 4 : 1;
-    if (dout_dtype == MTL_BF16 && d > 256 && (d + 511) / 512 * 512 <= d + d / 3) W = 8;
+    // Four columns per lane; one where a row is narrower than a wave (200 003 x 64 bf16: 65.3 us, with four 67). Eight of bf16 (16 bytes) halve the waves in flight: 8192 x 2048 41.9 us against
+    // 38.5 with four, 200 003 x 1024 141.5 against 139.9.
+    const int W = d > 64 ? 4 : 1;
     const int64_t chunks = chunks_of(d, W);
     const int S = window_of(N, chunks);
     const int64_t windows = (N + S - 1) / S;
