@@ -32,7 +32,8 @@ __device__ __forceinline__ float group_sum(float v) {
 
 // vectors at any element's address (global accesses need no more alignment than their elements have)
 typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
-template <typename T, int W>
+// NT: the data pass the cache by (vectors of bf16 only)
+template <typename T, int W, bool NT = false>
 __device__ __forceinline__ void load_w(const T* p, float (&x)[W]) {
     if constexpr (W == 1) {
         if constexpr (sizeof(T) == 4) x[0] = *p;
@@ -42,7 +43,9 @@ __device__ __forceinline__ void load_w(const T* p, float (&x)[W]) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) { x[j] = __uint_as_float(a[j]); x[4 + j] = __uint_as_float(b[j]); }
     } else {
-        const u32x4_any a = *reinterpret_cast<const u32x4_any*>(p);
+        u32x4_any a;
+        if constexpr (NT) a = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(p));
+        else a = *reinterpret_cast<const u32x4_any*>(p);
 #pragma unroll
         for (int j = 0; j < 4; ++j) { x[2 * j] = __uint_as_float(a[j] << 16); x[2 * j + 1] = __uint_as_float(a[j] & 0xffff0000u); }
     }
@@ -124,7 +127,7 @@ __device__ __forceinline__ void load_turn(const mtl_qk_norm_rope_args& a, int64_
 }
 
 // heads [h0, h1) of one row: forward
-template <typename T, int W, int LPH, int C, bool S>
+template <typename T, int W, int LPH, int C, bool S, bool NT>
 __device__ __forceinline__ void heads_fwd(const T* x, T* y, int h0, int h1, int D, float eps, float inv_d, const Lane<W, LPH, C, S>& L, const float (&wl)[C][W], const float (&wh)[C][W],
                                           const float (&cs)[C][W], const float (&sn)[C][W]) {
     constexpr int G = 64 / LPH, U = W == 8 ? 2 : 1;      // heads per step of the wave, steps whose loads are in flight together
@@ -137,8 +140,8 @@ __device__ __forceinline__ void heads_fwd(const T* x, T* y, int h0, int h1, int 
             for (int c = 0; c < C; ++c) {
                 const int hh = h + u * G + g;
                 if (hh < h1 && L.on[c]) {
-                    load_w<T, W>(x + (int64_t)hh * D + L.lo[c], lo[u][c]);
-                    load_w<T, W>(x + (int64_t)hh * D + L.hi[c], hi[u][c]);
+                    load_w<T, W, NT>(x + (int64_t)hh * D + L.lo[c], lo[u][c]);
+                    load_w<T, W, NT>(x + (int64_t)hh * D + L.hi[c], hi[u][c]);
                 } else {
 #pragma unroll
                     for (int j = 0; j < W; ++j) lo[u][c][j] = hi[u][c][j] = 0.f;
@@ -185,7 +188,7 @@ __device__ __forceinline__ Side side_of(const mtl_qk_norm_rope_args& a, bool key
     return s;
 }
 
-template <typename T, int W, int LPH, int C, bool S>
+template <typename T, int W, int LPH, int C, bool S, bool NT>
 __global__ __launch_bounds__(WAVES * 64) void qk_norm_rope_fwd_kernel(const mtl_qk_norm_rope_args a, int hq_per, int hk_per) {
     const Lane<W, LPH, C, S> L((int)a.D, (int)a.R);
     const int64_t rows = a.B * a.T;
@@ -200,12 +203,12 @@ __global__ __launch_bounds__(WAVES * 64) void qk_norm_rope_fwd_kernel(const mtl_
         const int64_t b = row / a.T, t = row - b * a.T;
         float cs[C][W], sn[C][W];
         load_turn(a, b, t, L, cs, sn);
-        heads_fwd<T, W, LPH, C, S>((const T*)s.x + b * s.x_bs + t * s.x_ts, (T*)s.y + b * s.y_bs + t * s.y_ts, h0, h1, (int)a.D, a.eps, inv_d, L, wl, wh, cs, sn);
+        heads_fwd<T, W, LPH, C, S, NT>((const T*)s.x + b * s.x_bs + t * s.x_ts, (T*)s.y + b * s.y_bs + t * s.y_ts, h0, h1, (int)a.D, a.eps, inv_d, L, wl, wh, cs, sn);
     }
 }
 
 // all heads of one row: backward; gl / gh accumulate dw
-template <typename T, int W, int LPH, int C, bool S, bool DW>
+template <typename T, int W, int LPH, int C, bool S, bool NT, bool DW>
 __device__ __forceinline__ void heads_bwd(const T* x, const T* dy, T* dx, int h1, int D, float eps, float inv_d, const Lane<W, LPH, C, S>& L, const float (&wl)[C][W],
                                           const float (&wh)[C][W], const float (&cs)[C][W], const float (&sn)[C][W], float (&gl)[C][W], float (&gh)[C][W]) {
     constexpr int G = 64 / LPH;
@@ -216,10 +219,10 @@ __device__ __forceinline__ void heads_bwd(const T* x, const T* dy, T* dx, int h1
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             if (hh < h1 && L.on[c]) {
-                load_w<T, W>(x + (int64_t)hh * D + L.lo[c], lo[c]);
-                load_w<T, W>(x + (int64_t)hh * D + L.hi[c], hi[c]);
-                load_w<T, W>(dy + (int64_t)hh * D + L.lo[c], al[c]);
-                load_w<T, W>(dy + (int64_t)hh * D + L.hi[c], ah[c]);
+                load_w<T, W, NT>(x + (int64_t)hh * D + L.lo[c], lo[c]);
+                load_w<T, W, NT>(x + (int64_t)hh * D + L.hi[c], hi[c]);
+                load_w<T, W, NT>(dy + (int64_t)hh * D + L.lo[c], al[c]);
+                load_w<T, W, NT>(dy + (int64_t)hh * D + L.hi[c], ah[c]);
             } else {
 #pragma unroll
                 for (int j = 0; j < W; ++j) lo[c][j] = hi[c][j] = al[c][j] = ah[c][j] = 0.f;
@@ -259,7 +262,7 @@ __device__ __forceinline__ void heads_bwd(const T* x, const T* dy, T* dx, int h1
 }
 
 // part [2][gridDim.x][D] (DW): every workgroup's weight gradient, summed over its waves and lane groups in a fixed order
-template <typename T, int W, int LPH, int C, bool S, bool DW>
+template <typename T, int W, int LPH, int C, bool S, bool NT, bool DW>
 __global__ __launch_bounds__(WAVES * 64) void qk_norm_rope_bwd_kernel(const mtl_qk_norm_rope_args a, float* __restrict__ part) {
     const Lane<W, LPH, C, S> L((int)a.D, (int)a.R);
     const int64_t rows = a.B * a.T;
@@ -275,7 +278,7 @@ __global__ __launch_bounds__(WAVES * 64) void qk_norm_rope_bwd_kernel(const mtl_
         const int64_t b = row / a.T, t = row - b * a.T;
         float cs[C][W], sn[C][W];
         load_turn(a, b, t, L, cs, sn);
-        heads_bwd<T, W, LPH, C, S, DW>((const T*)s.x + b * s.x_bs + t * s.x_ts, (const T*)s.dy + b * s.dy_bs + t * s.dy_ts, (T*)s.y + b * s.y_bs + t * s.y_ts, s.H, (int)a.D, a.eps, inv_d, L, wl, wh, cs, sn,
+        heads_bwd<T, W, LPH, C, S, NT, DW>((const T*)s.x + b * s.x_bs + t * s.x_ts, (const T*)s.dy + b * s.dy_bs + t * s.dy_ts, (T*)s.y + b * s.y_bs + t * s.y_ts, s.H, (int)a.D, a.eps, inv_d, L, wl, wh, cs, sn,
                                     gl, gh);
     }
     if (!DW) return;
@@ -321,13 +324,14 @@ __global__ __launch_bounds__(1024) void qk_norm_rope_dw_kernel(const float* __re
     }
 }
 
-// Workgroups per side; more rows are walked by the same ones. Forward 1024 / 2048: 30.1 / 32.0 us at 6656 x (32 + 8) heads of 128 in bf16, equal at 8224 x 64. Backward 512 / 768 / 1536: 102 / 90 / 96 us at
-// 8224 x 64 heads, 50 / 51 / 57 at 6656 x 40 (three of its workgroups fit a CU). Two of a wave's head steps in flight in the forward: 50 us, one 57, four 55.
+// Workgroups per side; more rows are walked by the same ones. Forward 1024 / 2048: 29.2 / 30.8 us at 6656 x (32 + 8) heads of 128 in bf16, 14.2 / 16.4 at 8192 x 24 of 64, 57.6 / 55.8 at 8224 x 64 of 128.
+// Backward 512 / 768 / 1536: 102 / 90 / 96 us at 8224 x 64 heads, 50 / 51 / 57 at 6656 x 40 (three of its workgroups fit a CU). Two of a wave's head steps in flight in the forward: 50 us, one 57,
+// four 55.
 inline unsigned fwd_blocks(int64_t rows) { const int64_t b = (rows + WAVES - 1) / WAVES; return (unsigned)(b < 1024 ? b : 1024); }
 inline unsigned bwd_blocks(int64_t rows) { const int64_t b = (rows + WAVES - 1) / WAVES; return (unsigned)(b < 768 ? b : 768); }
 
-template <typename T, int W, int LPH, int C, bool S>
-int launch(const mtl_qk_norm_rope_args& a, bool bwd, hipStream_t st) {
+template <typename T, int W, int LPH, int C, bool S, bool NT>
+int launch_with(const mtl_qk_norm_rope_args& a, bool bwd, hipStream_t st) {
     const int64_t rows = a.B * a.T;
     if (!bwd) {
         // One wave per row and side; where that leaves the chip empty, a row's heads go to several waves (each a whole number of the wave's head groups), up to 512 in all. 32 + 8 heads of 128:
@@ -338,22 +342,34 @@ int launch(const mtl_qk_norm_rope_args& a, bool bwd, hipStream_t st) {
         while (parts < steps && rows * parts < 512) parts *= 2;
         if (parts > steps) parts = (int)steps;
         const int hq = (int)(((a.Hq + parts - 1) / parts + G - 1) / G * G), hk = (int)(((a.Hkv + parts - 1) / parts + G - 1) / G * G);
-        hipLaunchKernelGGL((qk_norm_rope_fwd_kernel<T, W, LPH, C, S>), dim3(fwd_blocks(rows), 2, parts), dim3(WAVES * 64), 0, st, a, hq, hk);
+        hipLaunchKernelGGL((qk_norm_rope_fwd_kernel<T, W, LPH, C, S, NT>), dim3(fwd_blocks(rows), 2, parts), dim3(WAVES * 64), 0, st, a, hq, hk);
         MTL_CHECK_LAUNCH();
         return MTL_OK;
     }
     const unsigned blocks = bwd_blocks(rows);
     float* part = reinterpret_cast<float*>(a.workspace);
     if (!a.dwq) {
-        hipLaunchKernelGGL((qk_norm_rope_bwd_kernel<T, W, LPH, C, S, false>), dim3(blocks, 2), dim3(WAVES * 64), 0, st, a, part);
+        hipLaunchKernelGGL((qk_norm_rope_bwd_kernel<T, W, LPH, C, S, NT, false>), dim3(blocks, 2), dim3(WAVES * 64), 0, st, a, part);
         MTL_CHECK_LAUNCH();
         return MTL_OK;
     }
-    hipLaunchKernelGGL((qk_norm_rope_bwd_kernel<T, W, LPH, C, S, true>), dim3(blocks, 2), dim3(WAVES * 64), 0, st, a, part);
+    hipLaunchKernelGGL((qk_norm_rope_bwd_kernel<T, W, LPH, C, S, NT, true>), dim3(blocks, 2), dim3(WAVES * 64), 0, st, a, part);
     MTL_CHECK_LAUNCH();
     hipLaunchKernelGGL(qk_norm_rope_dw_kernel, dim3((unsigned)((a.D + 63) / 64), 2), dim3(1024), 0, st, part, (int)blocks, (int)a.D, a.dwq, a.dwk);
     MTL_CHECK_LAUNCH();
     return MTL_OK;
+}
+
+// Queries and keys of 64 MiB and more (the backward reads dy's as much again) do not stay in the 256 MB cache behind what is written: their loads pass it by and leave it to the outputs, which are read
+// next. Without / with, us, bf16 heads of 128: forward 42 MB 18.6 / 21.4, 67 MB 27.8 / 27.5, 101 MB 43.4 / 40.1, 135 MB 57.6 / 49.2, 270 MB 109 / 106; backward 42 MB 35.4 / 35.7, 67 MB 48.9 / 45.4,
+// 101 MB 68.7 / 62.9, 135 MB 86.4 / 78.6, 270 MB 160 / 156. Between a projection and the attention: 67 MB 126 / 122, 135 MB 286 / 273. Only where every half of a head is whole lines of 128 bytes and a
+// load takes 16 of each lane's: a line that two loads share comes twice (heads of 64, 101 MB: forward 51 / 52, backward 77 / 81; of 100: 78 / 83, 112 / 115; fp32, 135 MB: no gain). Stores that pass the
+// cache by gain 6 % alone and lose more in the kernel that reads them.
+template <typename T, int W, int LPH, int C, bool S>
+int launch(const mtl_qk_norm_rope_args& a, bool bwd, hipStream_t st) {
+    if constexpr (W == 8 && LPH >= 8 && !S && sizeof(T) == 2)
+        if (a.R % 128 == 0 && (a.D - a.R) % 128 == 0 && a.B * a.T * (a.Hq + a.Hkv) * a.D * 2 >= (int64_t)64 << 20) return launch_with<T, W, LPH, C, S, true>(a, bwd, st);
+    return launch_with<T, W, LPH, C, S, false>(a, bwd, st);
 }
 
 // 8 pairs per lane where the rotated pairs and the others are at least 8 (or none); else one pair per lane and chunk

@@ -324,6 +324,14 @@ def test_qk_norm_rope(ops, B, T, Hq, Hkv, D, R, dt, wt, pos, fused):
         assert b.data_ptr() == k.data_ptr()
 
 
+@pytest.mark.parametrize("fused", [True, False])
+@pytest.mark.parametrize("B,T,Hq,Hkv,D,R,pos", [(3, 2785, 32, 8, 128, 128, "i64"), (1, 3001, 24, 24, 256, 256, None), (1, 9001, 3, 5, 512, 256, "pos0")])
+def test_qk_norm_rope_larger_than_the_cache(ops, B, T, Hq, Hkv, D, R, pos, fused):
+    """64 MiB and more of queries and keys, whose loads pass the cache by: heads in 8, 16 and 32 lanes, in place among them"""
+    assert B * T * (Hq + Hkv) * D * 2 >= 64 << 20
+    test_qk_norm_rope(ops, B, T, Hq, Hkv, D, R, BF16, F32, pos, fused)
+
+
 def test_qk_norm_rope_positions_outside_the_table_and_masked_values(ops):
     """a row whose position is not in the table is NaN, and only that row; a NaN or an infinity in a head stays in that head; empty batches"""
     g = gen(9)
