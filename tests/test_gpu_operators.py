@@ -187,6 +187,27 @@ def test_calls_on_two_streams_at_once(ops):
         assert all(torch.equal(a, b) for x, y in zip(got, want) for a, b in zip(x, y))
 
 
+@pytest.mark.parametrize("N", [0, 1, 100, 9000])
+@pytest.mark.parametrize("V,d,gt", [(137003, 1001, BF16), (66001, 1024, F32)])
+def test_embedding_gradient_larger_than_the_cache(ops, N, V, d, gt):
+    """256 MiB and more of rows, an odd end among them, written over other values: every row without a token is zero, the others hold the sum"""
+    assert V * d * gt.itemsize >= 256 << 20
+    g = gen(N + V)
+    ids = torch.randint(0, V, (N,), generator=g, device="cuda")
+    if N > 1:
+        ids[0], ids[-1] = V - 1, 0
+    dout = randn(g, N, d, dtype=gt)
+    store = torch.ones(V * d + 64, dtype=gt, device="cuda")
+    grad = ops.embedding_bwd(dout, ids, V, out=store[:V * d].view(V, d))
+    n = torch.bincount(ids, minlength=V)
+    at = n.nonzero()[:, 0]
+    row = torch.zeros(V, dtype=torch.int64, device="cuda").index_put_((at,), torch.arange(len(at), device="cuda"))[ids]
+    ref, mag = (torch.zeros(len(at), d, dtype=F64, device="cuda").index_add_(0, row, x) for x in (dout.double(), dout.double().abs()))
+    bound = (n[at][:, None] + 1) * U * mag
+    within(grad[at], ref, bound + HALF[gt] * (ref.abs() + bound))
+    assert int(torch.count_nonzero(grad[n == 0])) == 0 and bool((store[V * d:] == 1).all())
+
+
 def test_embedding_offsets_beyond_32_bits(ops):
     """table, output and gradient of more than 2^31 elements (4.6 GB each in bf16): rows at both ends, looked up, summed and zeroed"""
     V, d, N = 140000, 16384, 140001
