@@ -21,10 +21,11 @@ namespace {
 constexpr int MAX_T = MTL_ADAM8_MAX_TENSORS;
 constexpr int THREADS = 256;
 // 4 elements per lane and iteration; all loads of a workgroup's iterations are in flight before the first use. Iterations, measured at 512 M elements: fp32 step 1 / 2 / 4: 1351 / 1475 /
-// 1413 us (6.1 TB/s); bf16 step 1066 / 968 / 1046 (5.3 TB/s: half of the bytes per element, the arithmetic shows); read-back 594 / 502 / 541.
-constexpr int ITERS_F32 = 1, ITERS_B16 = 2, ITERS_STATE = 2;
+// 1413 us (6.1 TB/s); bf16 step 1066 / 968 / 1046 (5.3 TB/s: half of the bytes per element, the arithmetic shows). At 410 M elements, outputs not reused: read-back in fp32 659 / 689 / 737, in bf16
+// 465 / 389 / 422, packing 934 / 966 / -. What these have in common: a workgroup moves 4 KB in a row of each wide array.
+constexpr int ITERS_F32 = 1, ITERS_B16 = 2;
 constexpr int chunk_of(int iters) { return THREADS * 4 * iters; }      // elements per workgroup: a whole number of 64-element blocks
-inline int step_chunk(int64_t dtype) { return chunk_of(dtype == MTL_BF16 ? ITERS_B16 : ITERS_F32); }
+inline __host__ __device__ int dtype_chunk(int64_t dtype) { return chunk_of(dtype == MTL_BF16 ? ITERS_B16 : ITERS_F32); }
 
 struct Adam8Table {
     mtl_adam8_tensor t[MAX_T];
@@ -286,30 +287,29 @@ __global__ __launch_bounds__(THREADS) void adam8_step_kernel(const Adam8Table ta
     else adam8_chunk<false>(t, at * chunk_of(ITERS_F32), h);
 }
 
-__device__ __forceinline__ void store_moment(void* dst, int64_t e0, int nv, const float (&x)[4], bool b16) {
+template <bool NT, typename V>
+__device__ __forceinline__ void store_vec(V x, void* p) {
+    if constexpr (NT) __builtin_nontemporal_store(x, reinterpret_cast<V*>(p));
+    else *reinterpret_cast<V*>(p) = x;
+}
+template <bool B16, bool NT>
+__device__ __forceinline__ void store_moment(void* dst, int64_t e0, int nv, const float (&x)[4]) {
     if (!dst) return;
-    if (b16) {
+    if constexpr (B16) {
         bf16_t* d = reinterpret_cast<bf16_t*>(dst) + e0;
-        if (nv == 4 && ((uintptr_t)d & 7) == 0) {
-            *reinterpret_cast<u32x2*>(d) = (u32x2){pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
-            return;
-        }
+        if (nv == 4 && ((uintptr_t)d & 7) == 0) return store_vec<NT>((u32x2){pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])}, d);
         for (int e = 0; e < nv; ++e) d[e] = f32_to_bf16(x[e]);
     } else {
         float* d = reinterpret_cast<float*>(dst) + e0;
-        if (nv == 4 && ((uintptr_t)d & 15) == 0) { *reinterpret_cast<f32x4*>(d) = (f32x4){x[0], x[1], x[2], x[3]}; return; }
+        if (nv == 4 && ((uintptr_t)d & 15) == 0) return store_vec<NT>((f32x4){x[0], x[1], x[2], x[3]}, d);
         for (int e = 0; e < nv; ++e) d[e] = x[e];
     }
 }
 
-// read-back of the codes: 2 B read, 4 (bf16) or 8 B written per element
-__global__ __launch_bounds__(THREADS) void adam8_moments_kernel(const State8Table tab) {
-    int ti = 0;
-    const int b = blockIdx.x;
-    while (ti + 1 < tab.count && b >= tab.first_block[ti + 1]) ++ti;
-    const mtl_adam8_state t = tab.t[ti];
-    constexpr int ITERS = ITERS_STATE;
-    const int64_t base = (int64_t)(b - tab.first_block[ti]) * chunk_of(ITERS);
+template <bool B16, bool NT>
+__device__ __forceinline__ void moments_chunk(const mtl_adam8_state& t, int64_t at) {
+    constexpr int ITERS = B16 ? ITERS_B16 : ITERS_F32;
+    const int64_t base = at * chunk_of(ITERS);
     const bool vec8 = (((uintptr_t)t.m8 | (uintptr_t)t.r8) & 3) == 0;
     uint32_t cm[ITERS], cr[ITERS], ex[ITERS];
 #pragma unroll
@@ -332,9 +332,21 @@ __global__ __launch_bounds__(THREADS) void adam8_moments_kernel(const State8Tabl
         decode4(cm[i], cr[i], (int8_t)(ex[i] & 0xffu), (int8_t)(ex[i] >> 8), m, r);
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = r[e] * r[e];
-        store_moment(t.m, e0, nv, m, t.dtype == MTL_BF16);
-        store_moment(t.v, e0, nv, v, t.dtype == MTL_BF16);
+        store_moment<B16, NT>(t.m, e0, nv, m);
+        store_moment<B16, NT>(t.v, e0, nv, v);
     }
+}
+
+// read-back of the codes: 2 B read, 4 (bf16) or 8 B written per element. NT: the written moments pass the cache by; where a call writes 192 MiB and more they would not stay in it for their reader.
+// Without / with, us, alone and with a copy behind it: 76 M elements fp32 (612 MB) 128 / 107, 302 / 278; 59 M bf16 (235 MB) 60 / 50, 154 / 148; but 17 M fp32 (134 MB) 26.9 / 25.3, 57 / 63.
+template <bool NT>
+__global__ __launch_bounds__(THREADS) void adam8_moments_kernel(const State8Table tab) {
+    int ti = 0;
+    const int b = blockIdx.x;
+    while (ti + 1 < tab.count && b >= tab.first_block[ti + 1]) ++ti;
+    const mtl_adam8_state t = tab.t[ti];
+    if (t.dtype == MTL_BF16) moments_chunk<true, NT>(t, b - tab.first_block[ti]);
+    else moments_chunk<false, NT>(t, b - tab.first_block[ti]);
 }
 
 // packing of fp32 moments (taking over a run whose moments are held in 32 bits)
@@ -343,21 +355,27 @@ __global__ __launch_bounds__(THREADS) void adam8_quantize_kernel(const State8Tab
     const int b = blockIdx.x;
     while (ti + 1 < tab.count && b >= tab.first_block[ti + 1]) ++ti;
     const mtl_adam8_state t = tab.t[ti];
-    constexpr int ITERS = ITERS_STATE;
-    const int64_t base = (int64_t)(b - tab.first_block[ti]) * chunk_of(ITERS);
+    const int64_t base = (int64_t)(b - tab.first_block[ti]) * chunk_of(ITERS_F32);
     const bool vec8 = (((uintptr_t)t.m8 | (uintptr_t)t.r8) & 3) == 0;
     const float* ms = reinterpret_cast<const float*>(t.m);
     const float* vs = reinterpret_cast<const float*>(t.v);
+    const bool vec = (((uintptr_t)ms | (uintptr_t)vs) & 15) == 0;
 #pragma unroll
-    for (int i = 0; i < ITERS; ++i) {
+    for (int i = 0; i < ITERS_F32; ++i) {
         const int64_t e0 = base + ((int64_t)i * THREADS + threadIdx.x) * 4;
         const int64_t left = t.n - e0;
         const int nv = left >= 4 ? 4 : (left > 0 ? (int)left : 0);
         float m[4], v[4], r[4];
+        if (nv == 4 && vec) {
+            const f32x4 a = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(ms + e0)), b = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(vs + e0));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            m[e] = e < nv ? ms[e0 + e] : 0.f;
-            v[e] = e < nv ? vs[e0 + e] : 0.f;
+            for (int e = 0; e < 4; ++e) { m[e] = a[e]; v[e] = b[e]; }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                m[e] = e < nv ? ms[e0 + e] : 0.f;
+                v[e] = e < nv ? vs[e0 + e] : 0.f;
+            }
         }
         uint32_t nm, nr, nx;
         encode4(m, v, r, (uint32_t)e0, t_thr, nm, nr, nx);
@@ -386,7 +404,7 @@ int for_tables(const mtl_adam8_state* states, int count, bool read_back, Launch 
         int64_t blocks = 0;
         for (; i < count && tab.count < MAX_T; ++i) {
             if (states[i].n == 0) continue;
-            const int64_t nb = (states[i].n + chunk_of(ITERS_STATE) - 1) / chunk_of(ITERS_STATE);
+            const int64_t nb = (states[i].n + dtype_chunk(states[i].dtype) - 1) / dtype_chunk(states[i].dtype);
             if (nb > 0x7fffffff) return MTL_ERR_UNSUPPORTED;
             if (blocks + nb > 0x7fffffff) break;                // (this one goes into the next launch)
             tab.t[tab.count] = states[i];
@@ -429,7 +447,7 @@ extern "C" int mtl_adam8_step(const mtl_adam8_tensor* tensors, int count, double
         for (; i < count && tab.count < MAX_T; ++i) {
             const mtl_adam8_tensor& t = tensors[i];
             if (t.n == 0) continue;
-            const int64_t nb = (t.n + step_chunk(t.param_dtype) - 1) / step_chunk(t.param_dtype);
+            const int64_t nb = (t.n + dtype_chunk(t.param_dtype) - 1) / dtype_chunk(t.param_dtype);
             if (nb > 0x7fffffff) return MTL_ERR_UNSUPPORTED;
             if (blocks + nb > 0x7fffffff) break;
             tab.t[tab.count] = t;
@@ -448,7 +466,12 @@ extern "C" int mtl_adam8_step(const mtl_adam8_tensor* tensors, int count, double
 extern "C" int mtl_adam8_moments(const mtl_adam8_state* states, int count, void* stream) {
     if (count < 0 || (count > 0 && !states)) return MTL_ERR_ARG;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    return for_tables(states, count, true, [&](const State8Table& tab, unsigned blocks) { hipLaunchKernelGGL(adam8_moments_kernel, dim3(blocks), dim3(THREADS), 0, st, tab); });
+    return for_tables(states, count, true, [&](const State8Table& tab, unsigned blocks) {
+        int64_t bytes = 0;
+        for (int i = 0; i < tab.count; ++i) bytes += tab.t[i].n * (tab.t[i].dtype == MTL_BF16 ? 2 : 4) * ((tab.t[i].m != nullptr) + (tab.t[i].v != nullptr));
+        if (bytes >= (int64_t)192 << 20) hipLaunchKernelGGL(adam8_moments_kernel<true>, dim3(blocks), dim3(THREADS), 0, st, tab);
+        else hipLaunchKernelGGL(adam8_moments_kernel<false>, dim3(blocks), dim3(THREADS), 0, st, tab);
+    });
 }
 
 extern "C" int mtl_adam8_quantize(const mtl_adam8_state* states, int count, int64_t step, void* stream) {

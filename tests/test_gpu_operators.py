@@ -490,6 +490,27 @@ def test_adam8_moments_and_quantize(optim):
         assert torch.equal(a16.float(), a) and torch.equal(b16, b.to(BF16))
 
 
+def test_adam8_moments_larger_than_the_cache(optim):
+    """192 MiB and more written by one call, ends that fill no vector: the values that the codes stand for, from packed moments that start on and off a 16-byte boundary"""
+    g = gen(8)
+    ns = (50_000_003, 1, 700_002)
+    sts = []
+    for n, off in zip(ns, (1, 0, 0)):
+        m, v = randn(g, n + off) * 1e-3, randn(g, n + off).square() * 1e-6
+        sts.append(optim.adam8_quantize(m[off:], v[off:], 7))
+        if off:
+            again = optim.adam8_quantize(m[off:].clone(), v[off:].clone(), 7)
+            assert all(torch.equal(getattr(again, k), getattr(sts[0], k)) for k in ("exp_avg", "exp_avg_sq", "exponents"))
+            del again
+        del m, v
+    e4m3, root = (torch.from_numpy(x).cuda() for x in (A8.E4M3, A8.ROOT))
+    for dt in (F32, BF16):
+        for n, st, (a, b) in zip(ns, sts, optim.adam8_moments(sts, dt)):
+            ex = torch.exp2(st.exponents.view(torch.int8).view(-1, 2).float()).repeat_interleave(64, 0)[:n]
+            r = root[st.exp_avg_sq.view(-1).int()] * ex[:, 1]
+            assert torch.equal(a.float(), e4m3[st.exp_avg.view(-1).int()] * ex[:, 0]) and torch.equal(b, (r * r).to(dt))
+
+
 def _run(opt_args, steps, seed, ps, opt=None):
     from med_ts_llm_amd.hip.optim import HipAdam
     opt = HipAdam(ps, **opt_args) if opt is None else opt
