@@ -113,8 +113,7 @@ __global__ __launch_bounds__(256) void embedding_fwd_narrow_kernel(const void* _
     }
 }
 
-// a wave owns ROWS consecutive tokens and walks their columns: ROWS loads are in flight per step. `split` > 1: few tokens,
-// a row's columns are spread over that many waves.
+// a wave owns ROWS consecutive tokens and walks their columns: ROWS loads are in flight per step. `split` > 1: a row's columns are spread over that many waves.
 template <typename TT, typename OT, int W, int ROWS>
 __global__ __launch_bounds__(256) void embedding_fwd_kernel(const void* __restrict__ ids, int ids_i64, int64_t N, const TT* __restrict__ table, int64_t V, int64_t d, int64_t ld_table, float scale,
                                                             OT* __restrict__ out, int64_t ld_out, int split) {
@@ -663,15 +662,20 @@ void launch_fwd_w(const void* ids, int ids_i64, int64_t N, const void* table, in
                            ld_out, lpr);
         return;
     }
-    if (N >= 131072) {
-        // two tokens per wave: 200 003 x 1024 bf16 119.6 us, with one 128.2, with four 121.0; 65 536 x 1024 fp32 84.6 against 82.6 with one, 8192 x 4096 fp32 51 against 42
-        const int64_t waves = (N + 1) / 2;
-        hipLaunchKernelGGL((embedding_fwd_kernel<TT, OT, W, 2>), dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, st, ids, ids_i64, N, (const TT*)table, V, d, ld_table, scale, (OT*)out, ld_out, 1);
+    // Few tokens: a row's columns go to several waves, up to 8192 in all. 133 x 768 fp32 2.4 us (one wave per row 2.8), 1000 x 4096 5.8 (9.3); up to 16384 waves: 6.4, and 4096 x 768 5.7 against 5.0.
+    // A row of more than four waves keeps four, one workgroup that writes 4 KB in a row per step: 8192 x 4096 fp32 41.6 us, one wave per row 47; 131 072 x 4096 bf16 297 against 333.
+    const int64_t full = (d + 64 * W - 1) / (64 * W);
+    int64_t split = full;
+    while (split > (full > 4 ? 4 : 1) && N * split > 8192) split = (split + 1) / 2;
+    // many tokens of rows up to four waves wide: as many waves as the row has, each with its columns of several rows. 65 536 x 1024 fp32 76.5 us with four rows, 81.9 with two, 91 with one, one wave
+    // per row 86; 200 003 x 1024 bf16 115.3 with eight, 119.0 with four, one wave per two rows 119.8; of 1001 columns 137 against 154; below 16 384 tokens the loop above (8192 x 768 fp32 7.6 against 7.7)
+    if (full <= 4 && N >= 16384) {
+        const int rows = N >= 131072 ? 8 : 4;
+        const unsigned blocks = (unsigned)(((N + rows - 1) / rows * full + 3) / 4);
+        if (rows == 8) hipLaunchKernelGGL((embedding_fwd_kernel<TT, OT, W, 8>), dim3(blocks), dim3(256), 0, st, ids, ids_i64, N, (const TT*)table, V, d, ld_table, scale, (OT*)out, ld_out, (int)full);
+        else hipLaunchKernelGGL((embedding_fwd_kernel<TT, OT, W, 4>), dim3(blocks), dim3(256), 0, st, ids, ids_i64, N, (const TT*)table, V, d, ld_table, scale, (OT*)out, ld_out, (int)full);
         return;
     }
-    // few tokens: a row's columns go to several waves, up to 8192 in all. 133 x 768 fp32 2.4 us (one wave per row 2.8), 1000 x 4096 5.8 (9.3); up to 16384 waves: 6.4, and 4096 x 768 5.7 against 5.0
-    int64_t split = (d + 64 * W - 1) / (64 * W);
-    while (split > 1 && N * split > 8192) split = (split + 1) / 2;
     hipLaunchKernelGGL((embedding_fwd_kernel<TT, OT, W, 1>), dim3((unsigned)((N * split + 3) / 4)), dim3(256), 0, st, ids, ids_i64, N, (const TT*)table, V, d, ld_table, scale, (OT*)out, ld_out, (int)split);
 }
 template <typename TT, typename OT>

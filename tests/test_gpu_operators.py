@@ -58,6 +58,11 @@ def test_embedding_lookup(ops, N, V, d, tt, ot, idt):
     assert torch.equal(ops.embedding_fwd(ids, table), torch.where(ok[..., None], table[ids.long().clamp(0, V - 1)], 0.0).to(tt))
 
 
+@pytest.mark.parametrize("N,V,d,tt,ot", [(16387, 500, 1024, BF16, BF16), (16389, 70, 1001, F32, F32), (131077, 300, 520, BF16, BF16), (131075, 40, 261, BF16, F32), (131073, 50, 301, F32, BF16), (9001, 60, 4100, F32, F32)])
+def test_embedding_lookup_of_many_tokens(ops, N, V, d, tt, ot):
+    test_embedding_lookup(ops, (N,), V, d, tt, ot, torch.int64)
+
+
 def test_embedding_lookup_strides_and_empty(ops):
     g = gen(2)
     big = randn(g, 40, 70)
