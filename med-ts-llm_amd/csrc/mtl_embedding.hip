@@ -698,11 +698,17 @@ extern "C" int mtl_embedding_fwd(const void* ids, int ids_i64, int64_t N, const 
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     // 16-byte accesses of the wider type (8 columns only where both are bf16), one column where the row is shorter
     const int W = table_dtype == MTL_BF16 && out_dtype == MTL_BF16 && d >= 8 ? 8 : (d >= 4 ? 4 : 1);
-    if (table_dtype == MTL_F32 && out_dtype == MTL_F32) launch_fwd<float, float>(ids, ids_i64, N, table, V, d, ld_table, scale, out, ld_out, W, st);
-    else if (table_dtype == MTL_F32) launch_fwd<float, bf16_t>(ids, ids_i64, N, table, V, d, ld_table, scale, out, ld_out, W, st);
-    else if (out_dtype == MTL_F32) launch_fwd<bf16_t, float>(ids, ids_i64, N, table, V, d, ld_table, scale, out, ld_out, W, st);
-    else launch_fwd<bf16_t, bf16_t>(ids, ids_i64, N, table, V, d, ld_table, scale, out, ld_out, W, st);
-    MTL_CHECK_LAUNCH();
+    // (a launch holds less than 2^32 threads: up to 256 per token)
+    for (int64_t done = 0, n; done < N; done += n) {
+        n = N - done < (int64_t)1 << 23 ? N - done : (int64_t)1 << 23;
+        const void* at = reinterpret_cast<const char*>(ids) + done * (ids_i64 ? 8 : 4);
+        void* to = reinterpret_cast<char*>(out) + done * ld_out * size_of(out_dtype);
+        if (table_dtype == MTL_F32 && out_dtype == MTL_F32) launch_fwd<float, float>(at, ids_i64, n, table, V, d, ld_table, scale, to, ld_out, W, st);
+        else if (table_dtype == MTL_F32) launch_fwd<float, bf16_t>(at, ids_i64, n, table, V, d, ld_table, scale, to, ld_out, W, st);
+        else if (out_dtype == MTL_F32) launch_fwd<bf16_t, float>(at, ids_i64, n, table, V, d, ld_table, scale, to, ld_out, W, st);
+        else launch_fwd<bf16_t, bf16_t>(at, ids_i64, n, table, V, d, ld_table, scale, to, ld_out, W, st);
+        MTL_CHECK_LAUNCH();
+    }
     return MTL_OK;
 }
 
@@ -725,7 +731,7 @@ extern "C" int mtl_embedding_bwd(const void* ids, int ids_i64, int64_t N, const 
     if (!accumulate && ld_grad == d) { f.rows = 1; f.row_bytes = V * d * gs; }
     for (int w : {4, 16})
         if (((uintptr_t)grad & (w - 1)) == 0 && (f.rows == 1 || f.ld_bytes % w == 0)) f.width = w;
-    f.once = f.rows == 1 && f.width == 16 && f.row_bytes >= (int64_t)144 << 20 && f.row_bytes < (int64_t)1 << 44;
+    f.once = f.rows == 1 && f.width == 16 && f.row_bytes >= (int64_t)144 << 20 && f.row_bytes < (int64_t)1 << 35;      // (2^32 threads per launch)
     const int64_t fill_want = f.once ? (f.row_bytes + (1 << 17) - 1) / (1 << 17) * 8 : f.rows == 1 ? (f.row_bytes / f.width + 4095) / 4096 : f.rows;
     const unsigned fill_blocks = (unsigned)(f.once || fill_want < 512 ? (f.rows > 0 && fill_want < 1 ? 1 : fill_want) : 512);
     char* ws = reinterpret_cast<char*>(workspace);
@@ -741,7 +747,7 @@ extern "C" int mtl_embedding_bwd(const void* ids, int ids_i64, int64_t N, const 
     const int64_t chunks = chunks_of(d, W);
     const int S = window_of(N, chunks);
     const int64_t windows = (N + S - 1) / S;
-    if (chunks > 0x7fffffff || windows * chunks > (int64_t)0x7fffffff * 4) return MTL_ERR_UNSUPPORTED;      // (one grid)
+    if (chunks >= 1 << 26 || windows * chunks >= 1 << 26) return MTL_ERR_UNSUPPORTED;      // (one grid: 2^32 threads)
     const Plan p = plan_for(N, V, d);
     uint32_t* list_n = reinterpret_cast<uint32_t*>(ws);
     uint32_t* sid = reinterpret_cast<uint32_t*>(ws + p.sid);

@@ -20,6 +20,7 @@ namespace {
 
 constexpr int MAX_T = MTL_ADAM8_MAX_TENSORS;
 constexpr int THREADS = 256;
+constexpr int64_t MAX_BLOCKS = (1 << 24) - 1;      // 2^32 threads per launch: 17 G elements in fp32, 34 G in bf16
 // 4 elements per lane and iteration; all loads of a workgroup's iterations are in flight before the first use. Iterations, measured at 512 M elements: fp32 step 1 / 2 / 4: 1351 / 1475 /
 // 1413 us (6.1 TB/s); bf16 step 1066 / 968 / 1046 (5.3 TB/s: half of the bytes per element, the arithmetic shows). At 410 M elements, outputs not reused: read-back in fp32 659 / 689 / 737, in bf16
 // 465 / 389 / 422, packing 934 / 966 / -. What these have in common: a workgroup moves 4 KB in a row of each wide array.
@@ -391,6 +392,7 @@ int check_state(const mtl_adam8_state& t, bool read_back) {
     if (t.n > 0 && !read_back && (!t.m || !t.v)) return MTL_ERR_ARG;
     if ((uintptr_t)t.ex & 1) return MTL_ERR_ALIGN;
     if (t.dtype != MTL_F32 && !(read_back && t.dtype == MTL_BF16)) return MTL_ERR_ARG;
+    if (t.n > MAX_BLOCKS * dtype_chunk(t.dtype)) return MTL_ERR_UNSUPPORTED;
     return ((uintptr_t)t.m | (uintptr_t)t.v) & (t.dtype == MTL_F32 ? 3 : 1) ? MTL_ERR_ALIGN : MTL_OK;
 }
 
@@ -405,8 +407,7 @@ int for_tables(const mtl_adam8_state* states, int count, bool read_back, Launch 
         for (; i < count && tab.count < MAX_T; ++i) {
             if (states[i].n == 0) continue;
             const int64_t nb = (states[i].n + dtype_chunk(states[i].dtype) - 1) / dtype_chunk(states[i].dtype);
-            if (nb > 0x7fffffff) return MTL_ERR_UNSUPPORTED;
-            if (blocks + nb > 0x7fffffff) break;                // (this one goes into the next launch)
+            if (blocks + nb > MAX_BLOCKS) break;                // (this one goes into the next launch)
             tab.t[tab.count] = states[i];
             tab.first_block[tab.count++] = (int)blocks;
             blocks += nb;
@@ -428,6 +429,7 @@ extern "C" int mtl_adam8_step(const mtl_adam8_tensor* tensors, int count, double
         if (t.n < 0 || (t.param_dtype != MTL_F32 && t.param_dtype != MTL_BF16)) return MTL_ERR_ARG;
         if (t.n == 0) continue;
         if (!t.p || !t.g || !t.m8 || !t.r8 || !t.ex) return MTL_ERR_ARG;
+        if (t.n > MAX_BLOCKS * dtype_chunk(t.param_dtype)) return MTL_ERR_UNSUPPORTED;
         if ((((uintptr_t)t.p | (uintptr_t)t.g) & (t.param_dtype == MTL_BF16 ? 1 : 3)) || ((uintptr_t)t.ex & 1) || ((uintptr_t)t.shadow & 1)) return MTL_ERR_ALIGN;
         if (t.shadow && (t.cols <= 0 || t.ld_shadow < t.cols || t.n % t.cols != 0 || t.n >= ((int64_t)1 << 32))) return MTL_ERR_ARG;
     }
@@ -448,8 +450,7 @@ extern "C" int mtl_adam8_step(const mtl_adam8_tensor* tensors, int count, double
             const mtl_adam8_tensor& t = tensors[i];
             if (t.n == 0) continue;
             const int64_t nb = (t.n + dtype_chunk(t.param_dtype) - 1) / dtype_chunk(t.param_dtype);
-            if (nb > 0x7fffffff) return MTL_ERR_UNSUPPORTED;
-            if (blocks + nb > 0x7fffffff) break;
+            if (blocks + nb > MAX_BLOCKS) break;
             tab.t[tab.count] = t;
             tab.first_block[tab.count++] = (int)blocks;
             blocks += nb;

@@ -63,6 +63,19 @@ def test_embedding_lookup_of_many_tokens(ops, N, V, d, tt, ot):
     test_embedding_lookup(ops, (N,), V, d, tt, ot, torch.int64)
 
 
+@pytest.mark.parametrize("d,ot", [(8, F32), (264, BF16)])
+def test_embedding_lookup_in_several_launches(ops, d, ot):
+    """more tokens than one launch takes (8 388 608)"""
+    N, V = (1 << 23) + 77, 100
+    g = gen(5)
+    table = randn(g, V, d, dtype=ot)
+    ids = torch.randint(-1, V, (N,), generator=g, device="cuda", dtype=torch.int32)
+    out = ops.embedding_fwd(ids, table)
+    at, ok = ids.long().clamp(0), ids >= 0
+    for i in range(0, N, 1 << 21):
+        assert torch.equal(out[i:i + (1 << 21)], table[at[i:i + (1 << 21)]] * ok[i:i + (1 << 21), None])
+
+
 def test_embedding_lookup_strides_and_empty(ops):
     g = gen(2)
     big = randn(g, 40, 70)

@@ -156,6 +156,23 @@ def test_c_entry_points_refuse_bad_arguments_without_a_gpu():
     assert lib.mtl_adam8_step(t, 1, 1e-3, 0.9, 0.999, 1e-8, 0.0, 0, 1, None) == 0
 
 
+def test_c_entry_points_refuse_more_threads_than_a_launch_holds():
+    """2^32 threads and more: an error before the first launch, also where a smaller tensor stands in front"""
+    import ctypes as C
+    from med_ts_llm_amd.hip import _native as N
+    lib = N.lib()
+    buf = (C.c_char * 4096)()
+    at = (C.addressof(buf) + 255) // 256 * 256
+    assert lib.mtl_embedding_bwd(at, 1, 1 << 30, at, 0, 4096, 5, 4096, -1, 1.0, at, 0, 4096, 0, at, 1 << 62, None) == -3
+    t = (N.Adam8Tensor * 200)()
+    s = (N.Adam8State * 200)()
+    for i in range(200):
+        t[i].p = t[i].g = t[i].m8 = t[i].r8 = t[i].ex = s[i].m8 = s[i].r8 = s[i].ex = s[i].m = s[i].v = at
+        t[i].n = s[i].n = 4 if i < 199 else 1 << 34
+    assert lib.mtl_adam8_step(t, 200, 1e-3, 0.9, 0.999, 1e-8, 0.0, 0, 1, None) == -3
+    assert lib.mtl_adam8_moments(s, 200, None) == -3 and lib.mtl_adam8_quantize(s, 200, 1, None) == -3
+
+
 def test_embedding_workspace_holds_every_part():
     from med_ts_llm_amd.hip import _native as N
     f = N.lib().mtl_embedding_bwd_workspace_bytes
