@@ -325,8 +325,8 @@ __global__ __launch_bounds__(1024) void qk_norm_rope_dw_kernel(const float* __re
 }
 
 // Workgroups per side; more rows are walked by the same ones. Forward 1024 / 2048: 29.2 / 30.8 us at 6656 x (32 + 8) heads of 128 in bf16, 14.2 / 16.4 at 8192 x 24 of 64, 57.6 / 55.8 at 8224 x 64 of 128.
-// Backward 512 / 768 / 1536: 102 / 90 / 96 us at 8224 x 64 heads, 50 / 51 / 57 at 6656 x 40 (three of its workgroups fit a CU). Two of a wave's head steps in flight in the forward: 50 us, one 57,
-// four 55.
+// Backward 512 / 768 / 1536: 102 / 90 / 96 us at 8224 x 64 heads, 50 / 51 / 57 at 6656 x 40 (three of its workgroups fit a CU). Two of a wave's head steps in flight in the forward: 49 us, four
+// 50 (without the loads below that pass the cache: 50, one step 57, four 55).
 inline unsigned fwd_blocks(int64_t rows) { const int64_t b = (rows + WAVES - 1) / WAVES; return (unsigned)(b < 1024 ? b : 1024); }
 inline unsigned bwd_blocks(int64_t rows) { const int64_t b = (rows + WAVES - 1) / WAVES; return (unsigned)(b < 768 ? b : 768); }
 
@@ -364,7 +364,7 @@ int launch_with(const mtl_qk_norm_rope_args& a, bool bwd, hipStream_t st) {
 // next. Without / with, us, bf16 heads of 128: forward 42 MB 18.6 / 21.4, 67 MB 27.8 / 27.5, 101 MB 43.4 / 40.1, 135 MB 57.6 / 49.2, 270 MB 109 / 106; backward 42 MB 35.4 / 35.7, 67 MB 48.9 / 45.4,
 // 101 MB 68.7 / 62.9, 135 MB 86.4 / 78.6, 270 MB 160 / 156. Between a projection and the attention: 67 MB 126 / 122, 135 MB 286 / 273. Only where every half of a head is whole lines of 128 bytes and a
 // load takes 16 of each lane's: a line that two loads share comes twice (heads of 64, 101 MB: forward 51 / 52, backward 77 / 81; of 100: 78 / 83, 112 / 115; fp32, 135 MB: no gain). Stores that pass the
-// cache by gain 6 % alone and lose more in the kernel that reads them.
+// cache by gain 6 % alone and lose up to 20 % with the kernel that reads them.
 template <typename T, int W, int LPH, int C, bool S>
 int launch(const mtl_qk_norm_rope_args& a, bool bwd, hipStream_t st) {
     if constexpr (W == 8 && LPH >= 8 && !S && sizeof(T) == 2)
