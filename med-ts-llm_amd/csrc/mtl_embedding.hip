@@ -663,7 +663,7 @@ void launch_fwd_w(const void* ids, int ids_i64, int64_t N, const void* table, in
         return;
     }
     // Few tokens: a row's columns go to several waves, up to 8192 in all. 133 x 768 fp32 2.4 us (one wave per row 2.8), 1000 x 4096 5.8 (9.3); up to 16384 waves: 6.4, and 4096 x 768 5.7 against 5.0.
-    // A row of more than four waves keeps four, one workgroup that writes 4 KB in a row per step: 8192 x 4096 fp32 41.6 us, one wave per row 47; 131 072 x 4096 bf16 297 against 333.
+    // A row of more than four waves keeps three or four, one workgroup that writes 4 KB in a row per step: 8192 x 4096 fp32 41.6 us, one wave per row 47; 131 072 x 4096 bf16 297 against 333.
     const int64_t full = (d + 64 * W - 1) / (64 * W);
     int64_t split = full;
     while (split > (full > 4 ? 4 : 1) && N * split > 8192) split = (split + 1) / 2;
