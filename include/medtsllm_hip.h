@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define MTL_ABI_VERSION 16
+#define MTL_ABI_VERSION 17
 
 enum { MTL_OK = 0, MTL_ERR_ARG = -1, MTL_ERR_ALIGN = -2, MTL_ERR_UNSUPPORTED = -3, MTL_ERR_LAUNCH = -4,
        MTL_ERR_WORKSPACE = -5 };
@@ -235,9 +235,12 @@ int mtl_adam_step(const mtl_adam_tensor* tensors, int count, float lr, float bet
  * the root of the second as unsigned 4.4 numbers, one power-of-two exponent each per block. fp32: 16 B of traffic per element instead of 28, 2.03 B of state instead of 8.
  * All arithmetic in fp32, one rounding per operation in a fixed order: the result is a function of the inputs and `step`, bit for bit, on any machine. The root is rounded
  * against a threshold taken from (step, element index); a tensor updated in two pieces is therefore not the tensor updated in one.
+ * The first moment is rounded to the nearest code, or (MTL_ADAM8_M_THRESHOLD) against 16 hashed bits of (step, element index). A run of steps needs the latter: to nearest, a first moment
+ * stands still wherever (1 - beta1) |g - m| is below half a step of its grid (csrc/mtl_optim8.hip).
  * Hyper-parameters are doubles (1 - beta is formed before the rounding to fp32). All-zero codes and exponents are zero moments. */
 #define MTL_ADAM8_MAX_TENSORS 40   /* per launch: 40 x 80 B of kernel arguments */
 #define MTL_ADAM8_BLOCK 64
+enum { MTL_ADAM8_DECOUPLED = 1 /* weight decay */, MTL_ADAM8_M_THRESHOLD = 2 };   /* flags of mtl_adam8_step */
 typedef struct mtl_adam8_tensor {
     void* p;
     const void* g;
@@ -249,7 +252,7 @@ typedef struct mtl_adam8_tensor {
     int64_t cols, ld_shadow;
     int64_t param_dtype; /* MTL_F32 | MTL_BF16 (p and g) */
 } mtl_adam8_tensor;
-int mtl_adam8_step(const mtl_adam8_tensor* tensors, int count, double lr, double beta1, double beta2, double eps, double weight_decay, int decoupled, int64_t step,
+int mtl_adam8_step(const mtl_adam8_tensor* tensors, int count, double lr, double beta1, double beta2, double eps, double weight_decay, int flags, int64_t step,
                    void* stream);
 typedef struct mtl_adam8_state {
     uint8_t* m8;

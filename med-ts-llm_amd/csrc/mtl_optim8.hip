@@ -1,13 +1,17 @@
 // Adam / AdamW step with the two moments held in 8 bits (mtl_adam8_step), their read-back (mtl_adam8_moments) and their packing (mtl_adam8_quantize).
 //
 // Blocks of 64 consecutive elements (flat index) share two power-of-two scales, one signed byte each:
-//   m = e4m3(cm) 2^em       round to nearest even, em = floor(log2 max |m|) - 7: the block's largest value lands in [128, 256] of e4m3's 448
+//   m = e4m3(cm) 2^em       em = floor(log2 max |m|) - 7: the block's largest value lands in [128, 256] of e4m3's 448
 //   r = u44(cr) 2^er        the ROOT of the second moment (v = r^2: half of v's exponent range), unsigned, 4 exponent and 4 mantissa bits:
 //                           u44(c) = c for c < 16, else (16 + c % 16) 2^(c / 16 - 1); er = floor(log2 max r) - 17, so codes end at 240; 255 is NaN
 // Both formats are floating, so a power-of-two scale costs no precision, multiplies exactly, and a block whose scale changes keeps every value on its grid.
 // r is rounded up or down by a threshold u(i, t) = frac(i a1 + t a2), (a1, a2) = the 2-D additive recurrence of the plastic number (1 / 1.3247.., 1 / 1.3247..^2):
 // equidistributed over the elements of a step and over the steps of an element. Rounding to nearest would freeze r: with beta2 = 0.999 a step moves it by
 // about 1 / 2000 of its value, half a grid step is 1 / 64 .. 1 / 32. No generator state: the step number and the element's index are all of it.
+// |m| is rounded up or down by a threshold as well (MTL_ADAM8_M_THRESHOLD; 16 hashed bits of (step, index): m moves by 1 - beta1 of its distance to g, up to a whole grid step at a time, too
+// fast for a recurrence to be independent of what it meets). To nearest, which a step without that flag does, is the closest code for ONE step, but over a run m stands still wherever
+// (1 - beta1) |g - m| is below half a grid step: a constant gradient is held at 0.78 / 0.54 / 0.20 of its value (beta1 0.9 / 0.95 / 0.99), and what is left of a gradient that has
+// stopped never goes, while r under it decays: a step of lr and more for ever. The thresholds cost 1 - 7 % of the fp32 step and 8 - 15 % of the bf16 step. mtl_adam8_quantize, which rounds once and feeds nothing back, takes the nearest code.
 // r > 0 never gets code 0 (m / (0 + eps) would explode); what is not finite becomes the NaN code of that element alone.
 //
 // Every operation is ONE fp32 operation, rounded to nearest, in the order written (no contraction into fma, exact division and square root): a change in the last bit moves
@@ -33,7 +37,7 @@ struct Adam8Table {
     int first_block[MAX_T + 1];
     int count;
 };
-struct Adam8Hyper { float om_b1, b2, om_b2, eps, wd, decay, inv_bc2, step_size; uint32_t t_thr; int mode; };   // mode: 0 no decay, 1 L2, 2 decoupled
+struct Adam8Hyper { float om_b1, b2, om_b2, eps, wd, decay, inv_bc2, step_size; uint32_t t_thr, m_base; int mode; };   // mode: 0 no decay, 1 L2, 2 decoupled
 
 struct State8Table {
     mtl_adam8_state t[MAX_T];
@@ -111,9 +115,19 @@ __device__ __forceinline__ float sqrt_near(float x) {
 }
 
 constexpr uint32_t DITHER_I = 0xC13FA9A9u;
+constexpr uint32_t M_STREAM = 0x6D38u;          // the first moment's words of the counter hash
 
-// Codes of 4 elements and the block's exponents (the same in the 16 lanes of a block) from m and v; r[] receives sqrt(v). Every lane of the wave is active.
-__device__ __forceinline__ void encode4(const float (&m)[4], const float (&v)[4], float (&r)[4], uint32_t idx, uint32_t t_thr, uint32_t& cm, uint32_t& cr, uint32_t& ex) {
+// e4m3 code of y, |y| <= 256, its magnitude rounded up where the fraction of a grid step and field / 2^16 (the middle of field's interval) reach one
+__device__ __forceinline__ uint32_t encode_m(float y, uint32_t field) {
+    const uint32_t b = __float_as_uint(y), a = b & 0x7fffffffu, u = field * 16u + 8u;
+    const uint32_t normal = ((a + u) >> 20) - 120u * 8u;                                                                        // 2^-6 and more: three mantissa bits stay
+    const uint32_t small = (uint32_t)__builtin_floorf(__uint_as_float(a) * 512.0f + (float)u * 0x1p-20f);                          // multiples of 2^-9
+    return ((a >= 0x3c800000u ? normal : small) & 0x7fu) | ((b >> 24) & 0x80u);
+}
+
+// Codes of 4 elements and the block's exponents (the same in the 16 lanes of a block) from m and v; r[] receives sqrt(v). Every lane of the wave is active. M_THR: m against thresholds.
+template <bool M_THR>
+__device__ __forceinline__ void encode4(const float (&m)[4], const float (&v)[4], float (&r)[4], int64_t e0, uint32_t t_thr, uint32_t m_base, uint32_t& cm, uint32_t& cr, uint32_t& ex) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) r[e] = sqrt_near(v[e]);
     uint32_t mb[4], rb[4];
@@ -121,7 +135,7 @@ __device__ __forceinline__ void encode4(const float (&m)[4], const float (&v)[4]
     for (int e = 0; e < 4; ++e) { mb[e] = __float_as_uint(m[e]) & 0x7fffffffu; rb[e] = __float_as_uint(r[e]); }
     uint32_t tm = row_max(max4(mb[0], mb[1], mb[2], mb[3])), tr = row_max(max4(rb[0], rb[1], rb[2], rb[3]));
     int em = scale_exp(tm, 7), er = scale_exp(tr, 17);
-    const uint32_t u0 = idx * DITHER_I + t_thr;
+    const uint32_t u0 = (uint32_t)e0 * DITHER_I + t_thr;
     // 16 in the block's scale, and 2^-48: smaller roots come from v < 2^-96, for which sqrt_near is not exact
     const uint32_t least = (uint32_t)(131 + er) << 23, lo = least > 0x27800000u ? least : 0x27800000u;
     if (__any(tm >= INF_BITS || tr >= INF_BITS || min4(rb[0], rb[1], rb[2], rb[3]) < lo)) {
@@ -144,9 +158,17 @@ __device__ __forceinline__ void encode4(const float (&m)[4], const float (&v)[4]
         for (int e = 0; e < 4; ++e) cr |= (((rb[e] + ((u0 + (uint32_t)e * DITHER_I) >> 13)) >> 19) - k) << (8 * e);
     }
     const float im = pow2i(-em);
-    int pk = __builtin_amdgcn_cvt_pk_fp8_f32(m[0] * im, m[1] * im, 0, false);
-    pk = __builtin_amdgcn_cvt_pk_fp8_f32(m[2] * im, m[3] * im, pk, true);
-    cm = (uint32_t)pk;
+    if constexpr (M_THR) {
+        const uint64_t quad = (uint64_t)e0 >> 2;                // (the hash takes 24 bits of each of its two coordinates)
+        const uint2 w = drop_quad(m_base, (uint32_t)(quad >> 24), (uint32_t)quad & 0xffffffu);
+        cm = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) cm |= encode_m(m[e] * im, drop_field(w, (uint32_t)e)) << (8 * e);
+    } else {
+        int pk = __builtin_amdgcn_cvt_pk_fp8_f32(m[0] * im, m[1] * im, 0, false);
+        pk = __builtin_amdgcn_cvt_pk_fp8_f32(m[2] * im, m[3] * im, pk, true);
+        cm = (uint32_t)pk;
+    }
     if (__any(max4(mb[0], mb[1], mb[2], mb[3]) >= INF_BITS))
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -181,7 +203,7 @@ __device__ __forceinline__ void adam8_moments_of(float& p, float g, float& m, fl
 __device__ __forceinline__ float adam8_update(float p, float m, float r, const Adam8Hyper& h) { return p - (m / (r * h.inv_bc2 + h.eps)) * h.step_size; }
 
 // HBM-bound: fp32 16 + 4/64 B per element (p read and written, g read, two code bytes read and written, two exponent bytes per 64 elements each way), bf16 10 + 4/64.
-template <bool P16>
+template <bool P16, bool M_THR>
 __device__ __forceinline__ void adam8_chunk(const mtl_adam8_tensor& t, int64_t base, const Adam8Hyper& h) {
     float* p32 = reinterpret_cast<float*>(t.p);
     const float* g32 = reinterpret_cast<const float*>(t.g);
@@ -239,7 +261,7 @@ __device__ __forceinline__ void adam8_chunk(const mtl_adam8_tensor& t, int64_t b
             if (e >= nv) m[e] = v[e] = 0.f;                     // (elements behind the tensor's end have no part in their block's scales)
         }
         uint32_t nm, nr, nx;
-        encode4(m, v, r, (uint32_t)e0, h.t_thr, nm, nr, nx);
+        encode4<M_THR>(m, v, r, e0, h.t_thr, h.m_base, nm, nr, nx);
 #pragma unroll
         for (int e = 0; e < 4; ++e) pp[i][e] = adam8_update(pp[i][e], m[e], r[e], h);
         if (nv == 0) continue;                                  // (no cross-lane operation below)
@@ -278,14 +300,15 @@ __device__ __forceinline__ void adam8_chunk(const mtl_adam8_tensor& t, int64_t b
     }
 }
 
+template <bool M_THR>
 __global__ __launch_bounds__(THREADS) void adam8_step_kernel(const Adam8Table tab, const Adam8Hyper h) {
     int ti = 0;
     const int b = blockIdx.x;
     while (ti + 1 < tab.count && b >= tab.first_block[ti + 1]) ++ti;
     const mtl_adam8_tensor t = tab.t[ti];
     const int64_t at = b - tab.first_block[ti];
-    if (t.param_dtype == MTL_BF16) adam8_chunk<true>(t, at * chunk_of(ITERS_B16), h);
-    else adam8_chunk<false>(t, at * chunk_of(ITERS_F32), h);
+    if (t.param_dtype == MTL_BF16) adam8_chunk<true, M_THR>(t, at * chunk_of(ITERS_B16), h);
+    else adam8_chunk<false, M_THR>(t, at * chunk_of(ITERS_F32), h);
 }
 
 template <bool NT, typename V>
@@ -379,7 +402,7 @@ __global__ __launch_bounds__(THREADS) void adam8_quantize_kernel(const State8Tab
             }
         }
         uint32_t nm, nr, nx;
-        encode4(m, v, r, (uint32_t)e0, t_thr, nm, nr, nx);
+        encode4<false>(m, v, r, e0, t_thr, 0u, nm, nr, nx);
         if (nv == 0) continue;
         store_codes(t.m8 + e0, nm, nv, vec8);
         store_codes(t.r8 + e0, nr, nv, vec8);
@@ -422,8 +445,8 @@ int for_tables(const mtl_adam8_state* states, int count, bool read_back, Launch 
 
 }  // namespace
 
-extern "C" int mtl_adam8_step(const mtl_adam8_tensor* tensors, int count, double lr, double beta1, double beta2, double eps, double weight_decay, int decoupled, int64_t step, void* stream) {
-    if (count < 0 || (count > 0 && !tensors) || step < 1 || !(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) || !(eps >= 0.0) || !(weight_decay >= 0.0)) return MTL_ERR_ARG;
+extern "C" int mtl_adam8_step(const mtl_adam8_tensor* tensors, int count, double lr, double beta1, double beta2, double eps, double weight_decay, int flags, int64_t step, void* stream) {
+    if (count < 0 || (count > 0 && !tensors) || step < 1 || !(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) || !(eps >= 0.0) || !(weight_decay >= 0.0) || (flags & ~(MTL_ADAM8_DECOUPLED | MTL_ADAM8_M_THRESHOLD))) return MTL_ERR_ARG;
     for (int i = 0; i < count; ++i) {
         const mtl_adam8_tensor& t = tensors[i];
         if (t.n < 0 || (t.param_dtype != MTL_F32 && t.param_dtype != MTL_BF16)) return MTL_ERR_ARG;
@@ -440,7 +463,8 @@ extern "C" int mtl_adam8_step(const mtl_adam8_tensor* tensors, int count, double
     h.inv_bc2 = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)step)));
     h.step_size = (float)(lr / (1.0 - pow(beta1, (double)step)));
     h.t_thr = (uint32_t)step * 0x91E10DA5u;
-    h.mode = weight_decay == 0.0 ? 0 : (decoupled ? 2 : 1);
+    h.m_base = drop_base((uint32_t)step, M_STREAM);
+    h.mode = weight_decay == 0.0 ? 0 : (flags & MTL_ADAM8_DECOUPLED ? 2 : 1);
     for (int i = 0; i < count;) {
         Adam8Table tab;
         tab.count = 0;
@@ -458,7 +482,8 @@ extern "C" int mtl_adam8_step(const mtl_adam8_tensor* tensors, int count, double
         }
         tab.first_block[tab.count] = (int)blocks;
         if (blocks == 0) continue;
-        MTL_LAUNCH("adam8_step_kernel", bytes, 1, adam8_step_kernel, dim3((unsigned)blocks), dim3(THREADS), 0, st, tab, h);
+        if (flags & MTL_ADAM8_M_THRESHOLD) MTL_LAUNCH("adam8_step_kernel", bytes, 1, adam8_step_kernel<true>, dim3((unsigned)blocks), dim3(THREADS), 0, st, tab, h);
+        else MTL_LAUNCH("adam8_step_kernel", bytes, 1, adam8_step_kernel<false>, dim3((unsigned)blocks), dim3(THREADS), 0, st, tab, h);
         MTL_CHECK_LAUNCH();
     }
     return MTL_OK;

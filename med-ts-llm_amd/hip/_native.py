@@ -14,7 +14,7 @@ LIB_PATH = os.environ.get("MTL_LIB_PATH") or os.path.join(_HERE, "libmedtsllm_hi
 MTL_F32, MTL_BF16 = 0, 1
 EPI_STORE, EPI_GELU, EPI_RESID, EPI_DGELU, EPI_ACCUM, EPI_SWIGLU, EPI_DSWIGLU = 0, 1, 2, 3, 4, 5, 6
 ARCH_GPT2, ARCH_LLAMA = 0, 1
-ABI_VERSION = 16
+ABI_VERSION = 17
 
 i64, vp, f32, i32 = C.c_int64, C.c_void_p, C.c_float, C.c_int
 
@@ -65,6 +65,7 @@ class Adam8State(C.Structure):
 
 
 ADAM8_BLOCK = 64
+ADAM8_DECOUPLED, ADAM8_M_THRESHOLD = 1, 2
 f64 = C.c_double
 
 

@@ -7,6 +7,7 @@ HipAdam(state_bits=8) holds both moments in 8 bits (`mtl_adam8_step`: 2.03 bytes
 parameter's shape), "q_exp" (exponents [blocks of 64, 2]). A state saved at the other width is converted at the first step after it is loaded."""
 import collections
 import ctypes as C
+import warnings
 
 import torch
 
@@ -61,10 +62,24 @@ def adam8_state(p):
                       torch.zeros(((p.numel() + N.ADAM8_BLOCK - 1) // N.ADAM8_BLOCK, 2), dtype=torch.uint8, device=p.device))
 
 
+_said_nearest = False
+
+
 @torch.no_grad()
-def adam8_step(params, grads, states, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, decoupled_weight_decay=False, shadows=None):
+def adam8_step(params, grads, states, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, decoupled_weight_decay=False, shadows=None, first_moment=None):
     """one Adam / AdamW step, in place, of several tensors (contiguous, f32 or bf16, gradients likewise) whose moments are Adam8States; `step` counts from 1 and is the same for all.
-    shadows: Bf16Shadow or None for each. One launch per 40 tensors. Same result for the same inputs and step, bit for bit. (In a captured graph the step number is a constant.)"""
+    shadows: Bf16Shadow or None for each. One launch per 40 tensors. Same result for the same inputs and step, bit for bit. (In a captured graph the step number is a constant.)
+    first_moment: how the new first moment is rounded to its code. "threshold": up or down, by a hash of (step, element), so that it is right in the mean over a run of steps, for every
+    beta1 (what HipAdam takes). "nearest": the closest code, for a single step; over a run it stands still wherever (1 - beta1) |g - m| is below half a step of its grid: a constant
+    gradient is held at 0.5 to 0.8 of its value, one that stops leaves a rest that moves its parameter for ever. Not given: "nearest", with a warning (once)."""
+    global _said_nearest
+    if first_moment is None:
+        if not _said_nearest:
+            _said_nearest = True
+            warnings.warn('adam8_step rounds the first moment to the nearest code, which a run of steps cannot follow: give first_moment="threshold" (or "nearest", for a single step)', stacklevel=3)
+    elif first_moment not in ("nearest", "threshold"):
+        raise ValueError(f'adam8_step: first_moment is "nearest" or "threshold", got {first_moment!r}')
+    flags = (N.ADAM8_DECOUPLED if decoupled_weight_decay else 0) | (N.ADAM8_M_THRESHOLD if first_moment == "threshold" else 0)
     params, grads, states = list(params), list(grads), list(states)
     shadows = [None] * len(params) if shadows is None else list(shadows)
     if not len(params) == len(grads) == len(states) == len(shadows):
@@ -95,7 +110,7 @@ def adam8_step(params, grads, states, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-
             raise ValueError(f"adam8_step: the same {name} twice in one step")
     _one_gpu(touched + read, "adam8_step")
     with N.on_device(params[0]):
-        N.check(N.lib().mtl_adam8_step((N.i64 * len(rows))(*rows), len(params), lr, b1, b2, eps, weight_decay, 1 if decoupled_weight_decay else 0, step, N.stream()), "mtl_adam8_step")
+        N.check(N.lib().mtl_adam8_step((N.i64 * len(rows))(*rows), len(params), lr, b1, b2, eps, weight_decay, flags, step, N.stream()), "mtl_adam8_step")
     torch.autograd.graph.increment_version(touched)   # the kernel wrote through raw pointers: bump the autograd versions like an in-place op
     for p, sh in zip(params, shadows):
         if sh is not None:
@@ -251,7 +266,7 @@ class HipAdam(torch.optim.Optimizer):
         if self.state_bits == 8:
             grads = [p.grad if p.grad.dtype == p.dtype and p.grad.is_contiguous() else p.grad.to(p.dtype).contiguous() for p in ps]
             adam8_step(ps, grads, [Adam8State(*(self.state[p][k] for k in _STATE8)) for p in ps], step, group["lr"], group["betas"], group["eps"], group["weight_decay"],
-                       group["decoupled_weight_decay"], [self._shadows.get(id(p)) for p in ps])
+                       group["decoupled_weight_decay"], [self._shadows.get(id(p)) for p in ps], "threshold")
             return
         arr = (N.AdamTensor * len(ps))()
         keep = []

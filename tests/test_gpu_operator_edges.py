@@ -1,0 +1,111 @@
+"""GPU tests of the token table, the query / key norm and the 8-bit Adam step where a call's effect reaches beyond the call: runs of many steps, values at the ends of their range, state read
+beside a running update, views and versions of what is written."""
+import numpy as np
+import pytest
+import torch
+
+import adam8_ref as A8
+import adam8_threshold_ref as T8
+from test_gpu_operators import codes_of, gen, np_of, randn
+
+pytestmark = pytest.mark.gpu
+F32, BF16, F64 = torch.float32, torch.bfloat16, torch.float64
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from med_ts_llm_amd.hip import ops
+    return ops
+
+
+@pytest.fixture(scope="module")
+def optim():
+    from med_ts_llm_amd.hip import optim
+    return optim
+
+
+# ================================================================================================ first moment against thresholds
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("wd,decoupled", [(0.0, False), (0.01, False), (0.01, True)])
+def test_adam8_threshold_step_bit_for_bit(optim, dt, wd, decoupled):
+    """parameters, codes and exponents equal the numpy restatement's bits over six steps: odd sizes, unaligned views, gradients of every magnitude, zeros, NaN and infinities"""
+    g = gen(3)
+    sizes = [1, 3, 63, 64, 65, 1000, 4097, 70001]
+    base = [randn(g, n + 1, dtype=dt, std=0.1) for n in sizes]
+    ps = [b[1:] if i % 2 else b[:-1] for i, b in enumerate(base)]
+    sts = [optim.adam8_state(p) for p in ps]
+    want = [(np_of(p), codes_of(st)) for p, st in zip(ps, sts)]
+    for t in range(1, 7):
+        gs = [(randn(g, p.numel()) * torch.exp(3 * randn(g, p.numel()))).to(dt) * 10.0 ** (t - 4) for p in ps]
+        if t > 1:
+            gs[5][100:300] = 0
+        if t == 4:
+            gs[5][10], gs[5][11], gs[6][64] = np.nan, np.inf, -np.inf
+        optim.adam8_step(ps, gs, sts, t, lr=1e-2, weight_decay=wd, decoupled_weight_decay=decoupled, first_moment="threshold")
+        for i, (p, gr, st) in enumerate(zip(ps, gs, sts)):
+            wp, wc = T8.step(want[i][0], np_of(gr), want[i][1], t, 1e-2, 0.9, 0.999, 1e-8, wd, decoupled)
+            if dt == BF16:
+                wp = torch.from_numpy(wp).to(BF16).float().numpy()
+            want[i] = (wp, wc)
+            assert np.array_equal(np_of(p), wp, equal_nan=True), (t, sizes[i])
+            for a, b, what in zip(codes_of(st), wc, "mre"):
+                assert np.array_equal(a, b), (t, sizes[i], what, np.flatnonzero(a != b)[:5])
+
+
+def test_adam8_threshold_step_of_a_large_tensor(optim):
+    """elements behind 2^31 get thresholds of their own index"""
+    n = (1 << 31) + 4097
+    big, gr = torch.zeros(n, dtype=BF16, device="cuda"), torch.full((n,), 1e-3, dtype=BF16, device="cuda")
+    lo = (n - 1) // 64 * 64 - 4096
+    gr[lo:] = randn(gen(1), n - lo, dtype=BF16, std=1e-3)
+    st = optim.adam8_state(big)
+    optim.adam8_step([big], [gr], [st], 1, lr=1e-2, first_moment="threshold")
+    k = n - lo
+    zero = (np.zeros(k, np.uint8), np.zeros(k, np.uint8), np.zeros(((k + 63) // 64, 2), np.int8))
+    wp, wc = T8.step(np.zeros(k, np.float32), np_of(gr[lo:]), zero, 1, 1e-2, 0.9, 0.999, 1e-8, first=lo)
+    assert np.array_equal(np_of(big[lo:]), torch.from_numpy(wp).to(BF16).float().numpy())
+    assert np.array_equal(st.exp_avg[lo:].cpu().numpy(), wc[0]) and np.array_equal(st.exp_avg_sq[lo:].cpu().numpy(), wc[1])
+
+
+@pytest.mark.parametrize("b1", [0.9, 0.95])
+def test_hip_adam_8_follows_gradients_over_many_steps(optim, b1):
+    """a constant gradient moves its parameters as exact Adam does; one that stops in half of every block stops moving them (bounds: tests/test_adam8_trajectory.py)"""
+    p = torch.zeros(4096, device="cuda", requires_grad=True)
+    opt = optim.HipAdam([p], lr=1e-3, betas=(b1, 0.999), state_bits=8)
+    for _ in range(300):
+        p.grad = torch.full_like(p, 0.01)
+        opt.step()
+    assert abs(p.mean().item() + 0.3) <= (0.03 + 0.32 / 64) * 0.3 and (p + 0.3).abs().max() <= 0.3
+    g = gen(4)
+    q = torch.zeros(4096, device="cuda", requires_grad=True)
+    opt = optim.HipAdam([q], lr=1e-3, betas=(b1, 0.999), state_bits=8)
+    dead = torch.arange(4096, device="cuda") % 64 < 32
+    x = m = v = 0.0
+    for t in range(1, 10001):
+        one = 1.0 if t <= 100 else 0.0
+        q.grad = torch.where(dead, one, randn(g, 4096))
+        opt.step()
+        m, v = b1 * m + (1 - b1) * one, 0.999 * v + 0.001 * one
+        x -= 1e-3 / (1 - b1 ** t) * m / ((v / (1 - 0.999 ** t)) ** 0.5 + 1e-8)
+    off = (q.detach()[dead] - x).abs()
+    assert off.mean().item() <= 0.16 * abs(x) and off.max().item() <= abs(x) and not opt.moments()[q][0][dead].any()
+
+
+def test_hip_adam_8_takes_thresholds(optim):
+    """HipAdam(state_bits=8) is adam8_step(first_moment="threshold"); without an answer adam8_step rounds to nearest and says so"""
+    g = gen(5)
+    p = randn(g, 33, 70).requires_grad_()
+    ref, st = p.detach().clone(), optim.adam8_state(p)
+    other, so = p.detach().clone(), optim.adam8_state(p)
+    opt = optim.HipAdam([p], lr=1e-2, state_bits=8)
+    optim._said_nearest = False
+    for t in range(1, 4):
+        p.grad = randn(g, 33, 70, std=1e-2)
+        opt.step()
+        optim.adam8_step([ref], [p.grad], [st], t, lr=1e-2, first_moment="threshold")
+        if t == 1:
+            with pytest.warns(UserWarning, match="nearest"):
+                optim.adam8_step([other], [p.grad], [so], t, lr=1e-2)
+        else:
+            optim.adam8_step([other], [p.grad], [so], t, lr=1e-2, first_moment="nearest")
+    assert torch.equal(p, ref) and torch.equal(opt.state[p]["exp_avg_q"], st.exp_avg) and not torch.equal(other, ref)

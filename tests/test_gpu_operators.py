@@ -554,7 +554,7 @@ def test_hip_adam_with_8_bit_state(optim):
     _run(None, 3, 50, ps, opt)
     for t in range(3):
         gg = gen(50 + t)
-        optim.adam8_step(ref, [randn(gg, *p.shape, std=1e-2) for p in ref], sts, t + 1, lr=1e-2, weight_decay=0.01, decoupled_weight_decay=True)
+        optim.adam8_step(ref, [randn(gg, *p.shape, std=1e-2) for p in ref], sts, t + 1, lr=1e-2, weight_decay=0.01, decoupled_weight_decay=True, first_moment="threshold")
     assert all(torch.equal(a, b) for a, b in zip(ps, ref)) and ps[0]._version > v0 and sh.fresh()
     assert torch.equal(sh.tensor[:, :101], ps[0].detach().to(BF16)) and not sh.tensor[:, 101:].any()
     sd = opt.state_dict()
