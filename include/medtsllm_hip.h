@@ -237,6 +237,7 @@ int mtl_adam_step(const mtl_adam_tensor* tensors, int count, float lr, float bet
  * against a threshold taken from (step, element index); a tensor updated in two pieces is therefore not the tensor updated in one.
  * The first moment is rounded to the nearest code, or (MTL_ADAM8_M_THRESHOLD) against 16 hashed bits of (step, element index). A run of steps needs the latter: to nearest, a first moment
  * stands still wherever (1 - beta1) |g - m| is below half a step of its grid (csrc/mtl_optim8.hip).
+ * A second moment that overflows fp32 (finite |g| > 1.8e19) is held as infinity: its parameter stands still, as with 32-bit moments. Any other value that is not finite is NaN.
  * Hyper-parameters are doubles (1 - beta is formed before the rounding to fp32). All-zero codes and exponents are zero moments. */
 #define MTL_ADAM8_MAX_TENSORS 40   /* per launch: 40 x 80 B of kernel arguments */
 #define MTL_ADAM8_BLOCK 64

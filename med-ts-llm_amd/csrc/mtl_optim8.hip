@@ -3,7 +3,7 @@
 // Blocks of 64 consecutive elements (flat index) share two power-of-two scales, one signed byte each:
 //   m = e4m3(cm) 2^em       em = floor(log2 max |m|) - 7: the block's largest value lands in [128, 256] of e4m3's 448
 //   r = u44(cr) 2^er        the ROOT of the second moment (v = r^2: half of v's exponent range), unsigned, 4 exponent and 4 mantissa bits:
-//                           u44(c) = c for c < 16, else (16 + c % 16) 2^(c / 16 - 1); er = floor(log2 max r) - 17, so codes end at 240; 255 is NaN
+//                           u44(c) = c for c < 16, else (16 + c % 16) 2^(c / 16 - 1); er = floor(log2 max r) - 17, so codes end at 240; 254 is infinity, 255 NaN
 // Both formats are floating, so a power-of-two scale costs no precision, multiplies exactly, and a block whose scale changes keeps every value on its grid.
 // r is rounded up or down by a threshold u(i, t) = frac(i a1 + t a2), (a1, a2) = the 2-D additive recurrence of the plastic number (1 / 1.3247.., 1 / 1.3247..^2):
 // equidistributed over the elements of a step and over the steps of an element. Rounding to nearest would freeze r: with beta2 = 0.999 a step moves it by
@@ -12,7 +12,8 @@
 // fast for a recurrence to be independent of what it meets). To nearest, which a step without that flag does, is the closest code for ONE step, but over a run m stands still wherever
 // (1 - beta1) |g - m| is below half a grid step: a constant gradient is held at 0.78 / 0.54 / 0.20 of its value (beta1 0.9 / 0.95 / 0.99), and what is left of a gradient that has
 // stopped never goes, while r under it decays: a step of lr and more for ever. The thresholds cost 1 - 7 % of the fp32 step and 8 - 15 % of the bf16 step. mtl_adam8_quantize, which rounds once and feeds nothing back, takes the nearest code.
-// r > 0 never gets code 0 (m / (0 + eps) would explode); what is not finite becomes the NaN code of that element alone.
+// r > 0 never gets code 0 (m / (0 + eps) would explode); what is not finite becomes the NaN code of that element alone, but for a second moment that a finite gradient takes beyond
+// fp32's range (|g| > 1.8e19): infinity, as with 32-bit moments (its parameter stands still).
 //
 // Every operation is ONE fp32 operation, rounded to nearest, in the order written (no contraction into fma, exact division and square root): a change in the last bit moves
 // a value that sits at a rounding border to the next code, and this way the codes are a function of the inputs that any IEEE machine reproduces bit for bit.
@@ -80,7 +81,7 @@ __device__ __forceinline__ void decode4(uint32_t cm, uint32_t cr, int em, int er
     const float sm = pow2i(em);
     m[0] = __builtin_amdgcn_cvt_f32_fp8((int)cm, 0) * sm; m[1] = __builtin_amdgcn_cvt_f32_fp8((int)cm, 1) * sm;
     m[2] = __builtin_amdgcn_cvt_f32_fp8((int)cm, 2) * sm; m[3] = __builtin_amdgcn_cvt_f32_fp8((int)cm, 3) * sm;
-    if (!__any(has_zero_byte(cr & 0xf0f0f0f0u) || has_zero_byte(~cr))) {      // no code below 16, no 255
+    if (!__any(has_zero_byte(cr & 0xf0f0f0f0u) || has_zero_byte(~cr & 0xfefefefeu))) {      // no code below 16, no 254 or 255
         const uint32_t k = (uint32_t)(130 * 16 + 16 * er);
 #pragma unroll
         for (int e = 0; e < 4; ++e) r[e] = __uint_as_float((((cr >> (8 * e)) & 0xffu) + k) << 19);
@@ -91,18 +92,19 @@ __device__ __forceinline__ void decode4(uint32_t cm, uint32_t cr, int em, int er
     for (int e = 0; e < 4; ++e) {
         const uint32_t c = (cr >> (8 * e)) & 0xffu;
         float v = c < 16u ? (float)c : __uint_as_float((c + 130u * 16u) << 19);
-        v = c == 255u ? __uint_as_float(0x7fc00000u) : v;
+        v = c >= 254u ? __uint_as_float(c == 254u ? INF_BITS : 0x7fc00000u) : v;
         r[e] = v * sr;
     }
 }
 
-__device__ __forceinline__ uint32_t encode_root(float r, float inv, uint32_t u) {
+__device__ __forceinline__ uint32_t encode_root(float r, float m, float inv, uint32_t u) {
     const float y = r * inv;
     const uint32_t large = ((__float_as_uint(y) + (u >> 13)) >> 19) - 130u * 16u;
     const uint32_t small = (uint32_t)__builtin_floorf(y + (float)(u >> 8) * 0x1p-24f);
     uint32_t c = y >= 16.0f ? large : small;
     c = (r > 0.f && c < 1u) ? 1u : c;
-    return (__float_as_uint(r) & INF_BITS) == INF_BITS ? 255u : c;
+    if ((__float_as_uint(r) & INF_BITS) != INF_BITS) return c;
+    return __float_as_uint(r) == INF_BITS && (__float_as_uint(m) & INF_BITS) != INF_BITS ? 254u : 255u;
 }
 
 // square root, rounded to nearest, of 0 and of x >= 2^-96: the hardware's estimate is off by at most one unit in the last place; the residuals of its two neighbours decide
@@ -150,7 +152,7 @@ __device__ __forceinline__ void encode4(const float (&m)[4], const float (&v)[4]
         em = scale_exp(row_max(tm), 7); er = scale_exp(row_max(tr), 17);
         cr = 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) cr |= encode_root(r[e], pow2i(-er), u0 + (uint32_t)e * DITHER_I) << (8 * e);
+        for (int e = 0; e < 4; ++e) cr |= encode_root(r[e], m[e], pow2i(-er), u0 + (uint32_t)e * DITHER_I) << (8 * e);
     } else {
         const uint32_t k = (uint32_t)(130 * 16 + 16 * er);
         cr = 0;

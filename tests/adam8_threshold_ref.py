@@ -7,6 +7,8 @@ from helpers import drop_u16
 
 F = np.float32
 M_STREAM = 0x6D38
+ROOT = A8.ROOT.copy()
+ROOT[254] = np.inf              # the root of a second moment beyond fp32's range
 
 
 def m_thresholds(n, step, first=0):
@@ -40,7 +42,12 @@ def encode(m, r, step, first=0):
     x = np.concatenate([m.reshape(-1), np.zeros(pad, F)]).astype(F).reshape(-1, A8.BLOCK)
     with np.errstate(invalid="ignore", over="ignore"):
         y = (x * (F(2) ** (-ex[:, 0].astype(np.int64)).astype(F))[:, None]).reshape(-1)
-    return encode_e4m3(y, m_thresholds(y.size, step, first))[:n], cr, ex
+    return encode_e4m3(y, m_thresholds(y.size, step, first))[:n], overflowed(cr, m, r), ex
+
+
+def overflowed(cr, m, r):
+    """root codes: infinity where the root is infinite and the first moment is not"""
+    return np.where(np.isposinf(r) & np.isfinite(m), 254, cr).astype(np.uint8)
 
 
 def step(p, g, codes, t, lr, b1, b2, eps, wd=0.0, decoupled=False, first=0):
@@ -50,9 +57,9 @@ def step(p, g, codes, t, lr, b1, b2, eps, wd=0.0, decoupled=False, first=0):
     def keep(m, r, t, nearest=False):
         kept["m"], kept["r"] = m, r
         return None
-    before, A8.encode = A8.encode, keep
+    before, A8.encode, A8.ROOT = (A8.encode, A8.ROOT), keep, ROOT
     try:
         p, _ = A8.step(p, g, codes, t, lr, b1, b2, eps, wd, decoupled)
     finally:
-        A8.encode = before
+        A8.encode, A8.ROOT = before
     return p, encode(kept["m"], kept["r"], t, first)

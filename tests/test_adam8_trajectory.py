@@ -100,3 +100,22 @@ def test_adam8_step_refuses_another_rounding():
     with pytest.raises(ValueError):
         optim.adam8_step([p], [g], [optim.adam8_state(p)], 1, first_moment="up")
     assert N.lib().mtl_adam8_step(None, 0, 1e-3, 0.9, 0.999, 1e-8, 0.0, 4, 1, None) == -1 and N.lib().mtl_adam8_step(None, 0, 1e-3, 0.9, 0.999, 1e-8, 0.0, 3, 1, None) == 0
+
+
+def test_gradient_whose_square_overflows():
+    """one finite gradient beyond 1.8e19: the second moment is infinite from there on and the parameter stands still (as with 32-bit moments); its neighbours go on"""
+    g = np.random.RandomState(5)
+    p, codes = np.zeros(128, np.float32), (np.zeros(128, np.uint8), np.zeros(128, np.uint8), np.zeros((2, 2), np.int8))
+    for t in range(1, 31):
+        x = g.randn(128).astype(np.float32)
+        if t == 10:
+            x[3], x[70], held = 1e20, -3e38, p[[3, 70]]
+        p, codes = T8.step(p, x, codes, t, LR, 0.9, 0.999, 1e-8)
+        if t >= 10:
+            assert np.array_equal(p[[3, 70]], held) and codes[1][3] == 254 and codes[1][70] == 254
+    assert np.isfinite(p).all()
+    old = (np.zeros(64, np.uint8), np.zeros(64, np.uint8), np.zeros((1, 2), np.int8))           # with every root that is not finite as NaN the parameter is lost
+    q = np.zeros(64, np.float32)
+    for x in (np.full(64, 1e20, np.float32), np.ones(64, np.float32)):
+        q, old = A8.step(q, x, old, 1, LR, 0.9, 0.999, 1e-8)
+    assert np.isnan(q).all()

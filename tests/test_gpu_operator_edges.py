@@ -109,3 +109,41 @@ def test_hip_adam_8_takes_thresholds(optim):
         else:
             optim.adam8_step([other], [p.grad], [so], t, lr=1e-2, first_moment="nearest")
     assert torch.equal(p, ref) and torch.equal(opt.state[p]["exp_avg_q"], st.exp_avg) and not torch.equal(other, ref)
+
+
+# ================================================================================================ ends of the range
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_adam8_gradient_whose_square_overflows(optim, dt):
+    """finite gradients beyond 1.8e19: parameters finite and where torch's Adam leaves them, codes as the restatement's; infinities and NaN still make their own element NaN"""
+    g = gen(6)
+    n = 4099
+    p = randn(g, n, dtype=dt)
+    q = p.float().clone().requires_grad_()
+    wide = torch.optim.Adam([q], lr=1e-2)
+    st = optim.adam8_state(p)
+    huge = torch.tensor([0, 5, 64, 1000, 1001, n - 1], device="cuda")
+    wp, wc = np_of(p), codes_of(st)
+    for t in range(1, 9):
+        gr = randn(g, n, dtype=dt)
+        if t == 3:
+            gr[huge] = torch.tensor([1e20, -1e20, 3e38, -3e38, 2e19, 1e30], device="cuda").to(dt)
+            held = p[huge].clone()
+        if t == 6:
+            gr[7], gr[900] = float("inf"), float("nan")
+        q.grad = gr.float()
+        wide.step()
+        optim.adam8_step([p], [gr], [st], t, lr=1e-2, first_moment="threshold")
+        wp, wc = T8.step(wp, np_of(gr), wc, t, 1e-2, 0.9, 0.999, 1e-8)
+        if dt == BF16:
+            wp = torch.from_numpy(wp).to(BF16).float().numpy()
+        assert np.array_equal(np_of(p), wp, equal_nan=True) and all(np.array_equal(a, b) for a, b in zip(codes_of(st), wc)), t
+        if t >= 3:
+            assert torch.equal(p[huge], held) and bool((st.exp_avg_sq[huge] == 254).all()), t
+            if dt == F32:
+                fixed = q.detach()[huge] if t == 3 else fixed
+                assert torch.equal(q.detach()[huge], fixed)
+    assert p.isnan().nonzero().view(-1).tolist() == [7, 900] == q.isnan().nonzero().view(-1).tolist()
+    (m, v), = optim.adam8_moments([st])
+    assert bool(v[huge].isposinf().all()) and bool(m[huge].isfinite().all())
+    back = optim.adam8_quantize(m, v, 8)
+    assert torch.equal(back.exp_avg_sq[huge], st.exp_avg_sq[huge])
