@@ -183,9 +183,19 @@ class HipAdam(torch.optim.Optimizer):
             torch.cuda.current_stream().wait_event(self._late_done)
             self._late_done = None
 
+    def _after_deferred(self):
+        """the current stream waits for the deferred updates, whose event stays for the stream that reads the parameters: whoever reads or replaces the optimiser's state comes here first"""
+        if self._late_done is not None:
+            torch.cuda.current_stream().wait_event(self._late_done)
+
+    def state_dict(self):
+        self._after_deferred()
+        return super().state_dict()
+
     def load_state_dict(self, state_dict):
         """torch's Optimizer.load_state_dict casts every floating-point state tensor to its parameter's dtype; the moments of bf16 parameters
         (setup.dtype = "bf16") must stay fp32 — the kernel reads and writes them as float*."""
+        self._after_deferred()
         super().load_state_dict(state_dict)
         # (re-widening the narrowed copies would keep their bf16 rounding: take the moments from the saved tensors themselves)
         mine = [p for g in self.param_groups for p in g["params"]]
@@ -202,11 +212,12 @@ class HipAdam(torch.optim.Optimizer):
                     self.state[p][k] = rec[k].detach().to(device=p.device).contiguous().clone()
 
     def moments(self, dtype=torch.float32):
-        """{parameter: (exp_avg, exp_avg_sq)} of every parameter that has been stepped, whatever width they are held in"""
+        """{parameter: (exp_avg, exp_avg_sq)} of every parameter that has been stepped, whatever width they are held in: copies, as of the last step, its deferred updates among it"""
+        self._after_deferred()
         held = {p: st for p, st in self.state.items() if st}
         coded = [p for p, st in held.items() if _STATE8[0] in st]
         out = dict(zip(coded, adam8_moments([Adam8State(*(held[p][k] for k in _STATE8)) for p in coded], dtype)))
-        return {p: out[p] if p in out else (st["exp_avg"].to(dtype), st["exp_avg_sq"].to(dtype)) for p, st in held.items()}
+        return {p: out[p] if p in out else (st["exp_avg"].to(dtype, copy=True), st["exp_avg_sq"].to(dtype, copy=True)) for p, st in held.items()}
 
     def _to_width(self, st, p):
         """a state at the optimiser's own width: new, or converted from what a checkpoint of the other width held"""

@@ -147,3 +147,39 @@ def test_adam8_gradient_whose_square_overflows(optim, dt):
     assert bool(v[huge].isposinf().all()) and bool(m[huge].isfinite().all())
     back = optim.adam8_quantize(m, v, 8)
     assert torch.equal(back.exp_avg_sq[huge], st.exp_avg_sq[huge])
+
+
+# ================================================================================================ state read beside a running update
+@pytest.mark.parametrize("bits", [8, 32])
+def test_moments_read_behind_a_deferred_step(optim, bits):
+    """moments() and state_dict() right after a step whose update still waits on the side stream (held back there by a long kernel) give the state behind it; moments() are copies"""
+    g = gen(21)
+    ps = [randn(g, 700, 501).requires_grad_(), randn(g, 70).requires_grad_()]
+    qs = [p.detach().clone().requires_grad_() for p in ps]
+    one, two = optim.HipAdam(ps, lr=1e-2, state_bits=bits), optim.HipAdam(qs, lr=1e-2, state_bits=bits)
+    two.defer(qs)
+    for t in range(4):
+        for p, q in zip(ps, qs):
+            p.grad = randn(g, *p.shape)
+            q.grad = p.grad.clone()
+        one.step()
+        want = one.moments()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(two._side):
+            torch.cuda._sleep(20_000_000)                       # (some 10 ms)
+        two.step()
+        if t % 2:
+            got = two.moments()
+        else:
+            sd = two.state_dict()["state"]
+            names = ("exp_avg_q", "exp_avg_sq_q") if bits == 8 else ("exp_avg", "exp_avg_sq")
+            got = {q: tuple(sd[i][k].clone() for k in names) for i, q in enumerate(qs)}
+            want = {p: tuple(one.state[p][k] for k in names) for p in ps}
+        assert two._late_done is not None                       # (still there for the stream that reads the parameters)
+        assert all(torch.equal(a, b) for p, q in zip(ps, qs) for a, b in zip(want[p], got[q])), t
+        two.wait_deferred()
+    m = two.moments()[qs[0]][0]
+    before = m.clone()
+    two.step()
+    two.wait_deferred()
+    assert torch.equal(m, before) and not torch.equal(two.moments()[qs[0]][0], before)
