@@ -220,14 +220,20 @@ class HipAdam(torch.optim.Optimizer):
         return {p: out[p] if p in out else (st["exp_avg"].to(dtype, copy=True), st["exp_avg_sq"].to(dtype, copy=True)) for p, st in held.items()}
 
     def _to_width(self, st, p):
-        """a state at the optimiser's own width: new, or converted from what a checkpoint of the other width held"""
+        """a state at the optimiser's own width: new, or converted from what a checkpoint of the other width held (which goes only once the conversion is done)"""
+        wide = ("exp_avg", "exp_avg_sq")
         if self.state_bits == 8 and _STATE8[0] not in st:
-            new = adam8_quantize(st.pop("exp_avg"), st.pop("exp_avg_sq"), st["step"]) if "exp_avg" in st else adam8_state(p)
-            st.update(zip(_STATE8, new))
-        elif self.state_bits == 32 and "exp_avg" not in st:
+            st.update(zip(_STATE8, adam8_quantize(*(st[k] for k in wide), st["step"]) if wide[0] in st else adam8_state(p)))
+            old = wide
+        elif self.state_bits == 32 and wide[0] not in st:
             # moments are fp32 also for bf16 parameters (setup.dtype = "bf16"): the update is formed in fp32 and the parameter rounded once
-            st["exp_avg"], st["exp_avg_sq"] = (adam8_moments([Adam8State(*(st.pop(k) for k in _STATE8))])[0] if _STATE8[0] in st else
-                                               [torch.zeros_like(p, dtype=torch.float32, memory_format=torch.contiguous_format) for _ in range(2)])
+            st.update(zip(wide, adam8_moments([Adam8State(*(st[k] for k in _STATE8))])[0] if _STATE8[0] in st else
+                          [torch.zeros_like(p, dtype=torch.float32, memory_format=torch.contiguous_format) for _ in range(2)]))
+            old = _STATE8
+        else:
+            return
+        for k in old:
+            st.pop(k, None)
 
     @torch.no_grad()
     def step(self, closure=None):

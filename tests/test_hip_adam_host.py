@@ -36,3 +36,18 @@ def test_moments_are_copies():
     opt.state[p]["exp_avg"].zero_()
     opt.state[p]["exp_avg_sq"].zero_()
     assert bool((m == 1).all()) and bool((v == 1).all())
+
+
+def test_a_failed_change_of_width_keeps_the_state():
+    """(here: for want of a GPU) the moments are still there afterwards"""
+    from med_ts_llm_amd.hip import _native as N
+    from med_ts_llm_amd.hip.optim import HipAdam, adam8_state
+    p = torch.nn.Parameter(torch.zeros(5))
+    narrow, wide = HipAdam([p], state_bits=8), HipAdam([p])
+    narrow.state[p].update(step=1, exp_avg=torch.ones(5), exp_avg_sq=torch.ones(5))
+    wide.state[p].update(step=1, **dict(zip(("exp_avg_q", "exp_avg_sq_q", "q_exp"), adam8_state(p))))
+    for opt in (narrow, wide):
+        held = dict(opt.state[p])
+        with pytest.raises(N.MtlError):
+            opt._to_width(opt.state[p], p)
+        assert opt.state[p].keys() == held.keys() and all(opt.state[p][k] is held[k] for k in held)
