@@ -407,6 +407,7 @@ def assemble_bwd(dh0, n_tok, drop=(0.0, 0)):
 # ---- token table: lookup with scaling, gradient by sorted tokens
 # (The checks of these entry points are one condition on the way through; what is wrong is worked out only where it fails: the calls are short enough for the host's time to count.)
 _TYPES = {F32: N.MTL_F32, BF16: N.MTL_BF16}
+_wrote = torch.autograd.graph.increment_version      # of a caller's tensor written through its pointer: for autograd that is an in-place operation
 _ID_TYPES = {torch.int32: 0, torch.int64: 1}
 
 
@@ -482,7 +483,10 @@ def embedding_bwd(dout, ids, V, scale=1.0, padding_idx=None, out=None, accumulat
         if a0 < b1 and b0 < a1:
             raise ValueError("embedding_bwd: out and dout share memory")
     _req_gpu(rows, flat, *(() if out is None else (out,)))
-    return _embedding_bwd(rows, ld_rows, flat, n, V, d, scale, padding_idx, out, ld, accumulate, out_dtype)
+    grad = _embedding_bwd(rows, ld_rows, flat, n, V, d, scale, padding_idx, out, ld, accumulate, out_dtype)
+    if out is not None:
+        _wrote(out)
+    return grad
 
 
 def _embedding_bwd(rows, ld_rows, flat, n, V, d, scale, padding_idx, out, ld, accumulate, out_dtype):
@@ -589,6 +593,8 @@ def _qk_fwd(q, k, wq, wk, cos, sin, Hq, Hkv, D, eps, positions, pos0, out=None):
         a.q_out, a.k_out = qo.data_ptr(), ko.data_ptr()
         (a.qo_bs, a.qo_ts, _), (a.ko_bs, a.ko_ts, _) = qo.stride(), ko.stride()
         check(lib().mtl_qk_norm_rope_fwd(C.byref(a), stream()), "mtl_qk_norm_rope_fwd")
+    if out is not None:
+        _wrote(out)
     return qo, ko, a, keep
 
 
@@ -621,6 +627,8 @@ def _qk_bwd(dq_out, dk_out, a, keep, want_dw, out=None):
             dwq, dwk = torch.empty_like(wq, dtype=F32), torch.empty_like(wk, dtype=F32)
             a.dwq, a.dwk, a.workspace, a.workspace_bytes = dwq.data_ptr(), dwk.data_ptr(), ws.data_ptr(), nbytes
         check(lib().mtl_qk_norm_rope_bwd(C.byref(a), stream()), "mtl_qk_norm_rope_bwd")
+    if out is not None:
+        _wrote(out)
     return dq, dk, dwq, dwk
 
 

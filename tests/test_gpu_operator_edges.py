@@ -183,3 +183,24 @@ def test_moments_read_behind_a_deferred_step(optim, bits):
     two.step()
     two.wait_deferred()
     assert torch.equal(m, before) and not torch.equal(two.moments()[qs[0]][0], before)
+
+
+# ================================================================================================ views and versions of what is written
+def test_overwriting_what_a_backward_pass_needs_is_noticed(ops):
+    """queries that QkNormRopeFn saved, rotated in place afterwards, and a table gradient written over a saved tensor: the backward pass raises instead of using the new values"""
+    g = gen(30)
+    a = torch.arange(8, device="cuda", dtype=F32)[:, None] * torch.ones(16, device="cuda")
+    w, cos, sin = torch.ones(16, device="cuda"), a.cos(), a.sin()
+    q, k = randn(g, 2, 8, 64).requires_grad_(), randn(g, 2, 8, 32)
+    x = q * 1.0
+    y, _ = ops.QkNormRopeFn.apply(x, k, w, w, cos, sin, 4, 2, 16)
+    with torch.no_grad():
+        ops.qk_norm_rope_fwd(x, k, w, w, cos, sin, 4, 2, 16, out=(x, k))
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.sum().backward()
+    table = randn(g, 20, 8).requires_grad_()
+    t = table * 1.0
+    z = (t * t).sum()
+    ops.embedding_bwd(randn(g, 5, 8), torch.arange(5, device="cuda"), 20, out=t.detach())
+    with pytest.raises(RuntimeError, match="inplace"):
+        z.backward()
