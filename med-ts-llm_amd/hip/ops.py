@@ -9,6 +9,7 @@ import ctypes as C
 import math
 import os
 
+import numpy as np
 import torch
 
 from . import _native as N
@@ -427,6 +428,35 @@ def _rows(x, d):
     return x if (d == 1 or cs == 1) and (n <= 1 or rs >= d) else x.contiguous()
 
 
+def _span(dims, size):
+    return sum((n - 1) * st for n, st in dims) + size
+
+
+def _apart(a, b):
+    """whether no byte of a belongs to b: both of unit inner stride"""
+    sa, sb = a.untyped_storage(), b.untyped_storage()
+    a0, b0 = sa.data_ptr(), sb.data_ptr()
+    if b0 >= a0 + sa.nbytes() or a0 >= b0 + sb.nbytes() or a.numel() == 0 or b.numel() == 0:
+        return True
+    (a0, ad, aw), (b0, bd, bw) = ((t.data_ptr(), [(n, st * t.element_size()) for n, st in zip(t.shape[:-1], t.stride()[:-1]) if n > 1 and st], t.shape[-1] * t.element_size()) for t in (a, b))
+    if b0 >= a0 + _span(ad, aw) or a0 >= b0 + _span(bd, bw):
+        return True
+    # The strides from `cut` on are multiples of their greatest common divisor P; what is inside them spans less than P, side by side: the columns of one buffer, the parts of one arena per sequence
+    for cut in sorted({st for _, st in ad + bd}):
+        P = math.gcd(*(st for _, st in ad + bd if st >= cut))
+        wa, wb = (_span([d for d in dims if d[1] < cut], w) for dims, w in ((ad, aw), (bd, bw)))
+        off = (b0 - a0) % P
+        if wa <= off and off + wb <= P:
+            return True
+    rows = []                                                   # what remains: row by row
+    for at, dims in ((a0, ad), (b0, bd)):
+        r = np.array([at], dtype=np.int64)
+        for n, st in dims:
+            r = (r[:, None] + np.arange(n, dtype=np.int64) * st).reshape(-1)
+        rows.append(np.sort(r))
+    return not bool((np.searchsorted(rows[1], rows[0] - bw, "right") < np.searchsorted(rows[1], rows[0] + aw, "left")).any())
+
+
 def _ids(ids):
     if ids.dtype not in _ID_TYPES:
         raise ValueError(f"embedding: ids must be int32 or int64, got {ids.dtype}")
@@ -477,11 +507,8 @@ def embedding_bwd(dout, ids, V, scale=1.0, padding_idx=None, out=None, accumulat
     flat, rows = _ids(ids), _rows(dout, d)
     n = rows.shape[0]
     ld_rows = rows.stride(0) if n > 1 else d
-    if out is not None and n:
-        a0, b0 = out.data_ptr(), rows.data_ptr()
-        a1, b1 = a0 + ((V - 1) * ld + d) * out.element_size(), b0 + ((n - 1) * ld_rows + d) * rows.element_size()
-        if a0 < b1 and b0 < a1:
-            raise ValueError("embedding_bwd: out and dout share memory")
+    if out is not None and not _apart(out, rows):
+        raise ValueError("embedding_bwd: out and dout share memory")
     _req_gpu(rows, flat, *(() if out is None else (out,)))
     grad = _embedding_bwd(rows, ld_rows, flat, n, V, d, scale, padding_idx, out, ld, accumulate, out_dtype)
     if out is not None:
@@ -553,7 +580,7 @@ def _row_views(t, like, name):
 
 
 def _same_view(a, b):
-    return a.data_ptr() == b.data_ptr() and a.stride() == b.stride()
+    return a.data_ptr() == b.data_ptr() and all(x == y for n, x, y in zip(a.shape, a.stride(), b.stride()) if n > 1)
 
 
 def _check_qk_outputs(q, k, out):
@@ -561,14 +588,10 @@ def _check_qk_outputs(q, k, out):
     qo, ko = out
     _row_views(qo, q, "the query output")
     _row_views(ko, k, "the key output")
-    ins = {t.untyped_storage().data_ptr() for t in (q, k)}
-    for o, own in ((qo, q), (ko, k)):
-        _req(o.untyped_storage().data_ptr() not in ins or _same_view(o, own), "qk_norm_rope: an output in an input's memory must be that input itself (in place)")
-    for a, b in ((q, k), (qo, ko)) if any(o.untyped_storage().data_ptr() in ins for o in out) else ((qo, ko),):
-        if a.untyped_storage().data_ptr() == b.untyped_storage().data_ptr():      # two column ranges of one buffer: apart in every row
-            ts, off = a.stride(1), (b.data_ptr() - a.data_ptr()) // a.element_size()
-            _req(a.stride() == b.stride() and ts > 0 and off % ts >= a.shape[2] and off % ts <= ts - b.shape[2] and (a.shape[0] <= 1 or a.stride(0) % ts == 0),
-                 "qk_norm_rope: queries and keys in one buffer have to be separate column ranges of it")
+    here = [_same_view(qo, q), _same_view(ko, k)]
+    for o, own, other, same in ((qo, q, k, here[0]), (ko, k, q, here[1])):
+        _req((same or _apart(o, own)) and (all(here) or _apart(o, other)), "qk_norm_rope: an output in an input's memory must be that input itself (in place)")
+    _req(_apart(qo, ko), "qk_norm_rope: the outputs share memory")
 
 
 def _new(t):
@@ -607,9 +630,8 @@ def qk_norm_rope_bwd(dq_out, dk_out, q, k, wq, wk, cos, sin, Hq, Hkv, D, eps=1e-
     if dq_out.stride(2) != 1 or dk_out.stride(2) != 1:
         dq_out, dk_out = dq_out.contiguous(), dk_out.contiguous()
     if out is not None:
-        ins = {t.untyped_storage().data_ptr() for t in (q, k)}
-        _req(all(o.untyped_storage().data_ptr() not in ins for o in out), "qk_norm_rope_bwd: out must not share memory with q or k")
         _check_qk_outputs(dq_out, dk_out, out)
+        _req(all(_apart(o, t) for o in out for t in (q, k)), "qk_norm_rope_bwd: out must not share memory with q or k")
     _req_gpu(*keep, dq_out, dk_out, *(out or ()))
     return _qk_bwd(dq_out, dk_out, a, keep, want_dw, out)
 

@@ -204,3 +204,30 @@ def test_overwriting_what_a_backward_pass_needs_is_noticed(ops):
     ops.embedding_bwd(randn(g, 5, 8), torch.arange(5, device="cuda"), 20, out=t.detach())
     with pytest.raises(RuntimeError, match="inplace"):
         z.backward()
+
+
+def test_qk_norm_rope_out_of_one_allocation(ops):
+    """queries and a key cache in one arena, one part per sequence; outputs beside the inputs in their own buffer: the same values, nothing else touched"""
+    g = gen(31)
+    B, Hq, Hkv, D, L = 3, 4, 2, 64, 9
+    a = torch.arange(L, device="cuda", dtype=F32)[:, None] * torch.logspace(0, -2, 64, device="cuda")
+    cos, sin, w = a.cos(), a.sin(), 1 + randn(g, D, std=0.1)
+    q, k = randn(g, B, 1, Hq * D, dtype=BF16), randn(g, B, 1, Hkv * D, dtype=BF16)
+    yq, yk = ops.qk_norm_rope_fwd(q, k, w, w, cos, sin, Hq, Hkv, D, pos0=5)
+    arena = torch.full((B, Hq * D + L * Hkv * D), 7.0, dtype=BF16, device="cuda")
+    to = arena[:, None, :Hq * D], arena[:, Hq * D:].unflatten(1, (L, Hkv * D))[:, 5:6]
+    ops.qk_norm_rope_fwd(q, k, w, w, cos, sin, Hq, Hkv, D, pos0=5, out=to)
+    assert torch.equal(to[0], yq) and torch.equal(to[1], yk)
+    to[0].fill_(7.0), to[1].fill_(7.0)
+    assert bool((arena == 7.0).all())
+    fused = randn(g, B, L, 2 * (Hq + Hkv) * D)
+    kept = fused.clone()
+    q, k = fused[..., :Hq * D], fused[..., Hq * D:(Hq + Hkv) * D]
+    want = ops.qk_norm_rope_fwd(q, k, w, w, cos, sin, Hq, Hkv, D)
+    to = fused[..., (Hq + Hkv) * D:(2 * Hq + Hkv) * D], fused[..., (2 * Hq + Hkv) * D:]
+    ops.qk_norm_rope_fwd(q, k, w, w, cos, sin, Hq, Hkv, D, out=to)
+    assert torch.equal(to[0], want[0]) and torch.equal(to[1], want[1]) and torch.equal(fused[..., :(Hq + Hkv) * D], kept[..., :(Hq + Hkv) * D])
+    dq, dk = randn(g, B, L, Hq * D), randn(g, B, L, Hkv * D)
+    want = ops.qk_norm_rope_bwd(dq, dk, q, k, w, w, cos, sin, Hq, Hkv, D)
+    got = ops.qk_norm_rope_bwd(dq, dk, q, k, w, w, cos, sin, Hq, Hkv, D, out=to)
+    assert all(torch.equal(x, y) for x, y in zip(got, want)) and torch.equal(fused[..., :(Hq + Hkv) * D], kept[..., :(Hq + Hkv) * D])

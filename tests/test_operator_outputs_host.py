@@ -55,3 +55,72 @@ def test_rotation_in_place_of_a_saved_tensor_is_noticed(ops):
         ops.qk_norm_rope_fwd(x, k, *rest, out=(x, k))
     with pytest.raises(RuntimeError, match="inplace"):
         y.backward()
+
+
+# ---------------------------------------------------------------- shared memory
+def elements(t):
+    return set(torch.arange(t.untyped_storage().nbytes() // t.element_size()).as_strided(t.shape, t.stride(), t.storage_offset()).reshape(-1).tolist())
+
+
+def test_apart_is_what_the_elements_say(ops):
+    """random views of one buffer: rows, columns, batches, orders, broadcast dimensions; the answer is exact"""
+    import random
+    rng = random.Random(1)
+    buf = torch.zeros(6000)
+    seen = [0, 0]
+    for _ in range(4000):
+        views = []
+        for _ in range(2):
+            B, T, W = rng.randint(1, 4), rng.randint(1, 5), rng.randint(1, 9)
+            strides = [rng.choice([0, W, W + 3, 16, 40, 48, 60, 100, 240]) for _ in range(2)]
+            views.append(buf.as_strided((B, T, W), (*strides, 1), rng.randint(0, 300)))
+        a, b = views
+        want = not (elements(a) & elements(b))
+        assert ops._apart(a, b) == want == ops._apart(b, a), [(v.shape, v.stride(), v.storage_offset()) for v in views]
+        seen[want] += 1
+    assert min(seen) > 500
+    assert ops._apart(buf[:0], buf) and ops._apart(buf[:10], buf[10:]) and not ops._apart(buf[:10], buf[9:])
+
+
+def test_outputs_and_inputs_out_of_one_allocation(ops):
+    """a query output and a key cache carved from one arena, an output beside the inputs in their own buffer: taken where no element is shared"""
+    q, k, *rest = qk(B=2, T=1)
+    arena = torch.zeros(2 * 16 + 2 * 10 * 8 * 2)
+    new_q, cache = arena[:32].view(2, 1, 16), arena[32:].view(2, 10, 2, 8)
+    ops.qk_norm_rope_fwd(q, k, *rest, out=(new_q, cache[:, 4:5, 0]))
+    per_sequence = torch.zeros(2, 16 + 10 * 8)                     # [query | its cache] of every sequence
+    ops.qk_norm_rope_fwd(q, k, *rest, out=(per_sequence[:, None, :16], per_sequence[:, 16:].view(2, 10, 8)[:, 4:5]))
+    fused = torch.zeros(2, 3, 64)
+    q, k, *rest = qk()
+    q, k = fused[..., :16], fused[..., 16:24]
+    ops.qk_norm_rope_fwd(q, k, *rest, out=(q, k))                  # in place
+    ops.qk_norm_rope_fwd(q, k, *rest, out=(q, fused[..., 24:32]))   # the queries in place, the keys beside them
+    ops.qk_norm_rope_fwd(q, k, *rest, out=(fused[..., 32:48], fused[..., 48:56]))
+    one = fused[:1, :1]
+    ops.qk_norm_rope_fwd(one[..., :16], one[..., 16:24], *rest, out=(one.as_strided((1, 1, 16), (16, 16, 1)), one[..., 16:24]))      # the same row under other strides
+    dq, dk = torch.zeros(2, 3, 16), torch.zeros(2, 3, 8)
+    ops.qk_norm_rope_bwd(dq, dk, q, k, *rest, out=(fused[..., 32:48], fused[..., 48:56]))
+    both = torch.zeros(30, 16)
+    ops.embedding_bwd(both[:3, 8:], torch.zeros(3, dtype=torch.int64), 30, out=both[:, :8])
+
+
+def test_outputs_that_share_elements_are_refused(ops):
+    q, k, *rest = qk()
+    fused = torch.zeros(2, 3, 64)
+    fq, fk = fused[..., :16], fused[..., 16:24]
+    flat = torch.zeros(400)
+    bad = [dict(q=fq, k=fk, out=(fq, fused[..., 8:16])), dict(q=fq, k=fk, out=(fk.expand(2, 3, 8).repeat(1, 1, 2), fq[..., :8])), dict(q=fq, k=fk, out=(fused[..., 8:24], fk)),
+           dict(q=fq, k=fused[..., 8:16], out=(fq, fused[..., 8:16])), dict(out=(fused[..., :16], fused[..., 15:23])),
+           dict(q=flat[:96].view(2, 3, 16), out=(flat[48:144].view(2, 3, 16), torch.zeros(2, 3, 8))),                         # the second sequence's queries where the first one's results go
+           dict(q=fq[:, :, :], k=fk, out=(fused.as_strided((2, 3, 16), (16, 64, 1)), torch.zeros(2, 3, 8))),
+           dict(out=(torch.zeros(2, 3), torch.zeros(2, 3, 8))), dict(out=(torch.zeros(()), torch.zeros(2, 3, 8)))]
+    for kw in bad:
+        out = kw.pop("out")
+        with pytest.raises(ValueError):
+            ops.qk_norm_rope_fwd(kw.get("q", q), kw.get("k", k), *rest, out=out)
+        if "q" in kw:
+            with pytest.raises(ValueError):
+                ops.qk_norm_rope_bwd(torch.zeros(2, 3, 16), torch.zeros(2, 3, 8), kw["q"], kw.get("k", k), *rest, out=out)
+    both = torch.zeros(30, 16)
+    with pytest.raises(ValueError):
+        ops.embedding_bwd(both[:3, 7:15], torch.zeros(3, dtype=torch.int64), 30, out=both[:, :8])
