@@ -165,13 +165,16 @@ class BaseTask(ABC):
             params = su.optimizer_params(params)          # owned-rows views instead of the full tensors
         lr = self.config.training.learning_rate
         opt = self.config.training.optimizer
-        if self.device.type == "cuda" and opt in ("adam", "adamw"):
+        # setup.optimizer_state_bits = 8: both moments in 8 bits (2.03 bytes of state per parameter instead of 8, 16 bytes of HBM traffic per step instead of 28). A step on a
+        # part of a tensor's rows would cut its 64-element blocks elsewhere than the whole tensor's step does: not combined with the row-sharded forms.
+        bits = int(self.config.setup.get("optimizer_state_bits", 32))
+        on_hip = self.device.type == "cuda" and opt in ("adam", "adamw")
+        if bits not in (8, 32) or (bits == 8 and not on_hip):
+            raise ValueError(f"setup.optimizer_state_bits = {bits}: 32, or 8 with optimizer adam or adamw on the GPU (here: {opt} on {self.device.type})")
+        if on_hip:
             # same update rule as torch.optim.Adam/AdamW, one streaming launch for all tensors, and the bf16 autocast
             # copy of the big mapping weight is written by the same kernel (hip/optim.py)
             from ..hip.optim import HipAdam
-            # setup.optimizer_state_bits = 8: both moments in 8 bits (2.03 bytes of state per parameter instead of 8, 16 bytes of HBM traffic per step instead of 28). A step on a
-            # part of a tensor's rows would cut its 64-element blocks elsewhere than the whole tensor's step does: not combined with the row-sharded forms.
-            bits = int(self.config.setup.get("optimizer_state_bits", 32))
             if bits != 32 and (su is not None or getattr(self.model, "_map_shard", None) is not None):
                 raise ValueError("setup.optimizer_state_bits = 8 cannot be combined with setup.shard_optimizer / setup.shard_mapping")
             o = HipAdam(params, lr=lr, weight_decay=0.01 if opt == "adamw" else 0.0, decoupled_weight_decay=opt == "adamw", state_bits=bits)

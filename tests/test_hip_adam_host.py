@@ -51,3 +51,20 @@ def test_a_failed_change_of_width_keeps_the_state():
         with pytest.raises(N.MtlError):
             opt._to_width(opt.state[p], p)
         assert opt.state[p].keys() == held.keys() and all(opt.state[p][k] is held[k] for k in held)
+
+
+@pytest.mark.parametrize("bits,optimizer,device,fine", [(8, "sgd", "cuda", False), (8, "adam", "cpu", False), (8, "adamw", "cpu", False), (16, "adam", "cuda", False), (16, "sgd", "cpu", False),
+                                                        (32, "sgd", "cuda", True), (32, "adam", "cpu", True), (None, "adamw", "cpu", True)])
+def test_the_trainer_does_not_ignore_the_width_of_its_state(bits, optimizer, device, fine):
+    from types import SimpleNamespace
+
+    from med_ts_llm_amd.tasks.base import BaseTask
+    from med_ts_llm_amd.utils import dict_to_object
+    setup = {} if bits is None else {"optimizer_state_bits": bits}
+    task = SimpleNamespace(finetuning=False, model=torch.nn.Linear(2, 2), device=torch.device(device),
+                           config=dict_to_object({"setup": setup, "training": {"learning_rate": 1e-3, "optimizer": optimizer}}))
+    if fine:
+        assert BaseTask.build_optimizer(task) is not None
+    else:
+        with pytest.raises(ValueError, match="optimizer_state_bits"):
+            BaseTask.build_optimizer(task)
