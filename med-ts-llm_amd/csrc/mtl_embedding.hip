@@ -617,6 +617,16 @@ inline int window_of(int64_t N, int64_t chunks) {
 }
 inline int64_t chunks_of(int64_t d, int W) { return (d + 64 * W - 1) / (64 * W); }
 
+// Four columns per lane; one where a row is narrower than a wave (200 003 x 64 bf16: 65.3 us, with four 67). Eight of bf16 (16 bytes) halve the waves in flight: 8192 x 2048 41.9 us against
+// 38.5 with four, 200 003 x 1024 141.5 against 139.9.
+inline int columns_of(int64_t d) { return d > 64 ? 4 : 1; }
+// ids and positions are 32 bits; the sum is one grid of less than 2^32 threads
+inline bool too_large(int64_t N, int64_t V, int64_t d) {
+    if (N > 0x7fffffff || V >= 0x7fffffff) return true;
+    const int64_t chunks = chunks_of(d, columns_of(d)), S = window_of(N, chunks);
+    return chunks >= 1 << 26 || (N + S - 1) / S * chunks >= 1 << 26;
+}
+
 struct Plan { int64_t sid, spos, sid2, spos2, hist, list, part, total; };
 inline Plan plan_for(int64_t N, int64_t V, int64_t d) {
     Plan p;
@@ -714,13 +724,15 @@ extern "C" int mtl_embedding_fwd(const void* ids, int ids_i64, int64_t N, const 
 
 extern "C" size_t mtl_embedding_bwd_workspace_bytes(int64_t N, int64_t V, int64_t d) {
     if (N <= 0 || V <= 0 || d <= 0) return 256;
+    if (too_large(N, V, d)) return 0;
     return (size_t)plan_for(N, V, d).total;
 }
 
 extern "C" int mtl_embedding_bwd(const void* ids, int ids_i64, int64_t N, const void* dout, int dout_dtype, int64_t ld_dout, int64_t V, int64_t d, int64_t padding_idx, float scale, void* grad,
                                  int grad_dtype, int64_t ld_grad, int accumulate, void* workspace, size_t workspace_bytes, void* stream) {
-    if (N < 0 || V <= 0 || d <= 0 || !grad || !dtype_ok(dout_dtype) || !dtype_ok(grad_dtype) || ld_grad < d || (N > 0 && (!ids || !dout || ld_dout < d || !workspace))) return MTL_ERR_ARG;
-    if (N > 0x7fffffff || V >= 0x7fffffff) return MTL_ERR_UNSUPPORTED;
+    if (N < 0 || V <= 0 || d <= 0 || !dtype_ok(dout_dtype) || !dtype_ok(grad_dtype) || ld_grad < d || (N > 0 && ld_dout < d)) return MTL_ERR_ARG;
+    if (too_large(N, V, d)) return MTL_ERR_UNSUPPORTED;
+    if (!grad || (N > 0 && (!ids || !dout || !workspace))) return MTL_ERR_ARG;
     if (N == 0 && accumulate) return MTL_OK;
     const int gs = size_of(grad_dtype);
     if (((uintptr_t)grad & (gs - 1)) || (N > 0 && (((uintptr_t)ids & (ids_i64 ? 7 : 3)) || ((uintptr_t)dout & (size_of(dout_dtype) - 1)) || ((uintptr_t)workspace & 15)))) return MTL_ERR_ALIGN;
@@ -741,13 +753,10 @@ extern "C" int mtl_embedding_bwd(const void* ids, int ids_i64, int64_t N, const 
         MTL_CHECK_LAUNCH();
         return MTL_OK;
     }
-    // Four columns per lane; one where a row is narrower than a wave (200 003 x 64 bf16: 65.3 us, with four 67). Eight of bf16 (16 bytes) halve the waves in flight: 8192 x 2048 41.9 us against
-    // 38.5 with four, 200 003 x 1024 141.5 against 139.9.
-    const int W = d > 64 ? 4 : 1;
+    const int W = columns_of(d);
     const int64_t chunks = chunks_of(d, W);
     const int S = window_of(N, chunks);
     const int64_t windows = (N + S - 1) / S;
-    if (chunks >= 1 << 26 || windows * chunks >= 1 << 26) return MTL_ERR_UNSUPPORTED;      // (one grid: 2^32 threads)
     const Plan p = plan_for(N, V, d);
     uint32_t* list_n = reinterpret_cast<uint32_t*>(ws);
     uint32_t* sid = reinterpret_cast<uint32_t*>(ws + p.sid);

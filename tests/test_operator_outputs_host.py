@@ -124,3 +124,18 @@ def test_outputs_that_share_elements_are_refused(ops):
     both = torch.zeros(30, 16)
     with pytest.raises(ValueError):
         ops.embedding_bwd(both[:3, 7:15], torch.zeros(3, dtype=torch.int64), 30, out=both[:, :8])
+
+
+# ---------------------------------------------------------------- sizes
+def test_token_gradient_sizes_and_their_workspace():
+    """the limit that the header states, of the call and of its workspace query alike (no pointer is followed: all are null or the call is refused)"""
+    from med_ts_llm_amd.hip import _native as N
+    lib = N.lib()
+
+    def call(n, v, d):
+        return lib.mtl_embedding_bwd(None, 1, n, None, 0, d, v, d, -1, 1.0, None, 0, d, 0, None, 0, None)
+
+    for n, v, d, fine in ((1, 5, 8, True), ((1 << 31) - 1, 5, 256, True), ((1 << 31) - 1, 5, 257, False), (1 << 31, 5, 8, False), (1, (1 << 31) - 1, 8, False), (1, (1 << 31) - 2, 8, True),
+                          ((1 << 28) - 64, 1000, 4096, True), (1 << 28, 1000, 4096, False), (1 << 30, 5, 4096, False), (128, 5, 256 * ((1 << 25) - 1), True), (128, 5, 1 << 33, False)):
+        assert call(n, v, d) == (-1 if fine else -3), (n, v, d)
+        assert (lib.mtl_embedding_bwd_workspace_bytes(n, v, d) > 0) == fine, (n, v, d)
