@@ -1,14 +1,16 @@
 #!/usr/bin/env python3
 """usage: tools/asm_loops.py <file.hip> <mangled-name substring>  -> per basic block of the kernel that contains MFMAs: instruction mix
 (compiles the device code to assembly; no GPU needed)"""
+import os
 import re
 import subprocess
 import sys
 from collections import Counter
 
+from build_flags import CSRC, cxxflags
+
 src, pat = sys.argv[1], sys.argv[2]
-subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-S", "--cuda-device-only", "-I",
-                "/root/repo/med-ts-llm_amd/csrc", src, "-o", "/tmp/_k.s"], check=True, stderr=subprocess.DEVNULL, cwd="/tmp")
+subprocess.run(["/opt/rocm/bin/hipcc", *cxxflags(), "-S", "--cuda-device-only", "-I", CSRC, os.path.abspath(src), "-o", "/tmp/_k.s"], check=True, stderr=subprocess.DEVNULL, cwd="/tmp")
 s = open("/tmp/_k.s").read()
 starts = [m for m in re.finditer(r"^(\S+):\s*(;.*)?$", s, re.M) if pat in m.group(1) and not m.group(1).startswith(".L")]
 for m in starts:

@@ -4,6 +4,8 @@ that point ("what de-pipelines an LDS-DMA loop").
 usage: python tools/asm_waits.py med-ts-llm_amd/csrc/mtl_gemm.hip [...]"""
 import re, subprocess, sys, tempfile, os
 
+from build_flags import cxxflags
+
 def demangle(names):
     out = subprocess.run(["c++filt"], input="\n".join(names), capture_output=True, text=True).stdout
     return out.split("\n")
@@ -11,7 +13,7 @@ def demangle(names):
 for src in sys.argv[1:]:
     with tempfile.TemporaryDirectory() as td:
         s = os.path.join(td, "k.s")
-        subprocess.run(["hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-S", "--cuda-device-only", src, "-o", s], check=True,
+        subprocess.run(["hipcc", *cxxflags(), "-S", "--cuda-device-only", src, "-o", s], check=True,
                        stderr=subprocess.DEVNULL)
         lines = open(s).read().split("\n")
     fn, rows, cur = None, [], None

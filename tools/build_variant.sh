@@ -9,13 +9,14 @@ case "$1" in only=*) ONLY=${1#only=}; shift;; esac
 R=$(cd "$(dirname "$0")/.." && pwd)
 OBJ=$R/build/obj_$TAG
 mkdir -p $OBJ $R/tools/diag
-ALL="mtl_gemm mtl_attention mtl_norm mtl_elementwise mtl_tokenizer mtl_backbone mtl_optim mtl_optim8 mtl_embedding mtl_qknorm mtl_stats"
+ALL=$(python3 $R/tools/build_flags.py names)
+FLAGS=$(python3 $R/tools/build_flags.py flags)
 for f in $ALL; do
   # mtl_elementwise holds mtl_build_flags(): it is always rebuilt with the variant's flags, so that the variant reports what it is
   if [ -n "$ONLY" ] && [ "$f" != mtl_elementwise ] && ! echo ",$ONLY," | grep -q ",$f,"; then
     cp $R/build/obj/$f.o $OBJ/$f.o
   else
-    hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wall -Wno-unused-function -Xclang -target-feature -Xclang -packed-fp32-ops "$@" -c $R/med-ts-llm_amd/csrc/$f.hip -o $OBJ/$f.o &
+    hipcc $FLAGS "$@" -c $R/med-ts-llm_amd/csrc/$f.hip -o $OBJ/$f.o &
   fi
 done
 wait

@@ -4,9 +4,13 @@ the cycle counts of wave 0 into the `lse` output (whose values are then meaningl
 tile 2 + epilogue, total] — tools/diag/attn_timing.py prints their distribution. Not shipped."""
 import os
 import subprocess
+import sys
 
 ROOT = os.path.dirname(os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 HERE = os.path.join(ROOT, "tools", "diag")
+sys.path.insert(0, os.path.join(ROOT, "tools"))
+from build_flags import cxxflags, objects  # noqa: E402
+
 s = open(os.path.join(ROOT, "med-ts-llm_amd", "csrc", "mtl_attention.hip")).read()
 i = s.index("__global__ __launch_bounds__(NW * 64) void attn_fwd_res_kernel")
 j = s.index("template <int D, int NW, bool DROP = false>", i)
@@ -26,9 +30,9 @@ body = body.replace("if (g == 0 && a.lse) a.lse[", "if (false) a.lse[")
 s = s[:i] + body + s[j:]
 src = os.path.join(HERE, "_attn_timing.hip")
 open(src, "w").write(s)
-objs = [os.path.join(ROOT, "build", "obj", f"mtl_{n}.o") for n in ("gemm", "norm", "elementwise", "tokenizer", "backbone", "optim")]
+objs = objects("mtl_attention")
 o = os.path.join(HERE, "_attn_timing.o")
-subprocess.run(["hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-I", os.path.join(ROOT, "med-ts-llm_amd", "csrc"), "-c", src, "-o", o], check=True, stderr=subprocess.DEVNULL)
+subprocess.run(["hipcc", *cxxflags(), "-I", os.path.join(ROOT, "med-ts-llm_amd", "csrc"), "-c", src, "-o", o], check=True, stderr=subprocess.DEVNULL)
 subprocess.run(["hipcc", "--offload-arch=gfx950", "-shared", "-fPIC", "-o", os.path.join(HERE, "libdiag_attn_timing.so"), o, *objs], check=True)
 os.remove(o); os.remove(src)
 print("built libdiag_attn_timing.so")

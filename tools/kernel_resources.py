@@ -1,13 +1,16 @@
 #!/usr/bin/env python3
 """usage: tools/kernel_resources.py <file.hip> [regex]  -> registers / scratch / occupancy / LDS per kernel, from hipcc's
 -Rpass-analysis=kernel-resource-usage remarks (cross-compiles gfx950 without a GPU)"""
+import os
 import re
 import subprocess
 import sys
 
+from build_flags import cxxflags
+
 src = sys.argv[1]
 filt = re.compile(sys.argv[2] if len(sys.argv) > 2 else ".")
-out = subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-c", src, "-o", "/tmp/_res.o",
+out = subprocess.run(["/opt/rocm/bin/hipcc", *cxxflags(), "-c", os.path.abspath(src), "-o", "/tmp/_res.o",
                       "-Rpass-analysis=kernel-resource-usage"], capture_output=True, text=True, cwd="/tmp").stderr
 cur, rows = None, {}
 for line in out.splitlines():

@@ -4,7 +4,7 @@
 //   tile   : 256 workgroups x 512 threads, one 256 x 96 tile each, the wave / lane -> (row, 4 columns) map of the GEMM's register epilogue
 //            (wave = 64 rows x 48 columns; a lane owns row l15 of each 16-row block and 4 consecutive columns per 16-column tile)
 //   tile8  : the same with the paired-column layout (8 consecutive columns per lane: two float4)
-// build: hipcc --offload-arch=gfx950 -O3 -o tools/probes/burst_floor tools/probes/burst_floor.hip ; run on the GPU box.
+// build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o tools/probes/burst_floor tools/probes/burst_floor.hip ; run on the GPU box.
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <vector>

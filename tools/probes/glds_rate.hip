@@ -1,6 +1,6 @@
 // probe: cost of one "issue N LDS-DMA loads -> s_waitcnt vmcnt(0) -> s_barrier" round per workgroup, vs N (loads per wave),
 // waves per workgroup and ring depth (loads left in flight across the barrier). Data is L2/MALL resident (16 MB window).
-// build: hipcc --offload-arch=gfx950 -O3 -o tools/probes/glds_rate tools/probes/glds_rate.hip ; run on the GPU box.
+// build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o tools/probes/glds_rate tools/probes/glds_rate.hip ; run on the GPU box.
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdint>

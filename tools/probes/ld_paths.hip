@@ -2,7 +2,7 @@
 // whole? One 512-thread workgroup per CU streams two GEMM-shaped operand panels (256 rows x 128 B per round each, row stride LD bytes,
 // L2-resident per XCD) with a two-round pipeline (counted vmcnt): MODE 0 = both panels through LDS-DMA (the GEMM kernels' way),
 // MODE 1 = both through plain global_load_dwordx4 into registers, MODE 2 = panel A into registers + panel B through LDS-DMA.
-// build: hipcc --offload-arch=gfx950 -O3 -o tools/probes/ld_paths tools/probes/ld_paths.hip ; run on the GPU box.
+// build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o tools/probes/ld_paths tools/probes/ld_paths.hip ; run on the GPU box.
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdint>
