@@ -104,8 +104,9 @@ def adam8_step(params, grads, states, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-
         read.append(g)
         if sh is not None:
             read.append(sh.tensor)
-    for name, at in (("parameter", 0), ("state", 2)):
-        ptrs = [x for x, n in zip(rows[at::10], rows[5::10]) if n]
+    held = rows[5::10]
+    for name, columns in (("parameter", (0,)), ("state", (2, 3, 4))):
+        ptrs = [x for at in columns for x, n in zip(rows[at::10], held) if n]
         if len(set(ptrs)) < len(ptrs):
             raise ValueError(f"adam8_step: the same {name} twice in one step")
     _one_gpu(touched + read, "adam8_step")

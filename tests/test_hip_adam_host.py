@@ -68,3 +68,16 @@ def test_the_trainer_does_not_ignore_the_width_of_its_state(bits, optimizer, dev
     else:
         with pytest.raises(ValueError, match="optimizer_state_bits"):
             BaseTask.build_optimizer(task)
+
+
+def test_a_part_of_a_state_twice_is_refused():
+    """codes of the first moment given as the root's too, one exponent tensor for two parameters"""
+    from med_ts_llm_amd.hip import _native as N
+    from med_ts_llm_amd.hip.optim import Adam8State, adam8_state, adam8_step
+    p, q, g = torch.zeros(70), torch.zeros(70), torch.zeros(70)
+    a, b, empty = adam8_state(p), adam8_state(q), torch.zeros(0)
+    for states in ([Adam8State(a.exp_avg, a.exp_avg, a.exponents), b], [a, Adam8State(b.exp_avg, b.exp_avg_sq, a.exponents)], [a, Adam8State(b.exp_avg, a.exp_avg, b.exponents)]):
+        with pytest.raises(ValueError, match="twice"):
+            adam8_step([p, q], [g, g], states, 1)
+    with pytest.raises(N.MtlError):                               # (sound, but on the CPU)
+        adam8_step([p, q, empty, empty], [g, g, empty, empty], [a, b, adam8_state(empty), adam8_state(empty)], 1)
