@@ -4,7 +4,7 @@ trainable tensors (`mtl_adam_step`), optionally emitting the bf16 autocast copy 
 state_dict layout matches torch.optim.Adam ("step", "exp_avg", "exp_avg_sq"), so checkpoints interchange.
 
 HipAdam(state_bits=8) holds both moments in 8 bits (`mtl_adam8_step`: 2.03 bytes of state per parameter instead of 8): state "step", "exp_avg_q", "exp_avg_sq_q" (codes of the
-parameter's shape), "q_exp" (exponents [blocks of 64, 2]). A state saved at the other width is converted at the first step after it is loaded."""
+parameter's shape), "q_exp" (exponents [blocks of 64, 2]). Both are rounded against thresholds of (step, element), so that a run of steps is right in the mean. A state saved at the other width is converted at the first step after it is loaded."""
 import collections
 import ctypes as C
 import warnings
