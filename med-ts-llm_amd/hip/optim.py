@@ -98,6 +98,8 @@ def adam8_step(params, grads, states, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-
         if n != p.numel():
             raise ValueError("adam8_step: a state of another size than its parameter")
         rows += (p.data_ptr(), g.data_ptr(), m8, r8, ex, n)
+        if sh is not None and (p.dim() != 2 or sh.tensor.shape[0] < p.shape[0] or sh.tensor.shape[1] < p.shape[1]):
+            raise ValueError("adam8_step: a bf16 copy of another parameter")
         rows += (0, 0, 0) if sh is None else (sh.tensor.data_ptr(), p.shape[1], sh.tensor.stride(0))
         rows.append(_PARAM_TYPES[dt])
         touched += (p, *st)

@@ -81,3 +81,16 @@ def test_a_part_of_a_state_twice_is_refused():
             adam8_step([p, q], [g, g], states, 1)
     with pytest.raises(N.MtlError):                               # (sound, but on the CPU)
         adam8_step([p, q, empty, empty], [g, g, empty, empty], [a, b, adam8_state(empty), adam8_state(empty)], 1)
+
+
+def test_a_bf16_copy_that_does_not_hold_its_parameter_is_refused():
+    """(the step writes [rows, cols] into it)"""
+    from med_ts_llm_amd.hip import _native as N
+    from med_ts_llm_amd.hip.optim import Bf16Shadow, adam8_state, adam8_step
+    small, wide, flat, cube = torch.zeros(3, 8), torch.zeros(6, 8), torch.zeros(24), torch.zeros(3, 4, 2)
+    copy = Bf16Shadow(small, torch.zeros(3, 16, dtype=torch.bfloat16))
+    for p in (wide, flat, cube, torch.zeros(1, 24)):
+        with pytest.raises(ValueError, match="copy"):
+            adam8_step([p], [torch.zeros_like(p)], [adam8_state(p)], 1, shadows=[copy], first_moment="threshold")
+    with pytest.raises(N.MtlError):                               # (sound, but on the CPU)
+        adam8_step([small], [torch.zeros_like(small)], [adam8_state(small)], 1, shadows=[copy], first_moment="threshold")
