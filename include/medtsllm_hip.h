@@ -465,7 +465,7 @@ int mtl_embedding_fwd(const void* ids, int ids_i64, int64_t N, const void* table
 /* grad[v, :] (+)= scale * sum over {i : ids[i] = v, v != padding_idx} of dout[i, :]. The tokens are sorted by id (stable, so a row's terms are added in one fixed order: the
  * result does not depend on how the launch is scheduled); sums in fp32, one rounding to grad_dtype. accumulate = 0 writes all V rows (zeros where no token points),
  * accumulate = 1 touches the rows that occur only. padding_idx < 0: none. N < 2^31, V < 2^31 - 1, and the sum has to fit one
- * grid: for N >= 128, ceil(N / 64) * ceil(d / 256) < 2^26 (no limit of its own for d <= 256, N < 2^28 at d = 4096). Beyond that MTL_ERR_UNSUPPORTED, and the workspace query returns 0. */
+ * grid: for N >= 128, ceil(N / 64) * ceil(d / 256) <= 2^26 - 4 (no limit of its own for d <= 256, N < 2^28 at d = 4096). Beyond that MTL_ERR_UNSUPPORTED, and the workspace query returns 0. */
 size_t mtl_embedding_bwd_workspace_bytes(int64_t N, int64_t V, int64_t d);
 int mtl_embedding_bwd(const void* ids, int ids_i64, int64_t N, const void* dout, int dout_dtype, int64_t ld_dout, int64_t V, int64_t d, int64_t padding_idx, float scale,
                       void* grad, int grad_dtype, int64_t ld_grad, int accumulate, void* workspace, size_t workspace_bytes, void* stream);

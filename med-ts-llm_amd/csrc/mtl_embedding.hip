@@ -624,7 +624,7 @@ inline int columns_of(int64_t d) { return d > 64 ? 4 : 1; }
 inline bool too_large(int64_t N, int64_t V, int64_t d) {
     if (N > 0x7fffffff || V >= 0x7fffffff) return true;
     const int64_t chunks = chunks_of(d, columns_of(d)), S = window_of(N, chunks);
-    return chunks >= 1 << 26 || (N + S - 1) / S * chunks >= 1 << 26;
+    return chunks >= 1 << 26 || (N + S - 1) / S * chunks > (1 << 26) - 4;      // (four waves per workgroup, and 2^24 workgroups would be 2^32 threads)
 }
 
 struct Plan { int64_t sid, spos, sid2, spos2, hist, list, part, total; };

@@ -136,6 +136,6 @@ def test_token_gradient_sizes_and_their_workspace():
         return lib.mtl_embedding_bwd(None, 1, n, None, 0, d, v, d, -1, 1.0, None, 0, d, 0, None, 0, None)
 
     for n, v, d, fine in ((1, 5, 8, True), ((1 << 31) - 1, 5, 256, True), ((1 << 31) - 1, 5, 257, False), (1 << 31, 5, 8, False), (1, (1 << 31) - 1, 8, False), (1, (1 << 31) - 2, 8, True),
-                          ((1 << 28) - 64, 1000, 4096, True), (1 << 28, 1000, 4096, False), (1 << 30, 5, 4096, False), (128, 5, 256 * ((1 << 25) - 1), True), (128, 5, 1 << 33, False)):
+                          ((1 << 28) - 64, 1000, 4096, True), (1 << 28, 1000, 4096, False), (1 << 30, 5, 4096, False), (128, 5, 256 * ((1 << 25) - 2), True), (128, 5, 256 * ((1 << 25) - 1), False), (128, 5, 1 << 33, False)):
         assert call(n, v, d) == (-1 if fine else -3), (n, v, d)
         assert (lib.mtl_embedding_bwd_workspace_bytes(n, v, d) > 0) == fine, (n, v, d)
